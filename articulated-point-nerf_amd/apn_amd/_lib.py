@@ -94,6 +94,16 @@ SIGNATURES = {
     "apn_cloud_bbox": (C.c_int, [P, I64, P, P, P, P]),
     "apn_idw_sum_fwd": (C.c_int, [I64, I32, P, P, P, P]),
     "apn_idw_sum_bwd": (C.c_int, [I64, I32, P, P, P, P, P, P]),
+    "apn_q8_pack": (C.c_int, [P, I32, I64, I64, I64, P, P, P]),
+    "apn_q8_unpack": (C.c_int, [P, P, I64, I64, P, I32, I64, P]),
+    "apn_q8_linear_fwd": (C.c_int, [P, I64, P, I64, P, I64, I64, I64, I32, F32, P, I64, P, P, P]),
+    "apn_q8_linear_bwd_dx": (C.c_int, [P, I64, P, F32, P, I64, I64, I64, I64, P, I64, P]),
+    "apn_q8_linear_bwd_dw_workspace_bytes": (SZ, [I64, I64, I64]),
+    "apn_q8_linear_bwd_dw": (C.c_int, [P, I64, P, F32, P, P, I64, I64, I64, P, P, P, P]),
+    "apn_q8_idw_sum_bwd": (C.c_int, [I64, I32, P, P, P, P, P, P, P]),
+    "apn_mx4_quantize": (C.c_int, [P, I32, I64, I64, I64, P, P, P]),
+    "apn_mx4_dequantize": (C.c_int, [P, P, I64, I64, P, I32, I64, P]),
+    "apn_mx4_linear": (C.c_int, [P, P, P, P, P, I64, I64, I64, I32, F32, P, I32, I64, P]),
     "apn_gemm_f32_splitk": (C.c_int, [P, P, P, P, P, I64, I64, I64, I64, I64, I32, I32, F32, I32, P, P]),
 }
 

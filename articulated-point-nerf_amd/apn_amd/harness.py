@@ -332,7 +332,9 @@ def render_viewpoints(model, render_poses, HW, Ks, ndc, render_kwargs, gt_imgs=N
             if eval_ssim:
                 ssims.append(rgb_ssim(rgb, gt_imgs[i], max_val=1))
 
-    if is_tp and in_flight > 1 and len(render_poses) > 1 and len({(int(h), int(w)) for h, w in HW}) == 1:
+    # (a feat_format frame is not captured: it renders one forward per view)
+    if is_tp and in_flight > 1 and model.feat_format is None and len(render_poses) > 1 and \
+            len({(int(h), int(w)) for h, w in HW}) == 1:
         from .pipeline import cached_pipeline
         dev = model.canonical_feat.device
         rgb_key = "rgb_marched_direct" if render_pcd_direct else "rgb_marched"

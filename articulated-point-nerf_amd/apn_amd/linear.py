@@ -14,6 +14,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import call, load, ptr, stream_ptr
+from .lowbit import sequential_q8
 
 SPLIT_ROWS = 512     # rows per split of the weight-gradient product (at least)
 SPLIT_TILES = 512    # aim: output tiles x splits of about this many workgroups (more measured slower)
@@ -133,27 +134,59 @@ def _flatten(net):
             yield m
 
 
-def sequential(net: torch.nn.Module, x: torch.Tensor, col_pos=None) -> torch.Tensor:
-    """A Sequential of Linear / LeakyReLU / ReLU (nested Sequentials flattened): each Linear runs
-    with the activation that follows it fused into its epilogue (``col_pos``: the first layer's,
-    see linear)."""
+def _layers(net):
+    """A Sequential's modules, each Linear paired with the LeakyReLU / ReLU after it: (Linear,
+    slope or None) tuples, other modules as they are."""
     mods = list(_flatten(net))
     i = 0
     while i < len(mods):
         m = mods[i]
         if isinstance(m, torch.nn.Linear):
             nxt = mods[i + 1] if i + 1 < len(mods) else None
-            cp, col_pos = col_pos, None
-            if isinstance(nxt, torch.nn.LeakyReLU):
-                x = linear(x, m, float(nxt.negative_slope), cp)
-                i += 2
-                continue
-            if isinstance(nxt, torch.nn.ReLU):
-                x = linear(x, m, 0.0, cp)
-                i += 2
-                continue
-            x = linear(x, m, None, cp)
+            slope = float(nxt.negative_slope) if isinstance(nxt, torch.nn.LeakyReLU) else \
+                0.0 if isinstance(nxt, torch.nn.ReLU) else None
+            yield m, slope
+            i += 1 if slope is None else 2
         else:
+            yield m
+            i += 1
+
+
+def layer_pairs(net: torch.nn.Module):
+    """A Sequential of Linear / LeakyReLU / ReLU only (nested ones flattened) as (Linear, slope)
+    pairs: the form lowbit.sequential_q8 and lowbit.mx4_layers take."""
+    pairs = list(_layers(net))
+    other = [type(m).__name__ for m in pairs if not isinstance(m, tuple)]
+    if other:
+        raise ValueError(f"layer_pairs: Linear with LeakyReLU / ReLU only, got {', '.join(other)}")
+    return pairs
+
+
+def sequential(net: torch.nn.Module, x: torch.Tensor, col_pos=None, checkpoint=None) -> torch.Tensor:
+    """A Sequential of Linear / LeakyReLU / ReLU (nested Sequentials flattened): each Linear runs
+    with the activation that follows it fused into its epilogue (``col_pos``: the first layer's,
+    see linear). ``checkpoint="q8"`` (device tensors under autograd): between forward and backward
+    the rows of consecutive Linear layers are kept in 8 bits (lowbit.sequential_q8) instead of
+    float32; elsewhere it changes nothing."""
+    if checkpoint not in (None, "q8"):
+        raise ValueError(f"apn linear: checkpoint must be None or 'q8', got {checkpoint!r}")
+    q8 = checkpoint == "q8" and x.is_cuda and torch.is_grad_enabled()
+    run = []   # consecutive layers of an 8-bit stack
+
+    def flush(x, col_pos):
+        if run:
+            x = sequential_q8(run, x, col_pos)
+            run.clear()
+            col_pos = None
+        return x, col_pos
+
+    for m in _layers(net):
+        if not isinstance(m, tuple):
+            x, col_pos = flush(x, col_pos)
             x = m(x)
-        i += 1
-    return x
+        elif q8:
+            run.append(m)
+        else:
+            x = linear(x, m[0], m[1], col_pos)
+            col_pos = None
+    return flush(x, col_pos)[0]

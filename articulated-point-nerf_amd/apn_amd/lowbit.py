@@ -1,0 +1,409 @@
+"""Narrow block formats for the Linear layers (apn_q8.hip, apn_mx4.hip).
+
+* q8: the 8-bit activation checkpoint. A training step of the neighbour MLP keeps every layer's
+  rows (8 per kept sample) for its backward pass; ``linear_q8`` writes a layer's f32 output and its
+  8-bit checkpoint in one pass, ``linear_q8_backward`` computes all three gradients from the
+  checkpoints, and ``sequential_q8`` is the autograd form for a stack of layers
+  (``linear.sequential(net, x, checkpoint="q8")``; ``TemporalPoints.activation_checkpoint``).
+  A kept row takes 33/128 of its f32 bytes.
+* mx4: microscaled 4-bit rows (E2M1 elements, one power-of-two scale per 32). ``mx4_linear`` is a
+  Linear layer with both operands in 4 bits, ``mx4_sequential`` a stack of them with the rows
+  between the layers in 4 bits (``TemporalPoints.feat_format``: preview renders).
+
+Both formats store a row of K values in blocks of 32 consecutive columns (include/apn_hip.h has the
+layout). A block that holds an infinity or NaN reads back as NaN, whole.
+
+Device tensors only. Rows are the last dimension; leading dimensions are flattened. Every call runs
+on the current stream of its tensors' device and allocates only through torch, so the functional
+forms (not the autograd one) can be captured into a graph.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib as L
+from ._lib import call, ptr, stream_ptr
+
+__all__ = ["Q8Rows", "q8_pack", "linear_q8", "linear_q8_backward", "sequential_q8", "MX4Rows", "mx4_quantize",
+           "mx4_linear", "MX4Layer", "mx4_layers", "mx4_sequential"]
+
+BLOCK = 32
+MAX_COLS = 1 << 20
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _blocks(k: int) -> int:
+    return -(-k // BLOCK)
+
+
+def _scale_bytes(k: int) -> int:
+    return -(-_blocks(k) // 4) * 4
+
+
+def _type(dtype, what):
+    if dtype not in _TYPES:
+        raise TypeError(f"{what}: float32, bfloat16 or float16, got {dtype}")
+    return _TYPES[dtype]
+
+
+def _same_device(what, *tensors):
+    L.require_cuda(*tensors, what=what)
+    devs = {t.device for t in tensors if t is not None}
+    if len(devs) > 1:
+        raise RuntimeError(f"{what}: tensors on different devices: {sorted(map(str, devs))}")
+
+
+def _rows(x, what):
+    """x [..., K] as a 2-D tensor with unit column stride and rows that do not overlap."""
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"{what}: expected rows of at least one column, got shape {tuple(x.shape)}")
+    if x.shape[-1] > MAX_COLS:
+        raise ValueError(f"{what}: at most {MAX_COLS} columns, got {x.shape[-1]}")
+    x2 = x.detach()
+    x2 = x2 if x2.dim() == 2 else x2.reshape(-1, x2.shape[-1])
+    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]):
+        x2 = x2.contiguous()
+    return x2
+
+
+def _ld(x2):
+    """Row stride of a _rows() tensor (a single row may report any)."""
+    return x2.stride(0) if x2.shape[0] > 1 else max(x2.stride(0), x2.shape[1])
+
+
+def _weight(w, K, what):
+    if w.dim() != 2 or w.shape[1] != K:
+        raise ValueError(f"{what}: input width {K} vs weight {tuple(w.shape)}")
+    if w.shape[0] == 0:
+        raise ValueError(f"{what}: weight without rows {tuple(w.shape)}")
+    return _rows(w, what)
+
+
+def _bias(b, N, what):
+    if b is None:
+        return None
+    if b.dim() != 1 or b.shape[0] != N:
+        raise ValueError(f"{what}: bias {tuple(b.shape)} for {N} outputs")
+    if b.dtype != torch.float32:
+        raise TypeError(f"{what}: float32 bias, got {b.dtype}")
+    return b.detach().contiguous()
+
+
+def _act(slope, what):
+    if slope is None:
+        return 0, 0.0
+    if not float("-inf") < float(slope) < float("inf"):
+        raise ValueError(f"{what}: slope must be finite, got {slope}")
+    return 1, float(slope)
+
+
+class _BlockRows:
+    """Codes and scales of [rows, cols] values; ``codes`` uint8 [rows, _BYTES ceil(cols / 32)],
+    ``scales`` uint8 [rows, 4 ceil(ceil(cols / 32) / 4)], both contiguous."""
+
+    _BYTES = 0
+
+    def __init__(self, codes, scales, cols):
+        cols = int(cols)
+        what = type(self).__name__
+        if not 1 <= cols <= MAX_COLS:
+            raise ValueError(f"{what}: 1 to {MAX_COLS} columns, got {cols}")
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError(f"{what}: uint8 codes and scales, got {codes.dtype} and {scales.dtype}")
+        want = (self._BYTES * _blocks(cols), _scale_bytes(cols))
+        if codes.dim() != 2 or scales.dim() != 2 or codes.shape[0] != scales.shape[0] or \
+                (codes.shape[1], scales.shape[1]) != want:
+            raise ValueError(f"{what}: codes [M, {want[0]}] and scales [M, {want[1]}] for {cols} columns, got "
+                             f"{tuple(codes.shape)} and {tuple(scales.shape)}")
+        if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() % 16:
+            raise ValueError(f"{what}: contiguous codes (16-byte aligned) and scales")
+        _same_device(what, codes, scales)
+        self.codes, self.scales, self.cols = codes, scales, cols
+
+    @classmethod
+    def empty(cls, rows, cols, device):
+        return cls(torch.empty(rows, cls._BYTES * _blocks(cols), dtype=torch.uint8, device=device),
+                   torch.empty(rows, _scale_bytes(cols), dtype=torch.uint8, device=device), cols)
+
+    @property
+    def shape(self):
+        return self.codes.shape[0], self.cols
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+    def _read(self, entry, dtype):
+        t = _type(dtype, f"{type(self).__name__}.dequantize")
+        M, K = self.shape
+        out = torch.empty(M, K, dtype=dtype, device=self.device)
+        with torch.cuda.device(self.device):
+            call(entry, ptr(self.codes), ptr(self.scales), M, K, ptr(out), t, K, stream_ptr(self.device))
+        return out
+
+
+class Q8Rows(_BlockRows):
+    """An 8-bit checkpoint of [rows, cols] values (``q8_pack``, ``linear_q8``)."""
+
+    _BYTES = 32
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """The values the codes stand for, [rows, cols] (exact in float32 and bfloat16)."""
+        return self._read("apn_q8_unpack", dtype)
+
+
+class MX4Rows(_BlockRows):
+    """Microscaled 4-bit rows (``mx4_quantize``)."""
+
+    _BYTES = 16
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """The values the codes stand for, [rows, cols] (exact in float32 and bfloat16)."""
+        return self._read("apn_mx4_dequantize", dtype)
+
+
+def _pack(cls, entry, x, what):
+    _same_device(what, x)
+    t = _type(x.dtype, what)
+    x2 = _rows(x, what)
+    M, K = x2.shape
+    out = cls.empty(M, K, x2.device)
+    with torch.cuda.device(x2.device):
+        call(entry, ptr(x2), t, M, K, _ld(x2), ptr(out.codes), ptr(out.scales), stream_ptr(x2.device))
+    return out
+
+
+def q8_pack(x: torch.Tensor) -> Q8Rows:
+    """The 8-bit checkpoint of x [..., K] (float32, bfloat16 or float16). Off by at most 2^-7 of the
+    largest magnitude of the value's block."""
+    return _pack(Q8Rows, "apn_q8_pack", x, "q8_pack")
+
+
+def linear_q8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, slope: float | None = None):
+    """(y, kept): y [M, N] = act(x weight^T + bias) in float32 and its 8-bit checkpoint, in one pass.
+    x [..., K] and weight [N, K] float32; ``slope``: None (no activation), 0 (ReLU) or the LeakyReLU
+    negative slope. The products are f32-accurate."""
+    what = "linear_q8"
+    _same_device(what, x, weight, bias)
+    if x.dtype != torch.float32 or weight.dtype != torch.float32:
+        raise TypeError(f"{what}: float32 only, got {x.dtype} and {weight.dtype}")
+    x2 = _rows(x, what)
+    M, K = x2.shape
+    w = _weight(weight, K, what)
+    N = w.shape[0]
+    b = _bias(bias, N, what)
+    act, sl = _act(slope, what)
+    dev = x2.device
+    y = torch.empty(M, N, device=dev)
+    kept = Q8Rows.empty(M, N, dev)
+    with torch.cuda.device(dev):
+        call("apn_q8_linear_fwd", ptr(x2), _ld(x2), ptr(w), _ld(w), ptr(b), M, N, K, act, sl, ptr(y), N,
+             ptr(kept.codes), ptr(kept.scales), stream_ptr(dev))
+    return y, kept
+
+
+def linear_q8_backward(dy: torch.Tensor, weight: torch.Tensor, x_kept: Q8Rows | None, y_kept: Q8Rows | None = None,
+                       slope: float | None = None, need=(True, True, True)):
+    """(dx, dw, db) of ``linear_q8`` from the checkpoints of its input and (with an activation) its
+    output: g = dy * (y > 0 ? 1 : slope), dx = g weight, dw = g^T x', db = sum g, with x' the
+    values of ``x_kept``. ``need``: which of the three are computed (None for the others; x_kept
+    may be None without dw). A gradient masked by slope 0 is 0 whatever dy holds there. Sums over
+    the rows are taken in a fixed order."""
+    what = "linear_q8_backward"
+    want_x, want_w, want_b = need
+    for kept, name in ((x_kept, "x_kept"), (y_kept, "y_kept")):
+        if kept is not None and not isinstance(kept, Q8Rows):
+            raise TypeError(f"{what}: {name} must be Q8Rows, got {type(kept).__name__}")
+    _same_device(what, dy, weight, *[k.codes for k in (x_kept, y_kept) if k is not None])
+    if dy.dtype != torch.float32 or weight.dtype != torch.float32:
+        raise TypeError(f"{what}: float32 only, got {dy.dtype} and {weight.dtype}")
+    dy = _rows(dy, what)
+    M, N = dy.shape
+    if weight.dim() != 2 or weight.shape[0] != N:
+        raise ValueError(f"{what}: gradient width {N} vs weight {tuple(weight.shape)}")
+    w = _rows(weight, what)
+    K = w.shape[1]
+    if want_w and x_kept is None:
+        raise ValueError(f"{what}: dw needs x_kept")
+    if x_kept is not None and x_kept.shape != (M, K):
+        raise ValueError(f"{what}: x_kept is {x_kept.shape}, expected {(M, K)}")
+    _, sl = _act(slope, what)
+    mask = None
+    if slope is not None:
+        if y_kept is None:
+            raise ValueError(f"{what}: an activation needs y_kept")
+        mask = y_kept.codes
+    if y_kept is not None and y_kept.shape != (M, N):
+        raise ValueError(f"{what}: y_kept is {y_kept.shape}, expected {(M, N)}")
+    dev = dy.device
+    dx = dw = db = None
+    with torch.cuda.device(dev):
+        s = stream_ptr(dev)
+        if want_x:
+            dx = torch.empty(M, K, device=dev)
+            call("apn_q8_linear_bwd_dx", ptr(dy), _ld(dy), ptr(mask), sl, ptr(w), _ld(w), M, N, K, ptr(dx), K, s)
+        if want_w or want_b:
+            dw = torch.empty(N, K, device=dev) if want_w else None
+            db = torch.empty(N, device=dev) if want_b else None
+            nbytes = int(L.load().apn_q8_linear_bwd_dw_workspace_bytes(M, N, K))
+            ws = torch.empty(max(nbytes // 4, 1), device=dev)
+            xk = (x_kept.codes, x_kept.scales) if want_w else (None, None)
+            call("apn_q8_linear_bwd_dw", ptr(dy), _ld(dy), ptr(mask), sl, ptr(xk[0]), ptr(xk[1]), M, N, K, ptr(dw),
+                 ptr(db), ptr(ws), s)
+    return dx, dw, db
+
+
+class _Q8Stack(torch.autograd.Function):
+    """A stack of Linear layers: f32 forward, everything the backward needs kept in 8 bits (the
+    stack's input and each layer's output, once)."""
+
+    @staticmethod
+    def forward(ctx, x, slopes, col_pos, holder, *params):
+        weights, biases = params[0::2], params[1::2]
+        lead = x.shape[:-1]
+        h = x.reshape(-1, x.shape[-1])
+        x0 = q8_pack(h) if weights[0].requires_grad else None
+        ws, kept = [], []
+        for i, (w, b, slope) in enumerate(zip(weights, biases, slopes)):
+            w = w.detach()
+            if i == 0 and col_pos is not None:   # x holds weight column j at column col_pos[j]
+                wide = torch.zeros(w.shape[0], -(-h.shape[1] // 4) * 4, device=w.device, dtype=w.dtype)
+                wide[:, col_pos] = w
+                w = wide[:, :h.shape[1]]
+            h, k = linear_q8(h, w, b, slope)
+            ws.append(w)
+            kept.append(k)
+        ctx.slopes, ctx.col_pos, ctx.in_shape, ctx.cols = slopes, col_pos, x.shape, [k.cols for k in kept]
+        flat = [t for k in kept for t in (k.codes, k.scales)]
+        ctx.save_for_backward(*(p for p in weights), *ws, *(() if x0 is None else (x0.codes, x0.scales)), *flat)
+        ctx.has_x0 = x0 is not None
+        if holder is not None:
+            holder.append(kept[-1])
+        return h.reshape(*lead, h.shape[-1])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        n = len(ctx.slopes)
+        saved = ctx.saved_tensors
+        ws, rest = saved[n:2 * n], saved[2 * n:]
+        x0 = None
+        if ctx.has_x0:
+            x0, rest = Q8Rows(rest[0], rest[1], ctx.in_shape[-1]), rest[2:]
+        kept = [Q8Rows(rest[2 * i], rest[2 * i + 1], ctx.cols[i]) for i in range(n)]
+        need = ctx.needs_input_grad
+        grads = [None] * (2 * n)
+        g = dy.reshape(-1, dy.shape[-1])
+        dx = None
+        for i in reversed(range(n)):
+            below = need[0] if i == 0 else need[0] or any(need[4:4 + 2 * i])
+            nw, nb = need[4 + 2 * i], need[5 + 2 * i]
+            dx, dw, db = linear_q8_backward(g, ws[i], x0 if i == 0 else kept[i - 1], kept[i], ctx.slopes[i],
+                                            (below, nw, nb))
+            if i == 0 and ctx.col_pos is not None and dw is not None:
+                dw = dw[:, ctx.col_pos]
+            grads[2 * i], grads[2 * i + 1] = dw, db
+            if not below:
+                break
+            g = dx
+        return (dx.reshape(ctx.in_shape) if need[0] else None, None, None, None, *grads)
+
+
+def sequential_q8(layers, x: torch.Tensor, col_pos=None, keep_output=False):
+    """A stack of (torch.nn.Linear, slope) pairs under autograd with 8-bit activation checkpoints:
+    between forward and backward no float row of the stack is kept, only the 8-bit checkpoint of x
+    and of each layer's output. ``col_pos``: linear.linear's. With ``keep_output`` returns
+    (y, Q8Rows of y).
+
+    Not under graph capture: a captured backward reaches the parameters' gradient accumulators, and
+    one that an eager step created earlier on another stream ends the capture and with it the
+    process; capture linear_q8 / linear_q8_backward instead."""
+    what = "sequential_q8"
+    layers = list(layers)
+    if not layers:
+        raise ValueError(f"{what}: no layers")
+    L.require_cuda(x, what=what)
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what}: autograd steps cannot be captured; capture linear_q8 / linear_q8_backward")
+    params = [p for layer, _ in layers for p in (layer.weight, layer.bias)]
+    holder = [] if keep_output else None
+    y = _Q8Stack.apply(x, tuple(s for _, s in layers), col_pos, holder, *params)
+    return (y, holder[0]) if keep_output else y
+
+
+# --- 4-bit rows -----------------------------------------------------------------------------------
+
+def mx4_quantize(x: torch.Tensor) -> MX4Rows:
+    """x [..., K] (float32, bfloat16 or float16) as microscaled 4-bit rows."""
+    return _pack(MX4Rows, "apn_mx4_quantize", x, "mx4_quantize")
+
+
+def mx4_linear(x, weight: MX4Rows, bias: torch.Tensor | None = None, slope: float | None = None,
+               out_dtype=torch.float32) -> torch.Tensor:
+    """act(mx4(x) weight^T + bias) as [M, N] of ``out_dtype`` (float32, bfloat16, float16): exact
+    4-bit products, float32 sums. x: MX4Rows, or a float tensor [..., K] that is quantized first."""
+    what = "mx4_linear"
+    if not isinstance(weight, MX4Rows):
+        raise TypeError(f"{what}: weight must be MX4Rows, got {type(weight).__name__}")
+    t = _type(out_dtype, what)
+    if not isinstance(x, MX4Rows):
+        _same_device(what, x, weight.codes)
+        if x.dim() and x.shape[-1] != weight.cols:
+            raise ValueError(f"{what}: input width {x.shape[-1]} vs weight {weight.shape}")
+        x = mx4_quantize(x)
+    if x.cols != weight.cols:
+        raise ValueError(f"{what}: input width {x.cols} vs weight {weight.shape}")
+    _same_device(what, x.codes, weight.codes, bias)
+    (M, K), N = x.shape, weight.shape[0]
+    if N == 0:
+        raise ValueError(f"{what}: weight without rows {weight.shape}")
+    b = _bias(bias, N, what)
+    act, sl = _act(slope, what)
+    dev = x.device
+    out = torch.empty(M, N, dtype=out_dtype, device=dev)
+    with torch.cuda.device(dev):
+        call("apn_mx4_linear", ptr(x.codes), ptr(x.scales), ptr(weight.codes), ptr(weight.scales), ptr(b), M, N, K, act,
+             sl, ptr(out), t, N, stream_ptr(dev))
+    return out
+
+
+class MX4Layer:
+    """A frozen Linear layer: 4-bit weight rows, float32 bias, activation slope (None: none)."""
+
+    def __init__(self, weight: MX4Rows, bias: torch.Tensor | None = None, slope: float | None = None):
+        if not isinstance(weight, MX4Rows):
+            raise TypeError(f"MX4Layer: weight must be MX4Rows, got {type(weight).__name__}")
+        _same_device("MX4Layer", weight.codes, bias)
+        self.weight, self.slope = weight, slope
+        self.bias = _bias(bias, weight.shape[0], "MX4Layer")
+        _act(slope, "MX4Layer")
+
+
+def mx4_layers(layers, col_pos=None, width=None):
+    """(torch.nn.Linear, slope) pairs as MX4Layers, their weights quantized once. ``col_pos``
+    (int64 [in_features]) with ``width``: the stack's input rows are ``width`` wide and hold input j
+    at column col_pos[j] (linear.linear's)."""
+    out = []
+    for i, (layer, slope) in enumerate(layers):
+        w = layer.weight.detach()
+        if i == 0 and col_pos is not None:
+            wide = torch.zeros(w.shape[0], int(width), device=w.device, dtype=w.dtype)
+            wide[:, col_pos] = w
+            w = wide
+        out.append(MX4Layer(mx4_quantize(w), layer.bias, slope))
+    return out
+
+
+def mx4_sequential(layers, x: torch.Tensor, out_dtype=torch.float32) -> torch.Tensor:
+    """A stack of MX4Layers on x [..., K]; the rows between the layers are 4-bit. Returns [M, N]."""
+    layers = list(layers)
+    if not layers:
+        raise ValueError("mx4_sequential: no layers")
+    h = x
+    for layer in layers[:-1]:
+        h = mx4_linear(h, layer.weight, layer.bias, layer.slope)
+    return mx4_linear(h, layers[-1].weight, layers[-1].bias, layers[-1].slope, out_dtype=out_dtype)

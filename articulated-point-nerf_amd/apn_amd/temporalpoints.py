@@ -345,6 +345,12 @@ class TemporalPoints(torch.nn.Module):
         # the neighbour MLP only on the kept samples the compositing reads (apn_point_mlp_ert: every
         # ray's samples up to its T < 1e-3 break, in passes); the frame is bit-identical either way
         self.early_termination = ERT
+        # "q8": a training step keeps feat_net's rows for its backward pass in 8 bits (apn_amd.lowbit:
+        # 0.26 of the float32 bytes); None: in float32
+        self.activation_checkpoint = None
+        # "mx4": frames without autograd run feat_net on 4-bit rows and weights, on the generic path
+        # (a preview: not within the fused frame's accuracy); None: float32
+        self.feat_format = None
         self.last_mlp_rows = None   # device int32 [ERT_PASSES]: samples per early-termination pass of the last frame
 
     # view_poc / pos_poc alias the TiNeuVox buffers (temporalpoints.py:148-150); as properties
@@ -1002,11 +1008,11 @@ class TemporalPoints(torch.nn.Module):
         # feat_depth != 4 (temporalpoints.py:53, 117-130): the fused MLP kernel is built for the
         # reference default; other depths render through the generic GPU path (HIP skinning / kNN /
         # loss kernels, the layers as GEMMs), the same code as the differentiable step
-        generic = len(self.feat_net) != 6
+        generic = len(self.feat_net) != 6 or self.feat_format is not None
         if torch.is_grad_enabled() or generic:
             if ray_shard is not None:
                 raise NotImplementedError("ray_shard is a render-path option of the fused pipeline "
-                                          "(torch.no_grad(), feat_depth=4)")
+                                          "(torch.no_grad(), feat_depth=4, feat_format=None)")
             from .train import forward_train
             return forward_train(self, t, render_depth, render_kwargs, query_radius, render_weights, rot_params,
                                  poses, Ks, calc_min_max, get_skeleton)
@@ -1016,6 +1022,8 @@ class TemporalPoints(torch.nn.Module):
 
     def _forward_render(self, t, render_depth, render_kwargs, query_radius, render_weights, rot_params, poses, Ks,
                         calc_min_max, get_skeleton, ray_shard):
+        if self.feat_format is not None:   # a captured or sharded frame would not be in that format
+            raise NotImplementedError("feat_format is a generic-path option: render with forward()")
         dev = self.canonical_feat.device
         L.require_cuda(self.canonical_feat, what="TemporalPoints.forward")
         self._last_ray_ws = None

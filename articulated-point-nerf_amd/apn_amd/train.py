@@ -26,13 +26,14 @@ import torch
 
 from . import _lib as L
 from . import linear as LIN
+from . import lowbit as LB
 from ._lib import call, ptr, stream_ptr
 from .ops import Alphas2Weights, Raw2Alpha
 from .tineuvox import poc_fre
 
 __all__ = ["forward_train", "LBSTrain", "lbs_train", "lbs_blend", "inv3x3", "radius_knn", "ordered_bbox",
            "reverse_csr", "NbrTVLoss", "ArapLoss",
-           "feat_net_forward", "SparsityLoss"]
+           "feat_net_forward", "neighbour_features", "IdwSumQ8", "SparsityLoss"]
 
 
 def cloud_min_max(xyz: torch.Tensor):
@@ -253,6 +254,34 @@ class IdwSum(torch.autograd.Function):
         return d_w, d_out
 
 
+class IdwSumQ8(torch.autograd.Function):
+    """IdwSum whose backward reads the rows from their 8-bit checkpoint (apn_q8_idw_sum_bwd): out
+    itself is not kept."""
+
+    @staticmethod
+    def forward(ctx, w, out, kept):
+        S, C = w.shape[0], out.shape[-1]
+        w, out = w.contiguous(), out.reshape(S * 8, C).contiguous()
+        if kept.shape != (S * 8, C):
+            raise ValueError(f"IdwSumQ8: checkpoint of {kept.shape} rows for {(S * 8, C)}")
+        h = torch.empty(S, C, device=out.device)
+        call("apn_idw_sum_fwd", S, C, ptr(w), ptr(out), ptr(h), stream_ptr(out.device))
+        ctx.save_for_backward(w, kept.codes, kept.scales)
+        ctx.cols = C
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        w, codes, scales = ctx.saved_tensors
+        S, C = w.shape[0], ctx.cols
+        d_out = torch.empty(S * 8, C, device=w.device) if ctx.needs_input_grad[1] else None
+        d_w = torch.empty_like(w) if ctx.needs_input_grad[0] else None
+        call("apn_q8_idw_sum_bwd", S, C, ptr(w), ptr(codes), ptr(scales), ptr(dh.contiguous()), ptr(d_out), ptr(d_w),
+             stream_ptr(w.device))
+        return d_w, d_out, None
+
+
 class NbrTVLoss(torch.autograd.Function):
     """get_neighbour_weight_tv_loss (temporalpoints.py:714-716): mean |w_i - w_nn(i,k)| over
     [N,K,J] as one fused HIP edge reduction (apn_nbr_tv_loss); backward apn_nbr_tv_loss_backward
@@ -365,6 +394,25 @@ def lbs_train(model, bone_Ts, global_t, identity_rules=None):
     weights = model.get_weights()
     xyz, G = lbs_blend(model.forward_warp.canonical_pcd, weights, bone_Ts, global_t)
     return xyz, inv3x3(G[:, :, :3]), weights
+
+
+def neighbour_features(model, feat_in, w, cols):
+    """feat_net on the neighbour rows and their IDW sum (temporalpoints.py:491-494). Under autograd
+    with ``model.activation_checkpoint == "q8"`` the rows are kept in 8 bits; without autograd and
+    with ``model.feat_format == "mx4"`` the network runs on 4-bit rows and weights."""
+    if torch.is_grad_enabled():
+        if model.activation_checkpoint == "q8":
+            out, kept = LB.sequential_q8(LIN.layer_pairs(model.feat_net), feat_in, cols, keep_output=True)
+            return IdwSumQ8.apply(w, out, kept)
+        if model.activation_checkpoint is not None:
+            raise ValueError(f"activation_checkpoint must be None or 'q8', got {model.activation_checkpoint!r}")
+    elif model.feat_format is not None:
+        if model.feat_format != "mx4":
+            raise ValueError(f"feat_format must be None or 'mx4', got {model.feat_format!r}")
+        # the weights (0.3 MB) are quantized per frame: nothing to go stale when they change
+        layers = LB.mx4_layers(LIN.layer_pairs(model.feat_net), cols, feat_in.shape[-1])
+        return IdwSum.apply(w, LB.mx4_sequential(layers, feat_in))
+    return IdwSum.apply(w, LIN.sequential(model.feat_net, feat_in, col_pos=cols))
 
 
 # The warp stage of a training step -- skeleton (TransformNet, Rodrigues, masks, the kinematic
@@ -640,8 +688,7 @@ def forward_train(model, t, render_depth=False, render_kwargs=None, query_radius
         model.canonical_alpha.clip(0, 1), model.pos_poc, model._eps)
     cols = feat_in_columns(model.pos_poc.numel(), model.canonical_feat.shape[1],
                            pose_embedding.shape[-1] if pose_embedding is not None else 0, dev)
-    out = LIN.sequential(model.feat_net, feat_in, col_pos=cols)
-    h = IdwSum.apply(w, out)   # 493-494
+    h = neighbour_features(model, feat_in, w, cols)
     w = w.unsqueeze(-1)
     # heads (496-515)
     density = LIN.linear(h, model.densitynet).squeeze(-1)

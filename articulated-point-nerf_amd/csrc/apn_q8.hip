@@ -1,0 +1,587 @@
+// 8-bit activation checkpoints of the training step's Linear layers (apn_lowbit.h: the format) and
+// the products that write and read them:
+//   pack / unpack      rows of a float matrix <-> codes and scales
+//   linear forward     Y = act(X W^T + b), and q8(Y) written by the epilogue
+//   linear backward    G = dY * (code of Y positive ? 1 : slope);  dX = G W;
+//                      dW = G^T X', db = sum_m G with X' the checkpoint of X
+//   IDW-sum backward   d_out = w dh, d_w = <out', dh> with out' the checkpoint of the rows
+//
+// f32 products on the bf16 matrix units: every f32 factor is cut (not rounded) into three bf16
+// numbers hi + mid + lo whose 3 x 8 mantissa bits are its 24 exactly, and
+//   x w = hi hi + (hi mid + mid hi) + (hi lo + mid mid + lo hi) + (<= 2^-22 |x w|, left out)
+// with f32 accumulation: six bf16 products, 2.5 PFLOP/s / 6 = 416 TFLOP/s against 157 of the
+// f32-input MFMA. A checkpoint factor q 2^s is one exact bf16 number, so dW takes three. Values
+// below 2^-110 lose mantissa bits to bf16's smallest subnormal (2^-133, absolute). An infinity
+// makes its row's outputs NaN (inf - inf in the cut, inf * 0 in the products): non-finite stays
+// non-finite.
+#include "apn_lowbit.h"
+
+#include <algorithm>
+
+namespace apn {
+namespace q8 {
+using namespace lb;
+
+// --- pack / unpack ---------------------------------------------------------------------------
+// One thread per 8 consecutive columns, 4 threads per block: the block maximum is two lane
+// exchanges; 32 B (f32) in and 8 B out per thread, consecutive threads on consecutive columns.
+// Bound by memory.
+template <int T>
+__global__ __launch_bounds__(256) void k_pack(const typename Elem<T>::type* __restrict__ x, uint32_t units, int K,
+                                              int64_t ldx, int vec, FastDiv upr, uint8_t* __restrict__ codes,
+                                              uint8_t* __restrict__ scales, int ss) {
+  const uint32_t u = blockIdx.x * 256u + threadIdx.x;
+  const bool live = u < units;
+  const uint32_t m = div_by(min(u, units - 1), upr), cu = min(u, units - 1) - m * upr.d;
+  const int c = (int)cu * 8;
+  const int n = min(8, K - c);   // <= 0 in the padding of the last block
+  float v[8];
+  load8<T>(x + (int64_t)m * ldx + c, n, vec && n == 8, v);
+  uint32_t a = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a = max(a, abs_bits(v[j]));
+  a = max(a, (uint32_t)__shfl_xor((int)a, 1));
+  a = max(a, (uint32_t)__shfl_xor((int)a, 2));
+  const int byte = q8_byte(a);
+  const float inv = inv_pow2_of(byte);
+  u32x2 w = {0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j >> 2] |= q8_code(v[j], inv) << (8 * (j & 3));
+  if (!live) return;
+  *(u32x2*)(codes + (int64_t)m * (8 * upr.d) + c) = w;
+  if ((cu & 3) == 0) {
+    uint8_t* s = scales + (int64_t)m * ss;
+    s[cu >> 2] = (uint8_t)byte;
+    if (cu + 4 == upr.d)
+      for (int i = (int)(cu >> 2) + 1; i < ss; ++i) s[i] = 0;
+  }
+}
+
+template <int T>
+__global__ __launch_bounds__(256) void k_unpack(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                uint32_t units, int K, FastDiv upr, int ss,
+                                                typename Elem<T>::type* __restrict__ out, int64_t ldo, int vec) {
+  const uint32_t u = blockIdx.x * 256u + threadIdx.x;
+  if (u >= units) return;
+  const uint32_t m = div_by(u, upr), cu = u - m * upr.d;
+  const int c = (int)cu * 8, n = min(8, K - c);
+  if (n <= 0) return;
+  const u32x2 w = *(const u32x2*)(codes + (int64_t)m * (8 * upr.d) + c);
+  const float sc = pow2_of(scales[(int64_t)m * ss + (cu >> 2)]);
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = q8_value((w[j >> 2] >> (8 * (j & 3))) & 0xffu, sc);
+  store8<T>(out + (int64_t)m * ldo + c, n, vec && n == 8, v);
+}
+
+// --- f32 products on bf16 matrix units -------------------------------------------------------
+
+// 8 floats as three bf16 octets, cut after 8 mantissa bits each
+__device__ __forceinline__ void cut3(const float (&v)[8], u32x4& hi, u32x4& mid, u32x4& lo) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = v[2 * j], b = v[2 * j + 1];
+    const float ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+    const float rb = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+    const float sa = ra - __uint_as_float(__float_as_uint(ra) & 0xffff0000u);
+    const float sb = rb - __uint_as_float(__float_as_uint(rb) & 0xffff0000u);
+    hi[j] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    mid[j] = __builtin_amdgcn_perm(__float_as_uint(rb), __float_as_uint(ra), 0x07060302u);
+    lo[j] = __builtin_amdgcn_perm(__float_as_uint(sb), __float_as_uint(sa), 0x07060302u);
+  }
+}
+__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                 0);
+}
+
+// Rows kernel: out[m][c] = sum_r in[m][r] Wop[c][r], the forward (r = input column, c = output
+// column) and dX (r = output column, c = input column, Wop = W^T, `in` masked by Y's signs).
+// 64 rows x 128 columns per 256-thread workgroup. The matrix operands are swapped -- A = W's rows,
+// B = the data rows -- so a lane's 16 results of a 32 x 32 tile are 16 of the 32 columns of ONE
+// data row (columns 8 j + 4 h + i; the other half in lane ^ 32), which makes the q8 block maximum
+// 15 in-lane maxima and one exchange. Data rows are staged through LDS once per workgroup, cut
+// into their three planes, in fragment order: 16-B piece (plane, k step, row tile, half, row), the
+// row slot xor-ed with the 8-column unit so that the 8 lanes which write one row's units and the
+// 8 lanes which read neighbouring rows both meet all 8 bank groups.
+constexpr int BM = 64, BC = 128, BR = 64;   // rows, columns, reduction per staged chunk
+
+struct RowArgs {
+  const float* in;
+  const uint8_t* mask;   // codes of Y beside `in`, or null
+  const float* w;
+  const float* bias;
+  float* out;
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t M, ld_in, ld_mask, ldw, ld_out, ld_codes;
+  int R, C, ss, act, vec_in, vec_out;
+  float slope;
+};
+
+template <bool WT>   // WT: W stored [r][c], else [c][r]
+__device__ __forceinline__ void load_w(const RowArgs& p, int c, int r, float (&v)[8]) {
+  if (c < p.C && r + 8 <= p.R) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = WT ? p.w[(int64_t)(r + j) * p.ldw + c] : p.w[(int64_t)c * p.ldw + r + j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = c < p.C && r + j < p.R ? (WT ? p.w[(int64_t)(r + j) * p.ldw + c] : p.w[(int64_t)c * p.ldw + r + j]) : 0.f;
+  }
+}
+
+template <bool WT, bool MASK, bool Q8>
+__global__ __launch_bounds__(256, 2) void k_rows(RowArgs p) {
+  __shared__ u32x4 sh[3 * 4 * 2 * 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int l = lane & 31, h = lane >> 5;
+  const int c0 = blockIdx.y * BC + wave * 32;
+  for (int64_t m0 = (int64_t)blockIdx.x * BM; m0 < p.M; m0 += (int64_t)gridDim.x * BM) {
+    f32x16 acc[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
+    for (int r0 = 0; r0 < p.R; r0 += BR) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {   // 64 rows x 8 units of 8 columns, two per thread
+        const int f = tid + 256 * i, row = f >> 3, u = f & 7;
+        const int64_t m = m0 + row;
+        const int r = r0 + 8 * u, n = m < p.M ? min(8, p.R - r) : 0;
+        float v[8];
+        load8<APN_F32>(p.in + m * p.ld_in + r, n, p.vec_in && n == 8, v);
+        if (MASK && n > 0) {
+          const u32x2 s = *(const u32x2*)(p.mask + m * p.ld_mask + r);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if ((s[j >> 2] >> (8 * (j & 3))) & 0x80u) v[j] = p.slope == 0.f ? 0.f : v[j] * p.slope;
+        }
+        u32x4 a, b, c;
+        cut3(v, a, b, c);
+        const int at = (u >> 1) * 128 + (row >> 5) * 64 + (u & 1) * 32 + ((row & 31) ^ u);
+        sh[at] = a, sh[512 + at] = b, sh[1024 + at] = c;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        if (r0 + 16 * ks >= p.R) break;
+        float wv[8];
+        load_w<WT>(p, c0 + l, r0 + 16 * ks + 8 * h, wv);
+        u32x4 wh, wm, wl;
+        cut3(wv, wh, wm, wl);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int at = ks * 128 + t * 64 + h * 32 + (l ^ (2 * ks + h));
+          const u32x4 xh = sh[at], xm = sh[512 + at], xl = sh[1024 + at];
+          f32x16 a = acc[t];
+          a = mma(wl, xh, a), a = mma(wh, xl, a), a = mma(wm, xm, a);
+          a = mma(wm, xh, a), a = mma(wh, xm, a), a = mma(wh, xh, a);
+          acc[t] = a;
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int64_t m = m0 + 32 * t + l;
+      if (c0 >= p.C) continue;   // uniform in the wave
+      float y[16];
+      uint32_t amax = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int c = c0 + 8 * (i >> 2) + 4 * h + (i & 3);
+        float v = acc[t][i];
+        if (p.bias && c < p.C) v += p.bias[c];
+        if (p.act) v = leaky(v, p.slope);
+        if (Q8 && c >= p.C) v = 0.f;
+        y[i] = v;
+        if (Q8) amax = max(amax, abs_bits(v));
+      }
+      if (m < p.M) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = c0 + 8 * j + 4 * h;
+          float* o = p.out + m * p.ld_out + c;
+          if (p.vec_out && c + 4 <= p.C) {
+            *(f32x4*)o = f32x4{y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]};
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (c + i < p.C) o[i] = y[4 * j + i];
+          }
+        }
+      }
+      if (Q8) {
+        amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
+        const int byte = q8_byte(amax);
+        const float inv = inv_pow2_of(byte);
+        if (m < p.M) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w |= q8_code(y[4 * j + i], inv) << (8 * i);
+            *(uint32_t*)(p.codes + m * p.ld_codes + c0 + 8 * j + 4 * h) = w;
+          }
+          if (h == 0) {
+            uint8_t* s = p.scales + m * p.ss;
+            s[c0 >> 5] = (uint8_t)byte;
+            if (c0 + 32 >= p.C)
+              for (int i = (c0 >> 5) + 1; i < p.ss; ++i) s[i] = 0;
+          }
+        }
+      }
+    }
+  }
+}
+
+// Weight gradient: dW[n][k] = sum_m G[m][n] X'[m][k], db[n] = sum_m G[m][n], 128 x 128 outputs per
+// workgroup, wave (i, j) its 64 x 64 quarter, the rows in chunks of 64 over the splits (blockIdx.z
+// takes every splits-th chunk), partial sums to the workspace and added in a fixed order. Both
+// operands need 8 consecutive rows m per lane: a thread reads 4 columns of 8 rows and writes the
+// four 8-row pieces in fragment order, column slots xor-ed with bits 3..4 of the column so that
+// the writing lanes (4 columns apart) meet all bank groups.
+struct DwArgs {
+  const float* dy;
+  const uint8_t* mask;
+  const uint8_t* xc;
+  const uint8_t* xs;
+  float* dw;        // [splits][N][K]
+  float* db;        // [splits][N] or null
+  int64_t M, ld_dy, ld_mask, ld_xc;
+  int N, K, ss, splits, vec_dy;
+  float slope;
+};
+
+__device__ __forceinline__ int slot32(int c) { return (c & 31) ^ ((c >> 3) & 3); }
+
+__global__ __launch_bounds__(256, 2) void k_dw(DwArgs p) {
+  __shared__ u32x4 sg[3 * 4 * 4 * 64];   // [plane][k step][column tile][half, slot]
+  __shared__ u32x4 sx[4 * 4 * 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int l = lane & 31, h = lane >> 5;
+  const int n0 = blockIdx.x * 128, k0 = blockIdx.y * 128;
+  const int cq = tid & 31, mo = tid >> 5;   // this thread's 4 columns 4 cq .. and 8 rows 8 mo ..
+  const int gc = n0 + 4 * cq, xk = k0 + 4 * cq;
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
+  float bs[4] = {0.f, 0.f, 0.f, 0.f};
+  const int64_t chunks = (p.M + 63) / 64;
+  for (int64_t ch = blockIdx.z; ch < chunks; ch += p.splits) {
+    const int64_t m0 = ch * 64 + 8 * mo;
+    float g[4][8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t m = m0 + j;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t s = 0;
+      if (m < p.M && gc < p.N) {
+        const float* q = p.dy + m * p.ld_dy + gc;
+        if (p.vec_dy && gc + 4 <= p.N) {
+          const f32x4 a = *(const f32x4*)q;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] = a[c];
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] = gc + c < p.N ? q[c] : 0.f;
+        }
+        if (p.mask) s = *(const uint32_t*)(p.mask + m * p.ld_mask + gc);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if ((s >> (8 * c)) & 0x80u) v[c] = p.slope == 0.f ? 0.f : v[c] * p.slope;
+        g[c][j] = v[c];
+        bs[c] += v[c];
+      }
+    }
+    uint32_t xw[8];
+    float xsc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t m = m0 + j;
+      const bool in = m < p.M && xk < p.K;
+      xw[j] = in ? *(const uint32_t*)(p.xc + m * p.ld_xc + xk) : 0u;
+      xsc[j] = in ? pow2_of(p.xs[m * p.ss + (xk >> 5)]) : 0.f;
+    }
+    __syncthreads();   // the previous chunk's operand reads are done
+    const int at = (mo >> 1) * 256 + (cq >> 3) * 64 + (mo & 1) * 32;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      u32x4 a, b, d;
+      cut3(g[c], a, b, d);
+      const int s = at + slot32(4 * cq + c);
+      sg[s] = a, sg[1024 + s] = b, sg[2048 + s] = d;
+      u32x4 x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {   // q 2^s is exact in the upper 16 bits
+        const float e = q8_value((xw[2 * j] >> (8 * c)) & 0xffu, xsc[2 * j]);
+        const float o = q8_value((xw[2 * j + 1] >> (8 * c)) & 0xffu, xsc[2 * j + 1]);
+        x[j] = __builtin_amdgcn_perm(__float_as_uint(o), __float_as_uint(e), 0x07060302u);
+      }
+      sx[s] = x;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      u32x4 xf[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int t = (wave & 1) * 2 + b;
+        xf[b] = sx[ks * 256 + t * 64 + h * 32 + slot32(l)];
+      }
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const int t = (wave >> 1) * 2 + a;
+        const int s = ks * 256 + t * 64 + h * 32 + slot32(l);
+        const u32x4 gh = sg[s], gm = sg[1024 + s], gl = sg[2048 + s];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          f32x16 c = acc[a][b];
+          c = mma(gl, xf[b], c), c = mma(gm, xf[b], c), c = mma(gh, xf[b], c);
+          acc[a][b] = c;
+        }
+      }
+    }
+  }
+  float* dw = p.dw + (int64_t)blockIdx.z * p.N * p.K;
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int k = k0 + (wave & 1) * 64 + b * 32 + l;
+      if (k >= p.K) continue;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int n = n0 + (wave >> 1) * 64 + a * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
+        if (n < p.N) dw[(int64_t)n * p.K + k] = acc[a][b][i];
+      }
+    }
+  if (p.db && blockIdx.y == 0) {   // 8 row octets per column, added in a fixed order
+    __syncthreads();
+    float* red = (float*)sx;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) red[mo * 128 + 4 * cq + c] = bs[c];
+    __syncthreads();
+    if (tid < 128 && n0 + tid < p.N) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += red[j * 128 + tid];
+      p.db[(int64_t)blockIdx.z * p.N + n0 + tid] = s;
+    }
+  }
+}
+
+// out[o] = sum_z part[z * n + o], 8 lanes per output each every 8th split, then a fixed tree
+__global__ __launch_bounds__(256) void k_add_splits(const float* __restrict__ part, int splits, int64_t n,
+                                                    float* __restrict__ out) {
+  const int z0 = threadIdx.x & 7;
+  for (int64_t o = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 3; o < n; o += (int64_t)gridDim.x * 32) {
+    float s = 0.f;
+#pragma unroll 4
+    for (int z = z0; z < splits; z += 8) s += part[(int64_t)z * n + o];
+    s += __shfl_xor(s, 1, 8);
+    s += __shfl_xor(s, 2, 8);
+    s += __shfl_xor(s, 4, 8);
+    if (z0 == 0) out[o] = s;
+  }
+}
+
+// Backward of h[s] = sum_k w[s,k] out[8s+k]: one wave per sample; lane = (row k, column eighth):
+// each lane walks its row's columns 4 at a time in steps of 32, so 8 lanes cover a block.
+__global__ __launch_bounds__(256) void k_idw_bwd(int64_t S, int C, const float* __restrict__ w,
+                                                 const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                 int64_t ldc, int ss, const float* __restrict__ dh,
+                                                 float* __restrict__ d_out, float* __restrict__ d_w, int vec) {
+  const int lane = threadIdx.x & 63, k = lane >> 3, q = lane & 7;
+  for (int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); s < S; s += (int64_t)gridDim.x * 4) {
+  const int64_t row = 8 * s + k;
+  const float wk = w[row];
+  float dot = 0.f;
+  for (int c = 4 * q; c < C; c += 32) {
+    float g[4];
+    if (vec) {
+      const f32x4 a = *(const f32x4*)(dh + s * C + c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[j] = a[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[j] = c + j < C ? dh[s * C + c + j] : 0.f;
+    }
+    if (d_w) {
+      const uint32_t x = *(const uint32_t*)(codes + row * ldc + c);
+      const float sc = pow2_of(scales[row * ss + (c >> 5)]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < C) dot = fmaf(q8_value((x >> (8 * j)) & 0xffu, sc), g[j], dot);
+    }
+    if (d_out) {
+      float* o = d_out + row * C + c;
+      if (vec) {
+        *(f32x4*)o = f32x4{wk * g[0], wk * g[1], wk * g[2], wk * g[3]};
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c + j < C) o[j] = wk * g[j];
+      }
+    }
+  }
+  dot += __shfl_xor(dot, 1);
+  dot += __shfl_xor(dot, 2);
+  dot += __shfl_xor(dot, 4);
+  if (d_w && q == 0) d_w[row] = dot;
+  }
+}
+
+// rows per launch of the unit kernels, so that units (and their thread indices) stay below 2^31
+inline int64_t row_piece(int64_t upr) { return std::max<int64_t>(1, ((int64_t)1 << 30) / upr); }
+
+template <int T>
+int pack(const void* x, int64_t M, int64_t K, int64_t ldx, uint8_t* codes, uint8_t* scales, hipStream_t s) {
+  typedef typename Elem<T>::type E;
+  const int64_t upr = blocks_of(K) * 4, ss = scale_stride(K), piece = row_piece(upr);
+  for (int64_t m = 0; m < M; m += piece) {
+    const int64_t rows = std::min(piece, M - m), units = rows * upr;
+    const E* p = (const E*)x + m * ldx;
+    hipLaunchKernelGGL((k_pack<T>), dim3((unsigned)ceil_div(units, 256)), dim3(256), 0, s, p, (uint32_t)units, (int)K,
+                       ldx, (int)vec_rows(p, ldx, T), fast_div((uint32_t)upr), codes + m * upr * 8, scales + m * ss,
+                       (int)ss);
+  }
+  return launch_status();
+}
+
+template <int T>
+int unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* out, int64_t ldo, hipStream_t s) {
+  typedef typename Elem<T>::type E;
+  const int64_t upr = blocks_of(K) * 4, ss = scale_stride(K), piece = row_piece(upr);
+  for (int64_t m = 0; m < M; m += piece) {
+    const int64_t rows = std::min(piece, M - m), units = rows * upr;
+    E* p = (E*)out + m * ldo;
+    hipLaunchKernelGGL((k_unpack<T>), dim3((unsigned)ceil_div(units, 256)), dim3(256), 0, s, codes + m * upr * 8,
+                       scales + m * ss, (uint32_t)units, (int)K, fast_div((uint32_t)upr), (int)ss, p, ldo,
+                       (int)vec_rows(p, ldo, T));
+  }
+  return launch_status();
+}
+
+constexpr int64_t MAX_COLS = (int64_t)1 << 20;   // row widths: 32-bit column arithmetic in the kernels
+
+// splits of the weight gradient: at most one per chunk of 64 rows, and about two workgroups a CU
+inline int64_t dw_tiles(int64_t N, int64_t K) { return ((N + 127) / 128) * ((K + 127) / 128); }
+inline int dw_splits(int64_t M, int64_t N, int64_t K) {
+  const int64_t chunks = (M + 63) / 64;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(chunks, 512 / std::max<int64_t>(1, dw_tiles(N, K))));
+}
+
+unsigned row_grid(int64_t M) { return (unsigned)std::min<int64_t>((M + BM - 1) / BM, 1 << 20); }
+
+}  // namespace q8
+}  // namespace apn
+
+using namespace apn;
+using namespace apn::lb;
+
+extern "C" int apn_q8_pack(const void* x, int32_t type, int64_t M, int64_t K, int64_t ldx, uint8_t* codes,
+                           uint8_t* scales, void* stream) {
+  if (M < 0 || K < 1 || K > q8::MAX_COLS || ldx < K || !ok_type(type)) return APN_ERR_ARG;
+  if (M == 0) return APN_OK;
+  if (!x || !codes || !scales || (uintptr_t)codes % 16) return APN_ERR_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  if (type == APN_F32) return q8::pack<APN_F32>(x, M, K, ldx, codes, scales, s);
+  if (type == APN_BF16) return q8::pack<APN_BF16>(x, M, K, ldx, codes, scales, s);
+  return q8::pack<APN_F16>(x, M, K, ldx, codes, scales, s);
+}
+
+extern "C" int apn_q8_unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* out,
+                             int32_t type, int64_t ldo, void* stream) {
+  if (M < 0 || K < 1 || K > q8::MAX_COLS || ldo < K || !ok_type(type)) return APN_ERR_ARG;
+  if (M == 0) return APN_OK;
+  if (!out || !codes || !scales || (uintptr_t)codes % 16) return APN_ERR_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  if (type == APN_F32) return q8::unpack<APN_F32>(codes, scales, M, K, out, ldo, s);
+  if (type == APN_BF16) return q8::unpack<APN_BF16>(codes, scales, M, K, out, ldo, s);
+  return q8::unpack<APN_F16>(codes, scales, M, K, out, ldo, s);
+}
+
+extern "C" int apn_q8_linear_fwd(const float* x, int64_t ldx, const float* w, int64_t ldw, const float* bias,
+                                 int64_t M, int64_t N, int64_t K, int32_t act, float slope, float* y, int64_t ldy,
+                                 uint8_t* codes, uint8_t* scales, void* stream) {
+  if (M < 0 || N < 1 || K < 1 || N > q8::MAX_COLS || K > q8::MAX_COLS || ldx < K || ldw < K || ldy < N)
+    return APN_ERR_ARG;
+  if (M == 0) return APN_OK;
+  if (!x || !w || !y || !codes || !scales || (uintptr_t)codes % 16) return APN_ERR_ARG;
+  q8::RowArgs a{x,   nullptr, w, bias, y, codes, scales, M, ldx, 0, ldw, ldy, blocks_of(N) * BLK, (int)K, (int)N,
+                (int)scale_stride(N), act, (int)vec_rows(x, ldx, APN_F32), (int)vec_rows(y, ldy, APN_F32), slope};
+  hipLaunchKernelGGL((q8::k_rows<false, false, true>), dim3(q8::row_grid(M), (unsigned)ceil_div(N, q8::BC)), dim3(256),
+                     0, (hipStream_t)stream, a);
+  return launch_status();
+}
+
+extern "C" int apn_q8_linear_bwd_dx(const float* dy, int64_t ld_dy, const uint8_t* y_codes, float slope,
+                                    const float* w, int64_t ldw, int64_t M, int64_t N, int64_t K, float* dx,
+                                    int64_t ld_dx, void* stream) {
+  if (M < 0 || N < 1 || K < 1 || N > q8::MAX_COLS || K > q8::MAX_COLS || ld_dy < N || ldw < K || ld_dx < K)
+    return APN_ERR_ARG;
+  if (M == 0) return APN_OK;
+  if (!dy || !w || !dx || (uintptr_t)y_codes % 16) return APN_ERR_ARG;
+  q8::RowArgs a{dy, y_codes, w, nullptr, dx, nullptr, nullptr, M, ld_dy, blocks_of(N) * BLK, ldw, ld_dx, 0, (int)N,
+                (int)K, 0, 0, (int)vec_rows(dy, ld_dy, APN_F32), (int)vec_rows(dx, ld_dx, APN_F32), slope};
+  const dim3 grid(q8::row_grid(M), (unsigned)ceil_div(K, q8::BC));
+  if (y_codes) hipLaunchKernelGGL((q8::k_rows<true, true, false>), grid, dim3(256), 0, (hipStream_t)stream, a);
+  else hipLaunchKernelGGL((q8::k_rows<true, false, false>), grid, dim3(256), 0, (hipStream_t)stream, a);
+  return launch_status();
+}
+
+extern "C" size_t apn_q8_linear_bwd_dw_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || N < 1 || K < 1) return 0;
+  return (size_t)q8::dw_splits(M, N, K) * (size_t)N * (size_t)(K + 1) * sizeof(float);
+}
+
+extern "C" int apn_q8_linear_bwd_dw(const float* dy, int64_t ld_dy, const uint8_t* y_codes, float slope,
+                                    const uint8_t* x_codes, const uint8_t* x_scales, int64_t M, int64_t N, int64_t K,
+                                    float* dw, float* db, void* workspace, void* stream) {
+  if (M < 0 || N < 1 || K < 1 || N > q8::MAX_COLS || K > q8::MAX_COLS || ld_dy < N) return APN_ERR_ARG;
+  if (!dw && !db) return APN_OK;
+  if (M > 0 && (!dy || !workspace || (dw && (!x_codes || !x_scales)))) return APN_ERR_ARG;
+  if ((uintptr_t)y_codes % 16 || (uintptr_t)x_codes % 16) return APN_ERR_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  if (M == 0) {   // no rows: zero gradients
+    if (dw) APN_TRY(fill_i32((int*)dw, 0, N * K, s));
+    return db ? fill_i32((int*)db, 0, N, s) : APN_OK;
+  }
+  const int sp = q8::dw_splits(M, N, K);
+  if (!dw) K = 0;   // column sums alone: no product columns
+  float* part = sp > 1 ? (float*)workspace : dw;
+  float* bpart = !db ? nullptr : sp > 1 ? part + (int64_t)sp * N * K : db;
+  q8::DwArgs a{dy, y_codes, x_codes, x_scales, part, bpart, M, ld_dy, blocks_of(N) * BLK, blocks_of(K) * BLK, (int)N,
+               (int)K, (int)scale_stride(K), sp, (int)vec_rows(dy, ld_dy, APN_F32), slope};
+  hipLaunchKernelGGL(q8::k_dw, dim3((unsigned)ceil_div(N, 128), (unsigned)std::max(1, ceil_div(K, 128)), (unsigned)sp),
+                     dim3(256), 0, s, a);
+  if (sp > 1) {
+    const int64_t n = N * K;
+    if (dw)
+      hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)std::min<int64_t>(ceil_div(n, 32), 4096)), dim3(256), 0, s,
+                         part, sp, n, dw);
+    if (db)
+      hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)std::min<int64_t>(ceil_div(N, 32), 4096)), dim3(256), 0, s,
+                         bpart, sp, N, db);
+  }
+  return launch_status();
+}
+
+extern "C" int apn_q8_idw_sum_bwd(int64_t S, int32_t C, const float* w, const uint8_t* codes, const uint8_t* scales,
+                                  const float* dh, float* d_out, float* d_w, void* stream) {
+  if (S < 0 || C < 1 || C > q8::MAX_COLS) return APN_ERR_ARG;
+  if (S == 0) return APN_OK;
+  if (!w || !dh || (d_w && (!codes || !scales)) || (uintptr_t)codes % 16) return APN_ERR_ARG;
+  const int vec = C % 4 == 0 && (uintptr_t)dh % 16 == 0 && (uintptr_t)d_out % 16 == 0;
+  hipLaunchKernelGGL(q8::k_idw_bwd, dim3((unsigned)std::min<int64_t>((S + 3) / 4, 1 << 20)), dim3(256), 0,
+                     (hipStream_t)stream, S, C, w, codes,
+                     scales, blocks_of(C) * BLK, (int)scale_stride(C), dh, d_out, d_w, vec);
+  return launch_status();
+}

@@ -26,6 +26,11 @@ extern "C" {
 #define APN_ERR_ARG 1
 #define APN_ERR_HIP 2
 
+/* element types of the entry points that take more than float rows */
+#define APN_F32 0
+#define APN_BF16 1
+#define APN_F16 2
+
 /* ---------------------------------------------------------------------------------------
  * Drop-in for the `render_utils_cuda` pybind module (lib/cuda/render_utils.cpp:144-155).
  * ------------------------------------------------------------------------------------- */
@@ -473,6 +478,55 @@ int apn_idw_sum_bwd(int64_t S, int32_t C, const float* w, const float* out, cons
  * order-preserving int32 encoding (the grid kernels' bbox_ord); workspace >= 1024 * 6 floats.
  * (temporalpoints.py:423-427 min/max of the warped cloud.) */
 int apn_cloud_bbox(const float* xyz, int64_t N, float* out6, int32_t* ord8, void* workspace, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Narrow block formats of the Linear layers. A row of K values is stored in blocks of 32
+ * consecutive columns (the last may be shorter), each with one scale 2^(byte - 127) (byte 255:
+ * the block held an infinity or NaN and reads back as NaN). Scale rows are padded with zero bytes
+ * to 4 ceil(ceil(K / 32) / 4) bytes. Code arrays are 16-B aligned. K, N <= 2^20.
+ *   q8:  32 ceil(K / 32) bytes a row, code = (x > 0 ? 0 : 0x80) | min(rint(|x| / scale), 127)
+ *        (pad: 0x80); the scale is the smallest that holds the block's largest magnitude, and the
+ *        sign bit says "not positive" also where the magnitude rounds to 0.
+ *   mx4: 16 ceil(K / 32) bytes a row, low nibble first, nibble = sign << 3 | index into
+ *        {0, 0.5, 1, 1.5, 2, 3, 4, 6}; scale = 2^(floor(log2 max|x|) - 2), nearest, ties to even,
+ *        saturating at 6 (the OCP microscaling conversion).
+ * ------------------------------------------------------------------------------------- */
+
+/* rows x [M, K] (type, row stride ldx) -> codes, scales; and back into out [M, K] (stride ldo) */
+int apn_q8_pack(const void* x, int32_t type, int64_t M, int64_t K, int64_t ldx, uint8_t* codes, uint8_t* scales,
+                void* stream);
+int apn_q8_unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* out, int32_t type,
+                  int64_t ldo, void* stream);
+/* Training Linear with its output kept in 8 bits: y [M, N] = act(x w^T + bias) in f32 accuracy
+ * (x [M, K], w [N, K], bias [N] or NULL; act: LeakyReLU(slope), slope 0 = ReLU), and the q8 codes
+ * and scales of y. */
+int apn_q8_linear_fwd(const float* x, int64_t ldx, const float* w, int64_t ldw, const float* bias, int64_t M,
+                      int64_t N, int64_t K, int32_t act, float slope, float* y, int64_t ldy, uint8_t* codes,
+                      uint8_t* scales, void* stream);
+/* Its backward from the checkpoints. G = dy * (code of y positive ? 1 : slope), G = dy when
+ * y_codes is NULL: dx [M, K] = G w;  dw [N, K] = G^T x', db [N] = sum_m G (either may be NULL), with x' the
+ * values of x's checkpoint. workspace: apn_q8_linear_bwd_dw_workspace_bytes(M, N, K); partial sums
+ * are added in a fixed order. */
+int apn_q8_linear_bwd_dx(const float* dy, int64_t ld_dy, const uint8_t* y_codes, float slope, const float* w,
+                         int64_t ldw, int64_t M, int64_t N, int64_t K, float* dx, int64_t ld_dx, void* stream);
+size_t apn_q8_linear_bwd_dw_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int apn_q8_linear_bwd_dw(const float* dy, int64_t ld_dy, const uint8_t* y_codes, float slope,
+                         const uint8_t* x_codes, const uint8_t* x_scales, int64_t M, int64_t N, int64_t K, float* dw,
+                         float* db, void* workspace, void* stream);
+/* apn_idw_sum_bwd with the rows `out` [8S, C] read from their checkpoint (d_out, d_w optional). */
+int apn_q8_idw_sum_bwd(int64_t S, int32_t C, const float* w, const uint8_t* codes, const uint8_t* scales,
+                       const float* dh, float* d_out, float* d_w, void* stream);
+
+/* rows x [M, K] (type, row stride ldx) -> mx4 codes, scales; and back into out [M, K] (stride ldo) */
+int apn_mx4_quantize(const void* x, int32_t type, int64_t M, int64_t K, int64_t ldx, uint8_t* codes, uint8_t* scales,
+                     void* stream);
+int apn_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* out, int32_t type,
+                       int64_t ldo, void* stream);
+/* out [M, N] (type, row stride ld_out) = act(a b^T + bias) of mx4 rows a [M, K] and b [N, K]: exact
+ * products, f32 sums, rounded once to the output type. */
+int apn_mx4_linear(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes, const uint8_t* b_scales,
+                   const float* bias, int64_t M, int64_t N, int64_t K, int32_t act, float slope, void* out,
+                   int32_t type, int64_t ld_out, void* stream);
 
 /* Utilities */
 size_t apn_scan_workspace_bytes(int64_t n);
