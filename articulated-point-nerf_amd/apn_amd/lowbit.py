@@ -19,10 +19,11 @@ forms (not the autograd one) can be captured into a graph.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib as L
-from ._lib import call, ptr, stream_ptr
 
 __all__ = ["Q8Rows", "q8_pack", "linear_q8", "linear_q8_backward", "sequential_q8", "MX4Rows", "mx4_quantize",
            "mx4_linear", "MX4Layer", "mx4_layers", "mx4_sequential"]
@@ -41,37 +42,62 @@ def _scale_bytes(k: int) -> int:
 
 
 def _type(dtype, what):
-    if dtype not in _TYPES:
+    t = _TYPES.get(dtype)
+    if t is None:
         raise TypeError(f"{what}: float32, bfloat16 or float16, got {dtype}")
-    return _TYPES[dtype]
+    return t
 
 
-def _same_device(what, *tensors):
-    L.require_cuda(*tensors, what=what)
-    devs = {t.device for t in tensors if t is not None}
-    if len(devs) > 1:
-        raise RuntimeError(f"{what}: tensors on different devices: {sorted(map(str, devs))}")
+def _device(what, first, *others):
+    """The index of the one device that all tensors (None: left out) are on."""
+    dev = first.get_device()
+    same = dev >= 0
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            same = False
+    if not same:
+        L.require_cuda(first, *others, what=what)
+        devs = {str(t.device) for t in (first, *others) if t is not None}
+        raise RuntimeError(f"{what}: tensors on different devices: {', '.join(sorted(devs))}")
+    return dev
+
+
+def _launch(dev, entry, *args):
+    """``entry(*args, stream)`` on device ``dev`` and its current stream. The smallest calls cost
+    what their host side costs, so addresses go in as plain integers, the stream as its raw handle,
+    and the device is switched only if it is not the current one."""
+    fn = getattr(L.load(), entry)
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc != 0:
+        raise L.APNError(f"{entry} failed: {L._STATUS.get(rc, rc)}")
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _rows(x, what):
-    """x [..., K] as a 2-D tensor with unit column stride and rows that do not overlap."""
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"{what}: expected rows of at least one column, got shape {tuple(x.shape)}")
-    if x.shape[-1] > MAX_COLS:
-        raise ValueError(f"{what}: at most {MAX_COLS} columns, got {x.shape[-1]}")
-    x2 = x.detach()
-    x2 = x2 if x2.dim() == 2 else x2.reshape(-1, x2.shape[-1])
-    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]):
-        x2 = x2.contiguous()
-    return x2
+    """x [..., K] as a 2-D tensor with unit column stride and rows that do not overlap, M, K and the
+    row stride (a single row may report any)."""
+    shape = x.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"{what}: expected rows of at least one column, got shape {tuple(shape)}")
+    K = shape[-1]
+    if K > MAX_COLS:
+        raise ValueError(f"{what}: at most {MAX_COLS} columns, got {K}")
+    if len(shape) != 2:
+        x = x.detach().reshape(-1, K)
+    M, (ld, unit) = x.shape[0], x.stride()
+    if (unit != 1 and K > 1) or (M > 1 and ld < K):
+        return x.detach().contiguous(), M, K, K
+    return x, M, K, max(ld, K)
 
 
-def _ld(x2):
-    """Row stride of a _rows() tensor (a single row may report any)."""
-    return x2.stride(0) if x2.shape[0] > 1 else max(x2.stride(0), x2.shape[1])
-
-
-def _weight(w, K, what):
+def _weight_rows(w, K, what):
     if w.dim() != 2 or w.shape[1] != K:
         raise ValueError(f"{what}: input width {K} vs weight {tuple(w.shape)}")
     if w.shape[0] == 0:
@@ -86,15 +112,16 @@ def _bias(b, N, what):
         raise ValueError(f"{what}: bias {tuple(b.shape)} for {N} outputs")
     if b.dtype != torch.float32:
         raise TypeError(f"{what}: float32 bias, got {b.dtype}")
-    return b.detach().contiguous()
+    return b if b.is_contiguous() else b.detach().contiguous()
 
 
 def _act(slope, what):
     if slope is None:
         return 0, 0.0
-    if not float("-inf") < float(slope) < float("inf"):
+    slope = float(slope)
+    if not -math.inf < slope < math.inf:
         raise ValueError(f"{what}: slope must be finite, got {slope}")
-    return 1, float(slope)
+    return 1, slope
 
 
 class _BlockRows:
@@ -117,13 +144,17 @@ class _BlockRows:
                              f"{tuple(codes.shape)} and {tuple(scales.shape)}")
         if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() % 16:
             raise ValueError(f"{what}: contiguous codes (16-byte aligned) and scales")
-        _same_device(what, codes, scales)
+        _device(what, codes, scales)
         self.codes, self.scales, self.cols = codes, scales, cols
 
     @classmethod
-    def empty(cls, rows, cols, device):
-        return cls(torch.empty(rows, cls._BYTES * _blocks(cols), dtype=torch.uint8, device=device),
-                   torch.empty(rows, _scale_bytes(cols), dtype=torch.uint8, device=device), cols)
+    def _empty(cls, rows, cols, device):
+        """Rows for a kernel to fill (their layout needs no check)."""
+        self = cls.__new__(cls)
+        self.codes = torch.empty((rows, cls._BYTES * _blocks(cols)), dtype=torch.uint8, device=device)
+        self.scales = torch.empty((rows, _scale_bytes(cols)), dtype=torch.uint8, device=device)
+        self.cols = cols
+        return self
 
     @property
     def shape(self):
@@ -139,10 +170,10 @@ class _BlockRows:
 
     def _read(self, entry, dtype):
         t = _type(dtype, f"{type(self).__name__}.dequantize")
-        M, K = self.shape
-        out = torch.empty(M, K, dtype=dtype, device=self.device)
-        with torch.cuda.device(self.device):
-            call(entry, ptr(self.codes), ptr(self.scales), M, K, ptr(out), t, K, stream_ptr(self.device))
+        codes, K = self.codes, self.cols
+        M = codes.shape[0]
+        out = torch.empty((M, K), dtype=dtype, device=codes.device)
+        _launch(codes.get_device(), entry, codes.data_ptr(), self.scales.data_ptr(), M, K, out.data_ptr(), t, K)
         return out
 
 
@@ -167,13 +198,11 @@ class MX4Rows(_BlockRows):
 
 
 def _pack(cls, entry, x, what):
-    _same_device(what, x)
     t = _type(x.dtype, what)
-    x2 = _rows(x, what)
-    M, K = x2.shape
-    out = cls.empty(M, K, x2.device)
-    with torch.cuda.device(x2.device):
-        call(entry, ptr(x2), t, M, K, _ld(x2), ptr(out.codes), ptr(out.scales), stream_ptr(x2.device))
+    x, M, K, ld = _rows(x, what)
+    dev = _device(what, x)
+    out = cls._empty(M, K, x.device)
+    _launch(dev, entry, x.data_ptr(), t, M, K, ld, out.codes.data_ptr(), out.scales.data_ptr())
     return out
 
 
@@ -188,21 +217,17 @@ def linear_q8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
     x [..., K] and weight [N, K] float32; ``slope``: None (no activation), 0 (ReLU) or the LeakyReLU
     negative slope. The products are f32-accurate."""
     what = "linear_q8"
-    _same_device(what, x, weight, bias)
     if x.dtype != torch.float32 or weight.dtype != torch.float32:
         raise TypeError(f"{what}: float32 only, got {x.dtype} and {weight.dtype}")
-    x2 = _rows(x, what)
-    M, K = x2.shape
-    w = _weight(weight, K, what)
-    N = w.shape[0]
+    x, M, K, ldx = _rows(x, what)
+    w, N, _, ldw = _weight_rows(weight, K, what)
     b = _bias(bias, N, what)
     act, sl = _act(slope, what)
-    dev = x2.device
-    y = torch.empty(M, N, device=dev)
-    kept = Q8Rows.empty(M, N, dev)
-    with torch.cuda.device(dev):
-        call("apn_q8_linear_fwd", ptr(x2), _ld(x2), ptr(w), _ld(w), ptr(b), M, N, K, act, sl, ptr(y), N,
-             ptr(kept.codes), ptr(kept.scales), stream_ptr(dev))
+    dev = _device(what, x, w, b)
+    y = torch.empty((M, N), dtype=torch.float32, device=x.device)
+    kept = Q8Rows._empty(M, N, x.device)
+    _launch(dev, "apn_q8_linear_fwd", x.data_ptr(), ldx, w.data_ptr(), ldw, _addr(b), M, N, K, act, sl, y.data_ptr(), N,
+            kept.codes.data_ptr(), kept.scales.data_ptr())
     return y, kept
 
 
@@ -218,42 +243,36 @@ def linear_q8_backward(dy: torch.Tensor, weight: torch.Tensor, x_kept: Q8Rows | 
     for kept, name in ((x_kept, "x_kept"), (y_kept, "y_kept")):
         if kept is not None and not isinstance(kept, Q8Rows):
             raise TypeError(f"{what}: {name} must be Q8Rows, got {type(kept).__name__}")
-    _same_device(what, dy, weight, *[k.codes for k in (x_kept, y_kept) if k is not None])
     if dy.dtype != torch.float32 or weight.dtype != torch.float32:
         raise TypeError(f"{what}: float32 only, got {dy.dtype} and {weight.dtype}")
-    dy = _rows(dy, what)
-    M, N = dy.shape
+    dy, M, N, ld_dy = _rows(dy, what)
     if weight.dim() != 2 or weight.shape[0] != N:
         raise ValueError(f"{what}: gradient width {N} vs weight {tuple(weight.shape)}")
-    w = _rows(weight, what)
-    K = w.shape[1]
+    w, _, K, ldw = _rows(weight, what)
     if want_w and x_kept is None:
         raise ValueError(f"{what}: dw needs x_kept")
     if x_kept is not None and x_kept.shape != (M, K):
         raise ValueError(f"{what}: x_kept is {x_kept.shape}, expected {(M, K)}")
-    _, sl = _act(slope, what)
-    mask = None
-    if slope is not None:
-        if y_kept is None:
-            raise ValueError(f"{what}: an activation needs y_kept")
-        mask = y_kept.codes
     if y_kept is not None and y_kept.shape != (M, N):
         raise ValueError(f"{what}: y_kept is {y_kept.shape}, expected {(M, N)}")
-    dev = dy.device
+    _, sl = _act(slope, what)
+    if slope is not None and y_kept is None:
+        raise ValueError(f"{what}: an activation needs y_kept")
+    mask = y_kept.codes if slope is not None else None
+    xc, xs = (x_kept.codes, x_kept.scales) if want_w else (None, None)
+    dev = _device(what, dy, w, mask, xc)
+    empty = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dy.device)  # noqa: E731
     dx = dw = db = None
-    with torch.cuda.device(dev):
-        s = stream_ptr(dev)
-        if want_x:
-            dx = torch.empty(M, K, device=dev)
-            call("apn_q8_linear_bwd_dx", ptr(dy), _ld(dy), ptr(mask), sl, ptr(w), _ld(w), M, N, K, ptr(dx), K, s)
-        if want_w or want_b:
-            dw = torch.empty(N, K, device=dev) if want_w else None
-            db = torch.empty(N, device=dev) if want_b else None
-            nbytes = int(L.load().apn_q8_linear_bwd_dw_workspace_bytes(M, N, K))
-            ws = torch.empty(max(nbytes // 4, 1), device=dev)
-            xk = (x_kept.codes, x_kept.scales) if want_w else (None, None)
-            call("apn_q8_linear_bwd_dw", ptr(dy), _ld(dy), ptr(mask), sl, ptr(xk[0]), ptr(xk[1]), M, N, K, ptr(dw),
-                 ptr(db), ptr(ws), s)
+    if want_x:
+        dx = empty(M, K)
+        _launch(dev, "apn_q8_linear_bwd_dx", dy.data_ptr(), ld_dy, _addr(mask), sl, w.data_ptr(), ldw, M, N, K,
+                dx.data_ptr(), K)
+    if want_w or want_b:
+        dw = empty(N, K) if want_w else None
+        db = empty(N) if want_b else None
+        ws = empty(max(int(L.load().apn_q8_linear_bwd_dw_workspace_bytes(M, N, K)) // 4, 1))
+        _launch(dev, "apn_q8_linear_bwd_dw", dy.data_ptr(), ld_dy, _addr(mask), sl, _addr(xc), _addr(xs), M, N, K,
+                _addr(dw), _addr(db), ws.data_ptr())
     return dx, dw, db
 
 
@@ -350,24 +369,22 @@ def mx4_linear(x, weight: MX4Rows, bias: torch.Tensor | None = None, slope: floa
     if not isinstance(weight, MX4Rows):
         raise TypeError(f"{what}: weight must be MX4Rows, got {type(weight).__name__}")
     t = _type(out_dtype, what)
-    if not isinstance(x, MX4Rows):
-        _same_device(what, x, weight.codes)
-        if x.dim() and x.shape[-1] != weight.cols:
-            raise ValueError(f"{what}: input width {x.shape[-1]} vs weight {weight.shape}")
-        x = mx4_quantize(x)
-    if x.cols != weight.cols:
-        raise ValueError(f"{what}: input width {x.cols} vs weight {weight.shape}")
-    _same_device(what, x.codes, weight.codes, bias)
-    (M, K), N = x.shape, weight.shape[0]
+    wc, K = weight.codes, weight.cols
+    width = x.cols if isinstance(x, MX4Rows) else x.shape[-1] if x.dim() else 0
+    if width != K:
+        raise ValueError(f"{what}: input width {width} vs weight {weight.shape}")
+    N = wc.shape[0]
     if N == 0:
         raise ValueError(f"{what}: weight without rows {weight.shape}")
     b = _bias(bias, N, what)
     act, sl = _act(slope, what)
-    dev = x.device
-    out = torch.empty(M, N, dtype=out_dtype, device=dev)
-    with torch.cuda.device(dev):
-        call("apn_mx4_linear", ptr(x.codes), ptr(x.scales), ptr(weight.codes), ptr(weight.scales), ptr(b), M, N, K, act,
-             sl, ptr(out), t, N, stream_ptr(dev))
+    dev = _device(what, x.codes if isinstance(x, MX4Rows) else x, wc, b)
+    if not isinstance(x, MX4Rows):
+        x = mx4_quantize(x)
+    M = x.codes.shape[0]
+    out = torch.empty((M, N), dtype=out_dtype, device=wc.device)
+    _launch(dev, "apn_mx4_linear", x.codes.data_ptr(), x.scales.data_ptr(), wc.data_ptr(), weight.scales.data_ptr(),
+            _addr(b), M, N, K, act, sl, out.data_ptr(), t, N)
     return out
 
 
@@ -377,7 +394,7 @@ class MX4Layer:
     def __init__(self, weight: MX4Rows, bias: torch.Tensor | None = None, slope: float | None = None):
         if not isinstance(weight, MX4Rows):
             raise TypeError(f"MX4Layer: weight must be MX4Rows, got {type(weight).__name__}")
-        _same_device("MX4Layer", weight.codes, bias)
+        _device("MX4Layer", weight.codes, bias)
         self.weight, self.slope = weight, slope
         self.bias = _bias(bias, weight.shape[0], "MX4Layer")
         _act(slope, "MX4Layer")

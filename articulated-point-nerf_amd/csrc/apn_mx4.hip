@@ -32,14 +32,14 @@ __device__ __forceinline__ float value4(uint32_t n, float scale) {
 // One thread per 8 columns, 4 threads per block, as the q8 pack.
 template <int T>
 __global__ __launch_bounds__(256) void k_quant(const typename Elem<T>::type* __restrict__ x, uint32_t units, int K,
-                                               int64_t ldx, int vec, FastDiv upr, uint8_t* __restrict__ codes,
+                                               int64_t ldx, FastDiv upr, uint8_t* __restrict__ codes,
                                                uint8_t* __restrict__ scales, int ss) {
   const uint32_t u = blockIdx.x * 256u + threadIdx.x;
   const bool live = u < units;
   const uint32_t m = div_by(min(u, units - 1), upr), cu = min(u, units - 1) - m * upr.d;
   const int c = (int)cu * 8, n = min(8, K - c);
   float v[8];
-  load8<T>(x + (int64_t)m * ldx + c, n, vec && n == 8, v);
+  load8<T>(x + (int64_t)m * ldx + c, n, v);
   uint32_t a = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) a = max(a, abs_bits(v[j]));
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256) void k_quant(const typename Elem<T>::type* __r
 template <int T>
 __global__ __launch_bounds__(256) void k_dequant(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                  uint32_t units, int K, FastDiv upr, int ss,
-                                                 typename Elem<T>::type* __restrict__ out, int64_t ldo, int vec) {
+                                                 typename Elem<T>::type* __restrict__ out, int64_t ldo) {
   const uint32_t u = blockIdx.x * 256u + threadIdx.x;
   if (u >= units) return;
   const uint32_t m = div_by(u, upr), cu = u - m * upr.d;
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void k_dequant(const uint8_t* __restrict__ cod
   float v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = value4((w >> (4 * j)) & 15u, sc);
-  store8<T>(out + (int64_t)m * ldo + c, n, vec && n == 8, v);
+  store8<T>(out + (int64_t)m * ldo + c, n, v);
 }
 
 // Y[m][n]: 32 x 32 tiles of v_mfma_scale_f32_32x32x64 (lane: row lane % 32, the 32 values -- 16 B
@@ -86,7 +86,7 @@ struct Args {
   const float* bias;
   void* out;
   int64_t M, ld_out;
-  int N, nb, ss, act, vec_out;   // nb: blocks of K; ss: bytes per scale row
+  int N, nb, ss, act;   // nb: blocks of K; ss: bytes per scale row
   float slope;
 };
 
@@ -94,19 +94,6 @@ __device__ __forceinline__ f32x16 mma(u32x4 a, int sa, u32x4 b, int sb, f32x16 c
   const i32x8 A = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
   const i32x8 B = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, 0, sa, 0, sb);
-}
-
-template <int T>
-__device__ __forceinline__ void store4(typename Elem<T>::type* o, int n, bool vec, const float* v) {
-  typedef typename Elem<T>::type E;
-  if (vec && n >= 4) {
-    typedef E e4 __attribute__((ext_vector_type(4)));
-    *(e4*)o = e4{(E)v[0], (E)v[1], (E)v[2], (E)v[3]};
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) o[i] = (E)v[i];
-  }
 }
 
 template <int T>
@@ -156,7 +143,7 @@ __global__ __launch_bounds__(256) void k_linear(Args p) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int n = n0 + 32 * t + 8 * j + 4 * h;
-        store4<T>((typename Elem<T>::type*)p.out + m * p.ld_out + n, p.N - n, p.vec_out, y + 4 * j);
+        store4<T>((typename Elem<T>::type*)p.out + m * p.ld_out + n, p.N - n, y + 4 * j);
       }
     }
   }
@@ -172,7 +159,7 @@ int quantize(const void* x, int64_t M, int64_t K, int64_t ldx, uint8_t* codes, u
     const int64_t rows = std::min(piece, M - m), units = rows * upr;
     const E* p = (const E*)x + m * ldx;
     hipLaunchKernelGGL((k_quant<T>), dim3((unsigned)ceil_div(units, 256)), dim3(256), 0, s, p, (uint32_t)units, (int)K,
-                       ldx, (int)vec_rows(p, ldx, T), fast_div((uint32_t)upr), codes + m * upr * 4, scales + m * ss,
+                       ldx, fast_div((uint32_t)upr), codes + m * upr * 4, scales + m * ss,
                        (int)ss);
   }
   return launch_status();
@@ -187,8 +174,7 @@ int dequantize(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K
     const int64_t rows = std::min(piece, M - m), units = rows * upr;
     E* p = (E*)out + m * ldo;
     hipLaunchKernelGGL((k_dequant<T>), dim3((unsigned)ceil_div(units, 256)), dim3(256), 0, s, codes + m * upr * 4,
-                       scales + m * ss, (uint32_t)units, (int)K, fast_div((uint32_t)upr), (int)ss, p, ldo,
-                       (int)vec_rows(p, ldo, T));
+                       scales + m * ss, (uint32_t)units, (int)K, fast_div((uint32_t)upr), (int)ss, p, ldo);
   }
   return launch_status();
 }
@@ -231,9 +217,8 @@ extern "C" int apn_mx4_linear(const uint8_t* a_codes, const uint8_t* a_scales, c
   if (M == 0) return APN_OK;
   if (!a_codes || !a_scales || !b_codes || !b_scales || !out) return APN_ERR_ARG;
   if ((uintptr_t)a_codes % 16 || (uintptr_t)b_codes % 16) return APN_ERR_ARG;
-  const int64_t tb = type_bytes(type);
   mx4::Args a{a_codes, a_scales, b_codes, b_scales, bias, out, M, ld_out, (int)N, (int)blocks_of(K),
-              (int)scale_stride(K), act, (uintptr_t)out % (4 * tb) == 0 && ld_out % 4 == 0, slope};
+              (int)scale_stride(K), act, slope};
   const dim3 grid((unsigned)std::min<int64_t>((M + 127) / 128, 1 << 20), (unsigned)ceil_div(N, 64));
   hipStream_t s = (hipStream_t)stream;
   if (type == APN_F32) hipLaunchKernelGGL((mx4::k_linear<APN_F32>), grid, dim3(256), 0, s, a);

@@ -28,7 +28,7 @@ using namespace lb;
 // Bound by memory.
 template <int T>
 __global__ __launch_bounds__(256) void k_pack(const typename Elem<T>::type* __restrict__ x, uint32_t units, int K,
-                                              int64_t ldx, int vec, FastDiv upr, uint8_t* __restrict__ codes,
+                                              int64_t ldx, FastDiv upr, uint8_t* __restrict__ codes,
                                               uint8_t* __restrict__ scales, int ss) {
   const uint32_t u = blockIdx.x * 256u + threadIdx.x;
   const bool live = u < units;
@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void k_pack(const typename Elem<T>::type* __re
   const int c = (int)cu * 8;
   const int n = min(8, K - c);   // <= 0 in the padding of the last block
   float v[8];
-  load8<T>(x + (int64_t)m * ldx + c, n, vec && n == 8, v);
+  load8<T>(x + (int64_t)m * ldx + c, n, v);
   uint32_t a = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) a = max(a, abs_bits(v[j]));
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256) void k_pack(const typename Elem<T>::type* __re
 template <int T>
 __global__ __launch_bounds__(256) void k_unpack(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                 uint32_t units, int K, FastDiv upr, int ss,
-                                                typename Elem<T>::type* __restrict__ out, int64_t ldo, int vec) {
+                                                typename Elem<T>::type* __restrict__ out, int64_t ldo) {
   const uint32_t u = blockIdx.x * 256u + threadIdx.x;
   if (u >= units) return;
   const uint32_t m = div_by(u, upr), cu = u - m * upr.d;
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void k_unpack(const uint8_t* __restrict__ code
   float v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = q8_value((w[j >> 2] >> (8 * (j & 3))) & 0xffu, sc);
-  store8<T>(out + (int64_t)m * ldo + c, n, vec && n == 8, v);
+  store8<T>(out + (int64_t)m * ldo + c, n, v);
 }
 
 // --- f32 products on bf16 matrix units -------------------------------------------------------
@@ -97,14 +97,14 @@ __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
 
 // Rows kernel: out[m][c] = sum_r in[m][r] Wop[c][r], the forward (r = input column, c = output
 // column) and dX (r = output column, c = input column, Wop = W^T, `in` masked by Y's signs).
-// 64 rows x 128 columns per 256-thread workgroup. The matrix operands are swapped -- A = W's rows,
-// B = the data rows -- so a lane's 16 results of a 32 x 32 tile are 16 of the 32 columns of ONE
-// data row (columns 8 j + 4 h + i; the other half in lane ^ 32), which makes the q8 block maximum
-// 15 in-lane maxima and one exchange. Data rows are staged through LDS once per workgroup, cut
-// into their three planes, in fragment order: 16-B piece (plane, k step, row tile, half, row), the
-// row slot xor-ed with the 8-column unit so that the 8 lanes which write one row's units and the
-// 8 lanes which read neighbouring rows both meet all 8 bank groups.
-constexpr int BM = 64, BC = 128, BR = 64;   // rows, columns, reduction per staged chunk
+// 64 rows x 32 NW columns per workgroup of NW waves. The matrix operands are swapped -- A = W's
+// rows, B = the data rows -- so a lane's 16 results of a 32 x 32 tile are 16 of the 32 columns of
+// ONE data row (columns 8 j + 4 h + i; the other half in lane ^ 32), which makes the q8 block
+// maximum 15 in-lane maxima and one exchange. Data rows are staged through LDS once per workgroup,
+// cut into their three planes, in fragment order: 16-B piece (plane, k step, row tile, half, row),
+// the row slot xor-ed with the 8-column unit so that the 8 lanes which write one row's units and
+// the 8 lanes which read neighbouring rows both meet all 8 bank groups.
+constexpr int BM = 64;   // rows of a workgroup's tile; the reduction is staged 64 columns at a time
 
 struct RowArgs {
   const float* in;
@@ -115,280 +115,412 @@ struct RowArgs {
   uint8_t* codes;
   uint8_t* scales;
   int64_t M, ld_in, ld_mask, ldw, ld_out, ld_codes;
-  int R, C, ss, act, vec_in, vec_out;
+  int R, C, ss, act;
   float slope;
 };
 
 template <bool WT>   // WT: W stored [r][c], else [c][r]
 __device__ __forceinline__ void load_w(const RowArgs& p, int c, int r, float (&v)[8]) {
-  if (c < p.C && r + 8 <= p.R) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = WT ? p.w[(int64_t)(r + j) * p.ldw + c] : p.w[(int64_t)c * p.ldw + r + j];
+  const int cc = min(c, p.C - 1);
+  if (!WT && r + 8 <= p.R) {
+    load8<APN_F32>(p.w + (int64_t)cc * p.ldw + r, 8, v);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      v[j] = c < p.C && r + j < p.R ? (WT ? p.w[(int64_t)(r + j) * p.ldw + c] : p.w[(int64_t)c * p.ldw + r + j]) : 0.f;
+    for (int j = 0; j < 8; ++j) {
+      const int rr = min(r + j, p.R - 1);
+      v[j] = p.w[WT ? (int64_t)rr * p.ldw + cc : (int64_t)cc * p.ldw + rr];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = r + j < p.R ? v[j] : 0.f;
+  }
+  if (c >= p.C) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
   }
 }
 
-template <bool WT, bool MASK, bool Q8>
-__global__ __launch_bounds__(256, 2) void k_rows(RowArgs p) {
-  __shared__ u32x4 sh[3 * 4 * 2 * 64];
+__device__ __forceinline__ float masked(float g, uint32_t code, float slope) {
+  return code & 0x80u ? (slope == 0.f ? 0.f : g * slope) : g;
+}
+
+// One thread's 8-column unit of a staged chunk: the loads, and later the cut into LDS. Rows and
+// columns behind the ends are read at the last one and zeroed: no lane branches around a load.
+struct Unit {
+  float v[8];
+  u32x2 s;
+};
+template <bool MASK>
+__device__ __forceinline__ void load_unit(const RowArgs& p, int64_t m, int r, bool full, Unit& u) {
+  const int64_t mm = min(m, p.M - 1);
+  const float* q = p.in + mm * p.ld_in;
+  if (full) {
+    load8<APN_F32>(q + r, 8, u.v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u.v[j] = q[min(r + j, p.R - 1)];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u.v[j] = m < p.M && r + j < p.R ? u.v[j] : 0.f;
+  }
+  if (MASK) u.s = *(const u32x2*)(p.mask + mm * p.ld_mask + min(r, (int)p.ld_mask - 8));
+}
+template <bool MASK>
+__device__ __forceinline__ void stage_unit(const RowArgs& p, int row, int u, Unit& x, u32x4* sh) {
+  if (MASK) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x.v[j] = masked(x.v[j], x.s[j >> 2] >> (8 * (j & 3)), p.slope);
+  }
+  u32x4 a, b, c;
+  cut3(x.v, a, b, c);
+  const int at = (u >> 1) * 128 + (row >> 5) * 64 + (u & 1) * 32 + ((row & 31) ^ u);
+  sh[at] = a, sh[512 + at] = b, sh[1024 + at] = c;
+}
+
+// six products of one 16-column step for the wave's NT row tiles from t0 on, small ones first
+template <int NT>
+__device__ __forceinline__ void step(const u32x4* sh, int ks, int t0, int l, int h, u32x4 wh, u32x4 wm, u32x4 wl,
+                                     f32x16 (&acc)[NT]) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int at = ks * 128 + (t0 + t) * 64 + h * 32 + (l ^ (2 * ks + h));
+    const u32x4 xh = sh[at], xm = sh[512 + at], xl = sh[1024 + at];
+    f32x16 a = acc[t];
+    a = mma(wl, xh, a), a = mma(wh, xl, a), a = mma(wm, xm, a);
+    a = mma(wm, xh, a), a = mma(wh, xm, a), a = mma(wh, xh, a);
+    acc[t] = a;
+  }
+}
+
+template <bool Q8, int NT>
+__device__ __forceinline__ void finish_rows(const RowArgs& p, int64_t m0, int c0, int l, int h,
+                                            const f32x16 (&acc)[NT]) {
+  if (c0 >= p.C) return;   // uniform in the wave
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t m = m0 + 32 * t + l;
+    float y[16];
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int c = c0 + 8 * (i >> 2) + 4 * h + (i & 3);
+      float v = acc[t][i];
+      if (p.bias) v += p.bias[min(c, p.C - 1)];
+      if (p.act) v = leaky(v, p.slope);
+      if (Q8) {
+        v = c < p.C ? v : 0.f;
+        amax = max(amax, abs_bits(v));
+      }
+      y[i] = v;
+    }
+    if (m < p.M) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = c0 + 8 * j + 4 * h;
+        store4<APN_F32>(p.out + m * p.ld_out + c, p.C - c, y + 4 * j);
+      }
+    }
+    if (Q8) {
+      amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
+      const int byte = q8_byte(amax);
+      const float inv = inv_pow2_of(byte);
+      if (m < p.M) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t w = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w |= q8_code(y[4 * j + i], inv) << (8 * i);
+          *(uint32_t*)(p.codes + m * p.ld_codes + c0 + 8 * j + 4 * h) = w;
+        }
+        if (h == 0) {
+          uint8_t* s = p.scales + m * p.ss;
+          s[c0 >> 5] = (uint8_t)byte;
+          if (c0 + 32 >= p.C)
+            for (int i = (c0 >> 5) + 1; i < p.ss; ++i) s[i] = 0;
+        }
+      }
+    }
+  }
+}
+
+// R <= 64 NCH: each wave keeps its 32 columns' weights, cut, in registers (48 per chunk) and the
+// workgroup -- NW column groups of RG waves, each wave 64 / RG rows -- walks the row tiles; LDS is double-buffered (one barrier per chunk) and the next
+// chunk's rows are on their way to registers while this one is multiplied.
+template <bool WT, bool MASK, bool Q8, int NCH, int NW, int RG>
+__global__ __launch_bounds__(64 * NW * RG, 2) void k_rows_held(RowArgs p) {
+  constexpr int T = 64 * NW * RG, UPT = (512 + T - 1) / T, NT = 2 / RG;
+  __shared__ u32x4 sh[2 * 1536];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int l = lane & 31, h = lane >> 5;
-  const int c0 = blockIdx.y * BC + wave * 32;
+  const int c0 = (blockIdx.y * NW + wave % NW) * 32, t0 = wave / NW * NT;
+  u32x4 wh[4 * NCH], wm[4 * NCH], wl[4 * NCH];
+#pragma unroll
+  for (int ks = 0; ks < 4 * NCH; ++ks) {
+    float v[8];
+    load_w<WT>(p, c0 + l, 16 * ks + 8 * h, v);
+    cut3(v, wh[ks], wm[ks], wl[ks]);
+  }
+  const int64_t tiles = (p.M + BM - 1) / BM;
+  Unit x[UPT];
+  auto load = [&](int64_t m0, int ch) __attribute__((always_inline)) {
+    const bool full = m0 + BM <= p.M && 64 * ch + 64 <= p.R;
+#pragma unroll
+    for (int i = 0; i < UPT; ++i) {
+      const int f = tid + T * i;
+      if (T * UPT == 512 || f < 512) load_unit<MASK>(p, m0 + (f >> 3), 64 * ch + 8 * (f & 7), full, x[i]);
+    }
+  };
+  int64_t tile = blockIdx.x;
+  if (tile < tiles) load(tile * BM, 0);
+  int buf = 0;
+  for (; tile < tiles; tile += gridDim.x) {
+    f32x16 acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
+#pragma unroll
+    for (int ch = 0; ch < NCH; ++ch) {
+      u32x4* s = sh + buf;
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        const int f = tid + T * i;
+        if (T * UPT == 512 || f < 512) stage_unit<MASK>(p, f >> 3, f & 7, x[i], s);
+      }
+      __syncthreads();
+      if (ch + 1 < NCH) load(tile * BM, ch + 1);
+      else if (tile + gridDim.x < tiles) load((tile + gridDim.x) * BM, 0);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        step<NT>(s, ks, t0, l, h, wh[4 * ch + ks], wm[4 * ch + ks], wl[4 * ch + ks], acc);
+        if (NCH == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+      buf ^= 1536;
+    }
+    finish_rows<Q8, NT>(p, tile * BM + 32 * t0, c0, l, h, acc);
+  }
+}
+
+// Any R: the weights are read (from the caches) and cut at each use, one step ahead.
+template <bool WT, bool MASK, bool Q8>
+__global__ __launch_bounds__(256, 2) void k_rows(RowArgs p) {
+  __shared__ u32x4 sh[2 * 1536];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int l = lane & 31, h = lane >> 5;
+  const int c0 = (blockIdx.y * 4 + wave) * 32;
+  const int nch = (p.R + 63) / 64, last = (p.R - 1) / 16;
+  int buf = 0;
   for (int64_t m0 = (int64_t)blockIdx.x * BM; m0 < p.M; m0 += (int64_t)gridDim.x * BM) {
     f32x16 acc[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
-    for (int r0 = 0; r0 < p.R; r0 += BR) {
-      __syncthreads();
+    Unit x[2];
+    float wv[8];
+    auto load = [&](int ch) __attribute__((always_inline)) {
+      const bool full = m0 + BM <= p.M && 64 * ch + 64 <= p.R;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {   // 64 rows x 8 units of 8 columns, two per thread
-        const int f = tid + 256 * i, row = f >> 3, u = f & 7;
-        const int64_t m = m0 + row;
-        const int r = r0 + 8 * u, n = m < p.M ? min(8, p.R - r) : 0;
-        float v[8];
-        load8<APN_F32>(p.in + m * p.ld_in + r, n, p.vec_in && n == 8, v);
-        if (MASK && n > 0) {
-          const u32x2 s = *(const u32x2*)(p.mask + m * p.ld_mask + r);
+      for (int i = 0; i < 2; ++i) {
+        const int f = tid + 256 * i;
+        load_unit<MASK>(p, m0 + (f >> 3), 64 * ch + 8 * (f & 7), full, x[i]);
+      }
+    };
+    load(0);
+    load_w<WT>(p, c0 + l, 8 * h, wv);
+    for (int ch = 0; ch < nch; ++ch) {
+      u32x4* s = sh + buf;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if ((s[j >> 2] >> (8 * (j & 3))) & 0x80u) v[j] = p.slope == 0.f ? 0.f : v[j] * p.slope;
-        }
-        u32x4 a, b, c;
-        cut3(v, a, b, c);
-        const int at = (u >> 1) * 128 + (row >> 5) * 64 + (u & 1) * 32 + ((row & 31) ^ u);
-        sh[at] = a, sh[512 + at] = b, sh[1024 + at] = c;
+      for (int i = 0; i < 2; ++i) {
+        const int f = tid + 256 * i;
+        stage_unit<MASK>(p, f >> 3, f & 7, x[i], s);
       }
       __syncthreads();
+      if (ch + 1 < nch) load(ch + 1);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        if (r0 + 16 * ks >= p.R) break;
-        float wv[8];
-        load_w<WT>(p, c0 + l, r0 + 16 * ks + 8 * h, wv);
         u32x4 wh, wm, wl;
         cut3(wv, wh, wm, wl);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int at = ks * 128 + t * 64 + h * 32 + (l ^ (2 * ks + h));
-          const u32x4 xh = sh[at], xm = sh[512 + at], xl = sh[1024 + at];
-          f32x16 a = acc[t];
-          a = mma(wl, xh, a), a = mma(wh, xl, a), a = mma(wm, xm, a);
-          a = mma(wm, xh, a), a = mma(wh, xm, a), a = mma(wh, xh, a);
-          acc[t] = a;
-        }
+        const int g = 4 * ch + ks;
+        if (g >= last + 1) break;
+        load_w<WT>(p, c0 + l, 16 * min(g + 1, last) + 8 * h, wv);
+        step<2>(s, ks, 0, l, h, wh, wm, wl, acc);
       }
+      buf ^= 1536;
     }
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int64_t m = m0 + 32 * t + l;
-      if (c0 >= p.C) continue;   // uniform in the wave
-      float y[16];
-      uint32_t amax = 0;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int c = c0 + 8 * (i >> 2) + 4 * h + (i & 3);
-        float v = acc[t][i];
-        if (p.bias && c < p.C) v += p.bias[c];
-        if (p.act) v = leaky(v, p.slope);
-        if (Q8 && c >= p.C) v = 0.f;
-        y[i] = v;
-        if (Q8) amax = max(amax, abs_bits(v));
-      }
-      if (m < p.M) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int c = c0 + 8 * j + 4 * h;
-          float* o = p.out + m * p.ld_out + c;
-          if (p.vec_out && c + 4 <= p.C) {
-            *(f32x4*)o = f32x4{y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]};
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (c + i < p.C) o[i] = y[4 * j + i];
-          }
-        }
-      }
-      if (Q8) {
-        amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
-        const int byte = q8_byte(amax);
-        const float inv = inv_pow2_of(byte);
-        if (m < p.M) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t w = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w |= q8_code(y[4 * j + i], inv) << (8 * i);
-            *(uint32_t*)(p.codes + m * p.ld_codes + c0 + 8 * j + 4 * h) = w;
-          }
-          if (h == 0) {
-            uint8_t* s = p.scales + m * p.ss;
-            s[c0 >> 5] = (uint8_t)byte;
-            if (c0 + 32 >= p.C)
-              for (int i = (c0 >> 5) + 1; i < p.ss; ++i) s[i] = 0;
-          }
-        }
-      }
-    }
+    finish_rows<Q8, 2>(p, m0, c0, l, h, acc);
   }
 }
 
 // Weight gradient: dW[n][k] = sum_m G[m][n] X'[m][k], db[n] = sum_m G[m][n], 128 x 128 outputs per
-// workgroup, wave (i, j) its 64 x 64 quarter, the rows in chunks of 64 over the splits (blockIdx.z
-// takes every splits-th chunk), partial sums to the workspace and added in a fixed order. Both
-// operands need 8 consecutive rows m per lane: a thread reads 4 columns of 8 rows and writes the
-// four 8-row pieces in fragment order, column slots xor-ed with bits 3..4 of the column so that
-// the writing lanes (4 columns apart) meet all bank groups.
+// workgroup of 8 waves, wave (i, j) 32 x 64 of them, the rows in chunks of 64 over the splits
+// (blockIdx.z takes every splits-th chunk), partial sums to the workspace and added in a fixed
+// order. Both operands need 8 consecutive rows m per lane: a thread reads 4 columns of 8 rows of G
+// (threads 0..255) or X' (256..511) and writes the four 8-row pieces in fragment order, column
+// slots xor-ed with bits 3..4 of the column so that the writing lanes (4 columns apart) meet all
+// bank groups.
 struct DwArgs {
   const float* dy;
   const uint8_t* mask;
   const uint8_t* xc;
   const uint8_t* xs;
-  float* dw;        // [splits][N][K]
-  float* db;        // [splits][N] or null
-  int64_t M, ld_dy, ld_mask, ld_xc;
-  int N, K, ss, splits, vec_dy;
+  float* dw;        // partial z at dw + z stride
+  float* db;        // partial z at db + z stride, or null
+  int64_t M, ld_dy, ld_mask, ld_xc, stride;
+  int N, K, ss, splits;
   float slope;
 };
 
 __device__ __forceinline__ int slot32(int c) { return (c & 31) ^ ((c >> 3) & 3); }
 
-__global__ __launch_bounds__(256, 2) void k_dw(DwArgs p) {
-  __shared__ u32x4 sg[3 * 4 * 4 * 64];   // [plane][k step][column tile][half, slot]
-  __shared__ u32x4 sx[4 * 4 * 64];
+constexpr int DW_BUF = 3 * 1024 + 1024;   // 16-B pieces: three planes of G, one of X'
+
+__global__ __launch_bounds__(512, 2) void k_dw(DwArgs p) {
+  extern __shared__ u32x4 dw_sh[];   // 2 DW_BUF
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int l = lane & 31, h = lane >> 5;
   const int n0 = blockIdx.x * 128, k0 = blockIdx.y * 128;
-  const int cq = tid & 31, mo = tid >> 5;   // this thread's 4 columns 4 cq .. and 8 rows 8 mo ..
+  const bool g_side = tid < 256;
+  const int cq = tid & 31, mo = (tid & 255) >> 5;   // this thread's 4 columns 4 cq .. and 8 rows 8 mo ..
   const int gc = n0 + 4 * cq, xk = k0 + 4 * cq;
-  f32x16 acc[2][2];
+  f32x16 acc[2];
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
+  for (int b = 0; b < 2; ++b)
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
+    for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
   float bs[4] = {0.f, 0.f, 0.f, 0.f};
+  f32x4 gv[8];        // G rows, or (X' side) codes and scale
+  uint32_t gs[8];
   const int64_t chunks = (p.M + 63) / 64;
-  for (int64_t ch = blockIdx.z; ch < chunks; ch += p.splits) {
+  auto load = [&](int64_t ch) __attribute__((always_inline)) {
     const int64_t m0 = ch * 64 + 8 * mo;
-    float g[4][8];
+    if (g_side) {
+      const bool full = gc + 4 <= p.N;
+      const int cc = min(gc, p.N - 1);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t m = m0 + j;
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      uint32_t s = 0;
-      if (m < p.M && gc < p.N) {
-        const float* q = p.dy + m * p.ld_dy + gc;
-        if (p.vec_dy && gc + 4 <= p.N) {
-          const f32x4 a = *(const f32x4*)q;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) v[c] = a[c];
+      for (int j = 0; j < 8; ++j) {
+        const int64_t m = min(m0 + j, p.M - 1);
+        const float* q = p.dy + m * p.ld_dy;
+        if (full) {
+          gv[j] = *(const typename Octet<float>::half*)(q + gc);
         } else {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) v[c] = gc + c < p.N ? q[c] : 0.f;
+          for (int c = 0; c < 4; ++c) gv[j][c] = q[min(gc + c, p.N - 1)];
         }
-        if (p.mask) s = *(const uint32_t*)(p.mask + m * p.ld_mask + gc);
+        gs[j] = p.mask ? *(const uint32_t*)(p.mask + m * p.ld_mask + (cc & ~3)) : 0u;
       }
+    } else if (p.K > 0) {
+      const int kk = min(xk, (int)p.ld_xc - 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int64_t m = min(m0 + j, p.M - 1);
+        gs[j] = *(const uint32_t*)(p.xc + m * p.ld_xc + kk);
+        gv[j][0] = __uint_as_float((uint32_t)p.xs[m * p.ss + (kk >> 5)]);
+      }
+    }
+  };
+  auto stage = [&](int64_t ch, u32x4* sh) __attribute__((always_inline)) {
+    const int64_t m0 = ch * 64 + 8 * mo;
+    const int at = (mo >> 1) * 256 + (cq >> 3) * 64 + (mo & 1) * 32;
+    if (g_side) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        if ((s >> (8 * c)) & 0x80u) v[c] = p.slope == 0.f ? 0.f : v[c] * p.slope;
-        g[c][j] = v[c];
-        bs[c] += v[c];
+        float g[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float v = masked(gv[j][c], gs[j] >> (8 * c), p.slope);
+          g[j] = m0 + j < p.M && gc + c < p.N ? v : 0.f;
+          bs[c] += g[j];
+        }
+        u32x4 a, b, d;
+        cut3(g, a, b, d);
+        const int s = at + slot32(4 * cq + c);
+        sh[s] = a, sh[1024 + s] = b, sh[2048 + s] = d;
+      }
+    } else {
+      float sc[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        sc[j] = p.K > 0 && m0 + j < p.M ? pow2_of((int)__float_as_uint(gv[j][0])) : 0.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        u32x4 x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {   // q 2^s is exact in the upper 16 bits
+          const float e = q8_value((gs[2 * j] >> (8 * c)) & 0xffu, sc[2 * j]);
+          const float o = q8_value((gs[2 * j + 1] >> (8 * c)) & 0xffu, sc[2 * j + 1]);
+          x[j] = __builtin_amdgcn_perm(__float_as_uint(o), __float_as_uint(e), 0x07060302u);
+        }
+        sh[3072 + at + slot32(4 * cq + c)] = x;
       }
     }
-    uint32_t xw[8];
-    float xsc[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t m = m0 + j;
-      const bool in = m < p.M && xk < p.K;
-      xw[j] = in ? *(const uint32_t*)(p.xc + m * p.ld_xc + xk) : 0u;
-      xsc[j] = in ? pow2_of(p.xs[m * p.ss + (xk >> 5)]) : 0.f;
-    }
-    __syncthreads();   // the previous chunk's operand reads are done
-    const int at = (mo >> 1) * 256 + (cq >> 3) * 64 + (mo & 1) * 32;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      u32x4 a, b, d;
-      cut3(g[c], a, b, d);
-      const int s = at + slot32(4 * cq + c);
-      sg[s] = a, sg[1024 + s] = b, sg[2048 + s] = d;
-      u32x4 x;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {   // q 2^s is exact in the upper 16 bits
-        const float e = q8_value((xw[2 * j] >> (8 * c)) & 0xffu, xsc[2 * j]);
-        const float o = q8_value((xw[2 * j + 1] >> (8 * c)) & 0xffu, xsc[2 * j + 1]);
-        x[j] = __builtin_amdgcn_perm(__float_as_uint(o), __float_as_uint(e), 0x07060302u);
-      }
-      sx[s] = x;
-    }
+  };
+  int64_t ch = blockIdx.z;
+  int buf = 0;
+  if (ch < chunks) load(ch);
+  for (; ch < chunks; ch += p.splits) {
+    u32x4* sh = dw_sh + buf;
+    stage(ch, sh);
     __syncthreads();
+    if (ch + p.splits < chunks) load(ch + p.splits);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      u32x4 xf[2];
+      const int o = h * 32 + slot32(l);
+      const int s = ks * 256 + (wave >> 1) * 64 + o;
+      const u32x4 gh = sh[s], gm = sh[1024 + s], gl = sh[2048 + s];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const int t = (wave & 1) * 2 + b;
-        xf[b] = sx[ks * 256 + t * 64 + h * 32 + slot32(l)];
+        const u32x4 xf = sh[3072 + ks * 256 + ((wave & 1) * 2 + b) * 64 + o];
+        f32x16 c = acc[b];
+        c = mma(gl, xf, c), c = mma(gm, xf, c), c = mma(gh, xf, c);
+        acc[b] = c;
       }
+    }
+    buf ^= DW_BUF;
+  }
+  float* dw = p.dw + (int64_t)blockIdx.z * p.stride;
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const int t = (wave >> 1) * 2 + a;
-        const int s = ks * 256 + t * 64 + h * 32 + slot32(l);
-        const u32x4 gh = sg[s], gm = sg[1024 + s], gl = sg[2048 + s];
+  for (int b = 0; b < 2; ++b) {
+    const int k = k0 + (wave & 1) * 64 + b * 32 + l;
+    if (k >= p.K) continue;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          f32x16 c = acc[a][b];
-          c = mma(gl, xf[b], c), c = mma(gm, xf[b], c), c = mma(gh, xf[b], c);
-          acc[a][b] = c;
-        }
-      }
+    for (int i = 0; i < 16; ++i) {
+      const int n = n0 + (wave >> 1) * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
+      if (n < p.N) dw[(int64_t)n * p.K + k] = acc[b][i];
     }
   }
-  float* dw = p.dw + (int64_t)blockIdx.z * p.N * p.K;
-#pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int k = k0 + (wave & 1) * 64 + b * 32 + l;
-      if (k >= p.K) continue;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int n = n0 + (wave >> 1) * 64 + a * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
-        if (n < p.N) dw[(int64_t)n * p.K + k] = acc[a][b][i];
-      }
-    }
   if (p.db && blockIdx.y == 0) {   // 8 row octets per column, added in a fixed order
     __syncthreads();
-    float* red = (float*)sx;
+    float* red = (float*)dw_sh;
+    if (g_side) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) red[mo * 128 + 4 * cq + c] = bs[c];
+      for (int c = 0; c < 4; ++c) red[mo * 128 + 4 * cq + c] = bs[c];
+    }
     __syncthreads();
     if (tid < 128 && n0 + tid < p.N) {
       float s = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) s += red[j * 128 + tid];
-      p.db[(int64_t)blockIdx.z * p.N + n0 + tid] = s;
+      p.db[(int64_t)blockIdx.z * p.stride + n0 + tid] = s;
     }
   }
 }
 
-// out[o] = sum_z part[z * n + o], 8 lanes per output each every 8th split, then a fixed tree
+// dw and db from their partial sums: output o (the first `split_at` of them dw's) is the sum over z
+// of part[z * n + o], 8 lanes each every 8th split, then a fixed tree
 __global__ __launch_bounds__(256) void k_add_splits(const float* __restrict__ part, int splits, int64_t n,
-                                                    float* __restrict__ out) {
+                                                    int64_t split_at, float* __restrict__ dw,
+                                                    float* __restrict__ db) {
   const int z0 = threadIdx.x & 7;
   for (int64_t o = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 3; o < n; o += (int64_t)gridDim.x * 32) {
     float s = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int z = z0; z < splits; z += 8) s += part[(int64_t)z * n + o];
     s += __shfl_xor(s, 1, 8);
     s += __shfl_xor(s, 2, 8);
     s += __shfl_xor(s, 4, 8);
-    if (z0 == 0) out[o] = s;
+    if (z0 == 0) {
+      if (o < split_at) dw[o] = s;
+      else db[o - split_at] = s;
+    }
   }
 }
 
@@ -397,7 +529,7 @@ __global__ __launch_bounds__(256) void k_add_splits(const float* __restrict__ pa
 __global__ __launch_bounds__(256) void k_idw_bwd(int64_t S, int C, const float* __restrict__ w,
                                                  const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                  int64_t ldc, int ss, const float* __restrict__ dh,
-                                                 float* __restrict__ d_out, float* __restrict__ d_w, int vec) {
+                                                 float* __restrict__ d_out, float* __restrict__ d_w) {
   const int lane = threadIdx.x & 63, k = lane >> 3, q = lane & 7;
   for (int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); s < S; s += (int64_t)gridDim.x * 4) {
   const int64_t row = 8 * s + k;
@@ -405,8 +537,8 @@ __global__ __launch_bounds__(256) void k_idw_bwd(int64_t S, int C, const float* 
   float dot = 0.f;
   for (int c = 4 * q; c < C; c += 32) {
     float g[4];
-    if (vec) {
-      const f32x4 a = *(const f32x4*)(dh + s * C + c);
+    if (c + 4 <= C) {
+      const f32x4 a = *(const Octet<float>::half*)(dh + s * C + c);
 #pragma unroll
       for (int j = 0; j < 4; ++j) g[j] = a[j];
     } else {
@@ -421,14 +553,8 @@ __global__ __launch_bounds__(256) void k_idw_bwd(int64_t S, int C, const float* 
         if (c + j < C) dot = fmaf(q8_value((x >> (8 * j)) & 0xffu, sc), g[j], dot);
     }
     if (d_out) {
-      float* o = d_out + row * C + c;
-      if (vec) {
-        *(f32x4*)o = f32x4{wk * g[0], wk * g[1], wk * g[2], wk * g[3]};
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c + j < C) o[j] = wk * g[j];
-      }
+      const float o[4] = {wk * g[0], wk * g[1], wk * g[2], wk * g[3]};
+      store4<APN_F32>(d_out + row * C + c, C - c, o);
     }
   }
   dot += __shfl_xor(dot, 1);
@@ -449,7 +575,7 @@ int pack(const void* x, int64_t M, int64_t K, int64_t ldx, uint8_t* codes, uint8
     const int64_t rows = std::min(piece, M - m), units = rows * upr;
     const E* p = (const E*)x + m * ldx;
     hipLaunchKernelGGL((k_pack<T>), dim3((unsigned)ceil_div(units, 256)), dim3(256), 0, s, p, (uint32_t)units, (int)K,
-                       ldx, (int)vec_rows(p, ldx, T), fast_div((uint32_t)upr), codes + m * upr * 8, scales + m * ss,
+                       ldx, fast_div((uint32_t)upr), codes + m * upr * 8, scales + m * ss,
                        (int)ss);
   }
   return launch_status();
@@ -463,22 +589,40 @@ int unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, vo
     const int64_t rows = std::min(piece, M - m), units = rows * upr;
     E* p = (E*)out + m * ldo;
     hipLaunchKernelGGL((k_unpack<T>), dim3((unsigned)ceil_div(units, 256)), dim3(256), 0, s, codes + m * upr * 8,
-                       scales + m * ss, (uint32_t)units, (int)K, fast_div((uint32_t)upr), (int)ss, p, ldo,
-                       (int)vec_rows(p, ldo, T));
+                       scales + m * ss, (uint32_t)units, (int)K, fast_div((uint32_t)upr), (int)ss, p, ldo);
   }
   return launch_status();
 }
 
 constexpr int64_t MAX_COLS = (int64_t)1 << 20;   // row widths: 32-bit column arithmetic in the kernels
 
-// splits of the weight gradient: at most one per chunk of 64 rows, and about two workgroups a CU
-inline int64_t dw_tiles(int64_t N, int64_t K) { return ((N + 127) / 128) * ((K + 127) / 128); }
+// splits of the weight gradient: at most one per chunk of 64 rows, and about one workgroup a CU
 inline int dw_splits(int64_t M, int64_t N, int64_t K) {
-  const int64_t chunks = (M + 63) / 64;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(chunks, 512 / std::max<int64_t>(1, dw_tiles(N, K))));
+  const int64_t chunks = (M + 63) / 64, tiles = ((N + 127) / 128) * ((K + 127) / 128);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(chunks, 256 / std::max<int64_t>(1, tiles)));
 }
 
-unsigned row_grid(int64_t M) { return (unsigned)std::min<int64_t>((M + BM - 1) / BM, 1 << 20); }
+template <bool WT, bool MASK, bool Q8, int NCH, int NW, int RG>
+void launch_held(const RowArgs& a, hipStream_t s) {
+  // as many workgroups as are resident together, each walking row tiles
+  const int cols = ceil_div(a.C, 32 * NW), per_cu = NW * RG <= 4 ? 2 : 1;
+  const int64_t tiles = (a.M + BM - 1) / BM;
+  hipLaunchKernelGGL((k_rows_held<WT, MASK, Q8, NCH, NW, RG>),
+                     dim3((unsigned)std::min<int64_t>(tiles, std::max(1, 256 * per_cu / cols)), (unsigned)cols),
+                     dim3(64 * NW * RG), 0, s, a);
+}
+
+template <bool WT, bool MASK, bool Q8>
+int launch_rows(const RowArgs& a, hipStream_t s) {
+  if (a.R <= 128 && a.C > 128 && a.C <= 192) launch_held<WT, MASK, Q8, 2, 6, 1>(a, s);   // rows read once, not twice
+  else if (a.R <= 128) launch_held<WT, MASK, Q8, 2, 4, 1>(a, s);
+  else if (a.R <= 192) launch_held<WT, MASK, Q8, 3, 4, 2>(a, s);
+  else
+    hipLaunchKernelGGL((k_rows<WT, MASK, Q8>),
+                       dim3((unsigned)std::min<int64_t>((a.M + BM - 1) / BM, 1 << 20), (unsigned)ceil_div(a.C, 128)),
+                       dim3(256), 0, s, a);
+  return launch_status();
+}
 
 }  // namespace q8
 }  // namespace apn
@@ -516,10 +660,8 @@ extern "C" int apn_q8_linear_fwd(const float* x, int64_t ldx, const float* w, in
   if (M == 0) return APN_OK;
   if (!x || !w || !y || !codes || !scales || (uintptr_t)codes % 16) return APN_ERR_ARG;
   q8::RowArgs a{x,   nullptr, w, bias, y, codes, scales, M, ldx, 0, ldw, ldy, blocks_of(N) * BLK, (int)K, (int)N,
-                (int)scale_stride(N), act, (int)vec_rows(x, ldx, APN_F32), (int)vec_rows(y, ldy, APN_F32), slope};
-  hipLaunchKernelGGL((q8::k_rows<false, false, true>), dim3(q8::row_grid(M), (unsigned)ceil_div(N, q8::BC)), dim3(256),
-                     0, (hipStream_t)stream, a);
-  return launch_status();
+                (int)scale_stride(N), act, slope};
+  return q8::launch_rows<false, false, true>(a, (hipStream_t)stream);
 }
 
 extern "C" int apn_q8_linear_bwd_dx(const float* dy, int64_t ld_dy, const uint8_t* y_codes, float slope,
@@ -530,11 +672,9 @@ extern "C" int apn_q8_linear_bwd_dx(const float* dy, int64_t ld_dy, const uint8_
   if (M == 0) return APN_OK;
   if (!dy || !w || !dx || (uintptr_t)y_codes % 16) return APN_ERR_ARG;
   q8::RowArgs a{dy, y_codes, w, nullptr, dx, nullptr, nullptr, M, ld_dy, blocks_of(N) * BLK, ldw, ld_dx, 0, (int)N,
-                (int)K, 0, 0, (int)vec_rows(dy, ld_dy, APN_F32), (int)vec_rows(dx, ld_dx, APN_F32), slope};
-  const dim3 grid(q8::row_grid(M), (unsigned)ceil_div(K, q8::BC));
-  if (y_codes) hipLaunchKernelGGL((q8::k_rows<true, true, false>), grid, dim3(256), 0, (hipStream_t)stream, a);
-  else hipLaunchKernelGGL((q8::k_rows<true, false, false>), grid, dim3(256), 0, (hipStream_t)stream, a);
-  return launch_status();
+                (int)K, 0, 0, slope};
+  hipStream_t s = (hipStream_t)stream;
+  return y_codes ? q8::launch_rows<true, true, false>(a, s) : q8::launch_rows<true, false, false>(a, s);
 }
 
 extern "C" size_t apn_q8_linear_bwd_dw_workspace_bytes(int64_t M, int64_t N, int64_t K) {
@@ -556,21 +696,16 @@ extern "C" int apn_q8_linear_bwd_dw(const float* dy, int64_t ld_dy, const uint8_
   }
   const int sp = q8::dw_splits(M, N, K);
   if (!dw) K = 0;   // column sums alone: no product columns
+  const int64_t n = N * K + (db ? N : 0);
   float* part = sp > 1 ? (float*)workspace : dw;
-  float* bpart = !db ? nullptr : sp > 1 ? part + (int64_t)sp * N * K : db;
-  q8::DwArgs a{dy, y_codes, x_codes, x_scales, part, bpart, M, ld_dy, blocks_of(N) * BLK, blocks_of(K) * BLK, (int)N,
-               (int)K, (int)scale_stride(K), sp, (int)vec_rows(dy, ld_dy, APN_F32), slope};
+  float* bpart = !db ? nullptr : sp > 1 ? part + N * K : db;
+  q8::DwArgs a{dy, y_codes, x_codes, x_scales, part, bpart, M, ld_dy, blocks_of(N) * BLK, blocks_of(K) * BLK, n, (int)N,
+               (int)K, (int)scale_stride(K), sp, slope};
   hipLaunchKernelGGL(q8::k_dw, dim3((unsigned)ceil_div(N, 128), (unsigned)std::max(1, ceil_div(K, 128)), (unsigned)sp),
-                     dim3(256), 0, s, a);
-  if (sp > 1) {
-    const int64_t n = N * K;
-    if (dw)
-      hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)std::min<int64_t>(ceil_div(n, 32), 4096)), dim3(256), 0, s,
-                         part, sp, n, dw);
-    if (db)
-      hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)std::min<int64_t>(ceil_div(N, 32), 4096)), dim3(256), 0, s,
-                         bpart, sp, N, db);
-  }
+                     dim3(512), 2 * q8::DW_BUF * 16, s, a);
+  if (sp > 1)
+    hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)std::min<int64_t>(ceil_div(n, 32), 4096)), dim3(256), 0, s,
+                       part, sp, n, N * K, dw, db);
   return launch_status();
 }
 
@@ -579,9 +714,8 @@ extern "C" int apn_q8_idw_sum_bwd(int64_t S, int32_t C, const float* w, const ui
   if (S < 0 || C < 1 || C > q8::MAX_COLS) return APN_ERR_ARG;
   if (S == 0) return APN_OK;
   if (!w || !dh || (d_w && (!codes || !scales)) || (uintptr_t)codes % 16) return APN_ERR_ARG;
-  const int vec = C % 4 == 0 && (uintptr_t)dh % 16 == 0 && (uintptr_t)d_out % 16 == 0;
   hipLaunchKernelGGL(q8::k_idw_bwd, dim3((unsigned)std::min<int64_t>((S + 3) / 4, 1 << 20)), dim3(256), 0,
                      (hipStream_t)stream, S, C, w, codes,
-                     scales, blocks_of(C) * BLK, (int)scale_stride(C), dh, d_out, d_w, vec);
+                     scales, blocks_of(C) * BLK, (int)scale_stride(C), dh, d_out, d_w);
   return launch_status();
 }
