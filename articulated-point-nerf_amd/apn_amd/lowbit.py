@@ -264,9 +264,12 @@ def linear_q8_backward(dy: torch.Tensor, weight: torch.Tensor, x_kept: Q8Rows | 
     empty = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dy.device)  # noqa: E731
     dx = dw = db = None
     if want_x:
-        dx = empty(M, K)
+        Kp = -(-K // 4) * 4   # rows of whole 16-byte pieces, as linear's: odd rows written 1.5 x as slowly
+        dx = empty(M, Kp)
         _launch(dev, "apn_q8_linear_bwd_dx", dy.data_ptr(), ld_dy, _addr(mask), sl, w.data_ptr(), ldw, M, N, K,
-                dx.data_ptr(), K)
+                dx.data_ptr(), Kp)
+        if Kp != K:
+            dx = dx[:, :K]
     if want_w or want_b:
         dw = empty(N, K) if want_w else None
         db = empty(N) if want_b else None

@@ -47,12 +47,18 @@ __device__ __forceinline__ float pow2_of(int byte) {   // 2^(byte - 127)
 __device__ __forceinline__ float inv_pow2_of(int byte) {   // 2^(127 - byte); byte 255 (no scale): 0
   return byte == 255 ? 0.f : __uint_as_float((uint32_t)(254 - byte) << 23);
 }
-// One q8 code; inv = inv_pow2_of(byte). |x| inv is exact (a power of two), + 2^23 rounds it half
-// to even into the low mantissa bits. With byte 255 the product is 0 or NaN: fminf drops the NaN
-// to 127, and the block reads back as NaN whatever the code.
-__device__ __forceinline__ uint32_t q8_code(float x, float inv) {
-  const float t = fminf(fabsf(x) * inv, 127.f) + 8388608.f;
-  return (__float_as_uint(t) & 0x7fu) | (x > 0.f ? 0u : 0x80u);
+// Four q8 codes; inv = inv_pow2_of(byte). |x| inv is exact (a power of two), + 2^23 rounds it half
+// to even into the low mantissa byte. With byte 255 the product is 0 or NaN: fminf makes the NaN
+// 127, and the block reads back as NaN whatever the code.
+__device__ __forceinline__ uint32_t q8_codes4(const float* x, float inv) {
+  uint32_t t[4], s = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    t[j] = __float_as_uint(fminf(fabsf(x[j]) * inv, 127.f) + 8388608.f);
+    s |= x[j] > 0.f ? 0u : 0x80u << (8 * j);
+  }
+  const uint32_t lo = __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(t[3], t[2], 0x04000c0cu);
+  return lo | hi | s;
 }
 __device__ __forceinline__ float q8_value(uint32_t code, float scale) {
   const float m = (float)(code & 0x7fu) * scale;

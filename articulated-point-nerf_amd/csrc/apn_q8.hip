@@ -44,9 +44,7 @@ __global__ __launch_bounds__(256) void k_pack(const typename Elem<T>::type* __re
   a = max(a, (uint32_t)__shfl_xor((int)a, 2));
   const int byte = q8_byte(a);
   const float inv = inv_pow2_of(byte);
-  u32x2 w = {0u, 0u};
-#pragma unroll
-  for (int j = 0; j < 8; ++j) w[j >> 2] |= q8_code(v[j], inv) << (8 * (j & 3));
+  const u32x2 w = {q8_codes4(v, inv), q8_codes4(v + 4, inv)};
   if (!live) return;
   *(u32x2*)(codes + (int64_t)m * (8 * upr.d) + c) = w;
   if ((cu & 3) == 0) {
@@ -192,8 +190,8 @@ __device__ __forceinline__ void step(const u32x4* sh, int ks, int t0, int l, int
 
 template <bool Q8, int NT>
 __device__ __forceinline__ void finish_rows(const RowArgs& p, int64_t m0, int c0, int l, int h,
-                                            const f32x16 (&acc)[NT]) {
-  if (c0 >= p.C) return;   // uniform in the wave
+                                            const f32x16 (&acc)[NT], const float* bias) {
+  if (c0 >= p.C) return;   // uniform in the wave; bias: the 32 columns', or null
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int64_t m = m0 + 32 * t + l;
@@ -203,7 +201,7 @@ __device__ __forceinline__ void finish_rows(const RowArgs& p, int64_t m0, int c0
     for (int i = 0; i < 16; ++i) {
       const int c = c0 + 8 * (i >> 2) + 4 * h + (i & 3);
       float v = acc[t][i];
-      if (p.bias) v += p.bias[min(c, p.C - 1)];
+      if (bias) v += bias[8 * (i >> 2) + 4 * h + (i & 3)];
       if (p.act) v = leaky(v, p.slope);
       if (Q8) {
         v = c < p.C ? v : 0.f;
@@ -225,10 +223,7 @@ __device__ __forceinline__ void finish_rows(const RowArgs& p, int64_t m0, int c0
       if (m < p.M) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          uint32_t w = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w |= q8_code(y[4 * j + i], inv) << (8 * i);
-          *(uint32_t*)(p.codes + m * p.ld_codes + c0 + 8 * j + 4 * h) = w;
+          *(uint32_t*)(p.codes + m * p.ld_codes + c0 + 8 * j + 4 * h) = q8_codes4(y + 4 * j, inv);
         }
         if (h == 0) {
           uint8_t* s = p.scales + m * p.ss;
@@ -241,61 +236,222 @@ __device__ __forceinline__ void finish_rows(const RowArgs& p, int64_t m0, int c0
   }
 }
 
-// R <= 64 NCH: each wave keeps its 32 columns' weights, cut, in registers (48 per chunk) and the
-// workgroup -- NW column groups of RG waves, each wave 64 / RG rows -- walks the row tiles; LDS is double-buffered (one barrier per chunk) and the next
-// chunk's rows are on their way to registers while this one is multiplied.
-template <bool WT, bool MASK, bool Q8, int NCH, int NW, int RG>
-__global__ __launch_bounds__(64 * NW * RG, 2) void k_rows_held(RowArgs p) {
-  constexpr int T = 64 * NW * RG, UPT = (512 + T - 1) / T, NT = 2 / RG;
-  __shared__ u32x4 sh[2 * 1536];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int l = lane & 31, h = lane >> 5;
-  const int c0 = (blockIdx.y * NW + wave % NW) * 32, t0 = wave / NW * NT;
-  u32x4 wh[4 * NCH], wm[4 * NCH], wl[4 * NCH];
+// R <= 32 KS, 16 CT columns a workgroup: the columns' weights lie cut in LDS in fragment order, and
+// each of 8 waves streams its own 32 rows (two tiles of 16) from memory straight into fragments of
+// the 16 x 16 x 32 product -- no barrier, every row cut once, and a wave's whole next rows
+// (32 x 32 KS floats) on their way while these are multiplied. The order of the reduction is free:
+// lane (row, q) takes columns 4 q .. 4 q + 3 and 16 + 4 q .. of a step, so that four lanes read 64
+// consecutive bytes of a row with each load, and the weights are laid out to match. (With 32-row
+// tiles and each lane on 64 B of its own, every load touched 64 lines: 77 / 90 us for dX / forward
+// of 203 k x 128 x 128.) A lane's results are 4 of 16 columns of one row.
+// A quad of columns that reaches behind R is read as the row's last four (so R >= 4), and its
+// weights move with it; weights of columns read twice or behind R are zero.
+constexpr int SW = 12, NU = 1;   // waves of a workgroup, 16-row tiles of a wave
+__device__ __forceinline__ int quad_start(int r0, int R) { return min(r0, R - 4); }
+__device__ __forceinline__ bool quad_has(int r0, int j, int R) {   // whether element j is this quad's own
+  const int c = quad_start(r0, R) + j;
+  return c >= r0 && c < R;
+}
+__device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                 0);
+}
+
+// One 32-column block of 16 rows: lane (row, q) holds columns 4 q .. and 16 + 4 q .. (v[0], v[1]).
+// Where things go: addresses of the tile's first row in scalar registers (out, codes, scales), the
+// lane's row and quad as 32-bit byte offsets.
+struct Dest {
+  char* out;
+  uint8_t* codes;
+  uint8_t* scales;
+  uint32_t out_at, codes_at, scales_at;
+  bool live;   // the lane's row exists
+};
+template <bool Q8>
+__device__ __forceinline__ void finish_block(const RowArgs& p, const Dest& d, int c0, int q, const f32x4 (&v)[2],
+                                             const float* bias) {
+  if (c0 >= p.C) return;   // uniform
+  const bool whole = c0 + 32 <= p.C;
+  float y[8];
 #pragma unroll
-  for (int ks = 0; ks < 4 * NCH; ++ks) {
-    float v[8];
-    load_w<WT>(p, c0 + l, 16 * ks + 8 * h, v);
-    cut3(v, wh[ks], wm[ks], wl[ks]);
+  for (int i = 0; i < 8; ++i) y[i] = v[i >> 2][i & 3];
+  if (Q8) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f32x4 b = *(const f32x4*)(bias + 16 * j + 4 * q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[4 * j + i] += b[i];
+    }
+    if (p.act) {   // two loops: the ReLU's select costs one more operation
+      if (p.slope == 0.f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = y[i] <= 0.f ? 0.f : y[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = y[i] > 0.f ? y[i] : y[i] * p.slope;
+      }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = c0 + 16 * (i >> 2) + 4 * q + (i & 3) < p.C ? y[i] : 0.f;
+    }
   }
-  const int64_t tiles = (p.M + BM - 1) / BM;
-  Unit x[UPT];
-  auto load = [&](int64_t m0, int ch) __attribute__((always_inline)) {
-    const bool full = m0 + BM <= p.M && 64 * ch + 64 <= p.R;
+  if (d.live) {
+    float* o = (float*)(d.out + d.out_at) + c0;
+    if (whole) {
 #pragma unroll
-    for (int i = 0; i < UPT; ++i) {
-      const int f = tid + T * i;
-      if (T * UPT == 512 || f < 512) load_unit<MASK>(p, m0 + (f >> 3), 64 * ch + 8 * (f & 7), full, x[i]);
+      for (int j = 0; j < 2; ++j)
+        *(typename Octet<float>::half*)(o + 16 * j) = f32x4{y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) store4<APN_F32>(o + 16 * j, p.C - c0 - 16 * j - 4 * q, y + 4 * j);
+    }
+  }
+  if (Q8) {
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = max(amax, abs_bits(y[i]));
+    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
+    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
+    const int byte = q8_byte(amax);
+    const float inv = inv_pow2_of(byte);
+    if (d.live) {
+      uint8_t* c = d.codes + d.codes_at + c0;
+      *(uint32_t*)c = q8_codes4(y, inv);
+      *(uint32_t*)(c + 16) = q8_codes4(y + 4, inv);
+      if (q == 0) {
+        uint8_t* s = d.scales + d.scales_at;
+        s[c0 >> 5] = (uint8_t)byte;
+        if (c0 + 32 >= p.C)
+          for (int i = (c0 >> 5) + 1; i < p.ss; ++i) s[i] = 0;
+      }
+    }
+  }
+}
+
+template <bool WT, bool MASK, bool Q8, int KS, int CT>
+__global__ __launch_bounds__(64 * SW, SW / 4) void k_rows_stream(RowArgs p) {
+  extern __shared__ u32x4 ws[];   // [plane][step][column tile][lane], then 16 CT biases
+  constexpr int PLANE = KS * CT * 64;
+  float* bias = (float*)(ws + 3 * PLANE);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // the tile's address stays in scalar registers
+  const int l = lane & 15, q = lane >> 4;
+  const int c0 = blockIdx.y * 16 * CT;
+  const int64_t tiles = (p.M + 16 * NU - 1) / (16 * NU), stride = (int64_t)gridDim.x * SW;
+  f32x4 x[KS][NU][2];   // [step][row tile][half of the step]
+  uint32_t s[MASK ? KS : 1][NU][2];
+  // a quad is at (the tile's rows less 32 columns, in scalar registers) + lane bytes + a constant; in
+  // the last step the lane part moves back by `back` where the quad reaches behind R, and stays
+  // positive by the 32 columns
+  const int last = (p.R - 1) / 32;
+  int back[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 32 * last + 16 * i + 4 * q;
+    back[i] = quad_start(r, p.R) - r;
+  }
+  const uint32_t out_at = (uint32_t)l * (uint32_t)p.ld_out * 4u + 16u * q;
+  const uint32_t codes_at = (uint32_t)l * (uint32_t)p.ld_codes + 4u * q, scales_at = (uint32_t)(l * p.ss);
+  uint32_t row[NU];
+  auto load = [&](int64_t tile, int ks) __attribute__((always_inline)) {
+    const char* in = (const char*)(p.in + tile * (16 * NU) * p.ld_in) - 128;
+    const uint8_t* c = MASK ? p.mask + tile * (16 * NU) * p.ld_mask - 32 : nullptr;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      if (ks == 0) row[u] = (uint32_t)min((int64_t)(16 * u + l), p.M - 1 - tile * (16 * NU));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = (ks == last ? back[i] : 0) + 4 * q + 32;   // back + 4 q >= R - 4 - 32 last - 16 > -20
+        x[ks][u][i] =
+            *(const Octet<float>::half*)(in + (uint32_t)(row[u] * (uint32_t)p.ld_in + at) * 4u + (32 * ks + 16 * i) * 4);
+        if (MASK) __builtin_memcpy(&s[ks][u][i], c + (uint32_t)(row[u] * (uint32_t)p.ld_mask + at) + (32 * ks + 16 * i), 4);
+      }
     }
   };
-  int64_t tile = blockIdx.x;
-  if (tile < tiles) load(tile * BM, 0);
-  int buf = 0;
-  for (; tile < tiles; tile += gridDim.x) {
-    f32x16 acc[NT];
+  int64_t tile = blockIdx.x + (int64_t)wave * gridDim.x;
+  if (tile < tiles) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int ks = 0; ks < KS; ++ks)
+      if (32 * ks < p.R) load(tile, ks);
+  }
+#pragma unroll 2
+  for (int f = tid; f < PLANE; f += 64 * SW) {
+    const int ln = f & 63, ct = (f >> 6) % CT, ks = (f >> 6) / CT;
+    const int c = c0 + 16 * ct + (ln & 15), r = 32 * ks + 4 * (ln >> 4), cc = min(c, p.C - 1);
+    float v[8];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
+    for (int i = 0; i < 2; ++i) {
+      const int at = quad_start(r + 16 * i, p.R);
+      if (WT) {
 #pragma unroll
-    for (int ch = 0; ch < NCH; ++ch) {
-      u32x4* s = sh + buf;
+        for (int j = 0; j < 4; ++j) v[4 * i + j] = p.w[(int64_t)(at + j) * p.ldw + cc];
+      } else {
+        const f32x4 a = *(const Octet<float>::half*)(p.w + (int64_t)cc * p.ldw + at);
 #pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-        const int f = tid + T * i;
-        if (T * UPT == 512 || f < 512) stage_unit<MASK>(p, f >> 3, f & 7, x[i], s);
+        for (int j = 0; j < 4; ++j) v[4 * i + j] = a[j];
       }
-      __syncthreads();
-      if (ch + 1 < NCH) load(tile * BM, ch + 1);
-      else if (tile + gridDim.x < tiles) load((tile + gridDim.x) * BM, 0);
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        step<NT>(s, ks, t0, l, h, wh[4 * ch + ks], wm[4 * ch + ks], wl[4 * ch + ks], acc);
-        if (NCH == 3) __builtin_amdgcn_sched_barrier(0);
-      }
-      buf ^= 1536;
     }
-    finish_rows<Q8, NT>(p, tile * BM + 32 * t0, c0, l, h, acc);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c < p.C && quad_has(r + 16 * (j >> 2), j & 3, p.R) ? v[j] : 0.f;
+    u32x4 a, b, d;
+    cut3(v, a, b, d);
+    ws[f] = a, ws[PLANE + f] = b, ws[2 * PLANE + f] = d;
+  }
+  if (Q8 && tid < 16 * CT) bias[tid] = p.bias && c0 + tid < p.C ? p.bias[c0 + tid] : 0.f;
+  __syncthreads();
+  for (; tile < tiles; tile += stride) {
+    asm volatile("" : "+v"(back[0]), "+v"(back[1]));   // or every step's lane address is kept (and spilled)
+    f32x4 acc[CT][NU];
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int u = 0; u < NU; ++u) acc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const bool more = tile + stride < tiles;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if (32 * ks >= p.R) break;
+      u32x4 xh[NU], xm[NU], xl[NU];
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[j] = x[ks][u][j >> 2][j & 3];
+          if (MASK) v[j] = masked(v[j], s[ks][u][j >> 2] >> (8 * (j & 3)), p.slope);
+        }
+        cut3(v, xh[u], xm[u], xl[u]);
+      }
+      if (more) load(tile + stride, ks);
+      // the next weights are read while these are multiplied; the scheduler stays within a step
+      // (left alone it hoists all of them and spills)
+      const u32x4* w = ws + ks * CT * 64 + lane;
+      u32x4 wh = w[0], wm = w[PLANE], wl = w[2 * PLANE];
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+        u32x4 nh, nm, nl;
+        if (t + 1 < CT) nh = w[64 * (t + 1)], nm = w[PLANE + 64 * (t + 1)], nl = w[2 * PLANE + 64 * (t + 1)];
+#pragma unroll
+        for (int i = 0; i < 6; ++i)   // small products first
+#pragma unroll
+          for (int u = 0; u < NU; ++u)
+            acc[t][u] = mma16(i == 0 ? wl : i == 2 || i == 3 ? wm : wh, i == 1 ? xl[u] : i == 2 || i == 4 ? xm[u] : xh[u],
+                              acc[t][u]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (t + 1 < CT) wh = nh, wm = nm, wl = nl;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < CT; t += 2)
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const f32x4 v[2] = {acc[t][u], acc[t + 1][u]};
+        const int64_t m = (tile * NU + u) * 16;
+        const Dest d{(char*)(p.out + m * p.ld_out), p.codes + m * p.ld_codes, p.scales + m * p.ss, out_at, codes_at,
+                     scales_at, l < p.M - m};
+        finish_block<Q8>(p, d, c0 + 16 * t, q, v, bias + 16 * t);
+        __builtin_amdgcn_sched_barrier(0);
+      }
   }
 }
 
@@ -303,9 +459,14 @@ __global__ __launch_bounds__(64 * NW * RG, 2) void k_rows_held(RowArgs p) {
 template <bool WT, bool MASK, bool Q8>
 __global__ __launch_bounds__(256, 2) void k_rows(RowArgs p) {
   __shared__ u32x4 sh[2 * 1536];
+  __shared__ float bias[128];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int l = lane & 31, h = lane >> 5;
   const int c0 = (blockIdx.y * 4 + wave) * 32;
+  if (Q8 && tid < 128) {   // read behind the first chunk's barrier
+    const int c = blockIdx.y * 128 + tid;
+    bias[tid] = p.bias && c < p.C ? p.bias[c] : 0.f;
+  }
   const int nch = (p.R + 63) / 64, last = (p.R - 1) / 16;
   int buf = 0;
   for (int64_t m0 = (int64_t)blockIdx.x * BM; m0 < p.M; m0 += (int64_t)gridDim.x * BM) {
@@ -346,7 +507,7 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowArgs p) {
       }
       buf ^= 1536;
     }
-    finish_rows<Q8, 2>(p, m0, c0, l, h, acc);
+    finish_rows<Q8, 2>(p, m0, c0, l, h, acc, Q8 ? bias + 32 * wave : nullptr);
   }
 }
 
@@ -602,21 +763,22 @@ inline int dw_splits(int64_t M, int64_t N, int64_t K) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(chunks, 256 / std::max<int64_t>(1, tiles)));
 }
 
-template <bool WT, bool MASK, bool Q8, int NCH, int NW, int RG>
-void launch_held(const RowArgs& a, hipStream_t s) {
-  // as many workgroups as are resident together, each walking row tiles
-  const int cols = ceil_div(a.C, 32 * NW), per_cu = NW * RG <= 4 ? 2 : 1;
-  const int64_t tiles = (a.M + BM - 1) / BM;
-  hipLaunchKernelGGL((k_rows_held<WT, MASK, Q8, NCH, NW, RG>),
-                     dim3((unsigned)std::min<int64_t>(tiles, std::max(1, 256 * per_cu / cols)), (unsigned)cols),
-                     dim3(64 * NW * RG), 0, s, a);
+template <bool WT, bool MASK, bool Q8, int KS, int CT>
+void launch_stream(const RowArgs& a, hipStream_t s) {
+  const int cols = ceil_div(a.C, 16 * CT);
+  const int64_t tiles = (a.M + 16 * NU - 1) / (16 * NU);   // one workgroup a CU, at first one tile each
+  hipLaunchKernelGGL((k_rows_stream<WT, MASK, Q8, KS, CT>),
+                     dim3((unsigned)std::min<int64_t>(tiles, std::max(1, 256 / cols)), (unsigned)cols), dim3(64 * SW),
+                     3 * KS * CT * 64 * 16 + 16 * CT * 4, s, a);
 }
 
 template <bool WT, bool MASK, bool Q8>
 int launch_rows(const RowArgs& a, hipStream_t s) {
-  if (a.R <= 128 && a.C > 128 && a.C <= 192) launch_held<WT, MASK, Q8, 2, 6, 1>(a, s);   // rows read once, not twice
-  else if (a.R <= 128) launch_held<WT, MASK, Q8, 2, 4, 1>(a, s);
-  else if (a.R <= 192) launch_held<WT, MASK, Q8, 3, 4, 2>(a, s);
+  // R < 4, or rows so far apart that a tile of them passes 32 bits of bytes: the general kernel
+  const bool stream = a.R >= 4 && a.R <= 192 && a.ld_in < (1 << 24) && a.ld_out < (1 << 24);
+  if (stream && a.R <= 128 && a.C > 128 && a.C <= 192) launch_stream<WT, MASK, Q8, 4, 12>(a, s);   // rows read once, not twice
+  else if (stream && a.R <= 128) launch_stream<WT, MASK, Q8, 4, 8>(a, s);
+  else if (stream) launch_stream<WT, MASK, Q8, 6, 8>(a, s);
   else
     hipLaunchKernelGGL((k_rows<WT, MASK, Q8>),
                        dim3((unsigned)std::min<int64_t>((a.M + BM - 1) / BM, 1 << 20), (unsigned)ceil_div(a.C, 128)),
