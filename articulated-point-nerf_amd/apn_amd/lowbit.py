@@ -30,6 +30,7 @@ __all__ = ["Q8Rows", "q8_pack", "linear_q8", "linear_q8_backward", "sequential_q
 
 BLOCK = 32
 MAX_COLS = 1 << 20
+MAX_LD = 1 << 24     # rows further apart are copied
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -82,7 +83,7 @@ def _addr(t):
 
 def _rows(x, what):
     """x [..., K] as a 2-D tensor with unit column stride and rows that do not overlap, M, K and the
-    row stride (a single row may report any)."""
+    row stride."""
     shape = x.shape
     if not shape or shape[-1] == 0:
         raise ValueError(f"{what}: expected rows of at least one column, got shape {tuple(shape)}")
@@ -92,9 +93,9 @@ def _rows(x, what):
     if len(shape) != 2:
         x = x.detach().reshape(-1, K)
     M, (ld, unit) = x.shape[0], x.stride()
-    if (unit != 1 and K > 1) or (M > 1 and ld < K):
+    if (unit != 1 and K > 1) or (M > 1 and (ld < K or ld >= MAX_LD)):
         return x.detach().contiguous(), M, K, K
-    return x, M, K, max(ld, K)
+    return x, M, K, ld if M > 1 else K
 
 
 def _weight_rows(w, K, what):

@@ -137,6 +137,7 @@ __device__ __forceinline__ void load_w(const RowArgs& p, int c, int r, float (&v
   }
 }
 
+// the gradient through the activation; slope 0 gives 0 whatever g holds
 __device__ __forceinline__ float masked(float g, uint32_t code, float slope) {
   return code & 0x80u ? (slope == 0.f ? 0.f : g * slope) : g;
 }
@@ -517,7 +518,8 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowArgs p) {
 // order. Both operands need 8 consecutive rows m per lane: a thread reads 4 columns of 8 rows of G
 // (threads 0..255) or X' (256..511) and writes the four 8-row pieces in fragment order, column
 // slots xor-ed with bits 3..4 of the column so that the writing lanes (4 columns apart) meet all
-// bank groups.
+// bank groups. While a chunk is multiplied the next one is cut into the other LDS buffer, a column
+// per step, and the two after it are on their way.
 struct DwArgs {
   const float* dy;
   const uint8_t* mask;
@@ -525,7 +527,8 @@ struct DwArgs {
   const uint8_t* xs;
   float* dw;        // partial z at dw + z stride
   float* db;        // partial z at db + z stride, or null
-  int64_t M, ld_dy, ld_mask, ld_xc, stride;
+  int64_t M, stride;
+  uint32_t ld_dy, ld_mask, ld_xc;   // below 2^24: 64 rows stay within 32 bits of bytes
   int N, K, ss, splits;
   float slope;
 };
@@ -534,109 +537,154 @@ __device__ __forceinline__ int slot32(int c) { return (c & 31) ^ ((c >> 3) & 3);
 
 constexpr int DW_BUF = 3 * 1024 + 1024;   // 16-B pieces: three planes of G, one of X'
 
+// One thread's part of a chunk: 8 rows of 4 columns of dY and Y's codes, or of X's codes and scales
+struct DwRows {
+  f32x4 v[8];
+  uint32_t s[8];
+};
+struct DwAt {   // where a thread works
+  int wave, l, h, cq, mo;
+  uint32_t gc, mc, xc;   // its first column of dY, of Y's codes, of X's codes
+};
+
+// Loads of chunk ch (one behind the last: the last one's again). Columns behind the ends are read
+// somewhere in the row: their results are not stored. G: this wave's side.
+template <bool G, bool QUADS, bool MASK>
+__device__ __forceinline__ void dw_load(const DwArgs& p, const DwAt& w, int64_t ch, int64_t chunks, DwRows& x) {
+  const int64_t m0 = min(ch, chunks - 1) * 64;
+  const uint32_t lim = (uint32_t)min((int64_t)63, p.M - 1 - m0);
+  if (G) {
+    const char* q = (const char*)p.dy + m0 * p.ld_dy * 4;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t row = __umul24(min((uint32_t)(8 * w.mo + j), lim), p.ld_dy);
+      if (QUADS) {
+        x.v[j] = *(const Octet<float>::half*)(q + (row + w.gc) * 4u);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x.v[j][c] = *(const float*)(q + (row + min(w.gc + c, (uint32_t)p.N - 1)) * 4u);
+      }
+    }
+    if (MASK) {
+      const uint8_t* c = p.mask + m0 * p.ld_mask;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        x.s[j] = *(const uint32_t*)(c + (__umul24(min((uint32_t)(8 * w.mo + j), lim), p.ld_mask) + w.mc));
+    }
+  } else {
+    const uint8_t* c = p.xc + m0 * p.ld_xc;
+    const uint8_t* s = p.xs + m0 * p.ss;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t row = min((uint32_t)(8 * w.mo + j), lim);
+      x.s[j] = *(const uint32_t*)(c + (__umul24(row, p.ld_xc) + w.xc));
+      x.v[j][0] = __uint_as_float((uint32_t)s[__umul24(row, (uint32_t)p.ss) + (w.xc >> 5)]);
+    }
+  }
+}
+// Column c of the thread's four, cut, as one 8-row piece per plane
+template <bool G, bool MASK>
+__device__ __forceinline__ void dw_stage(const DwArgs& p, const DwAt& w, const DwRows& x, int c, u32x4* sh) {
+  const int s = (w.mo >> 1) * 256 + (w.cq >> 3) * 64 + (w.mo & 1) * 32 + slot32(4 * w.cq + c);
+  if (G) {
+    float g[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = x.v[j][c];
+    u32x4 a, b, d;
+    cut3(g, a, b, d);
+    sh[s] = a, sh[1024 + s] = b, sh[2048 + s] = d;
+  } else {
+    u32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {   // q 2^s is exact in the upper 16 bits; the signs go in pairs
+      const float e = (float)((x.s[2 * j] >> (8 * c)) & 0x7fu) * x.v[2 * j][0];
+      const float o = (float)((x.s[2 * j + 1] >> (8 * c)) & 0x7fu) * x.v[2 * j + 1][0];
+      const uint32_t sign = __builtin_amdgcn_perm(x.s[2 * j + 1], x.s[2 * j], 0x040c000cu + 0x01000100u * c);
+      v[j] = __builtin_amdgcn_perm(__float_as_uint(o), __float_as_uint(e), 0x07060302u) | (sign & 0x80008000u);
+    }
+    sh[3072 + s] = v;
+  }
+}
+// One side's waves: both sides' meet the same barriers.
+template <bool G, bool QUADS, bool MASK>
+__device__ __forceinline__ void dw_side(const DwArgs& p, const DwAt& w, u32x4* sh, f32x16 (&acc)[2], float (&bs)[4]) {
+  const int64_t chunks = (p.M + 63) / 64, step = p.splits;
+  int64_t ch = blockIdx.z;
+  // rows behind the last one as zeros (X's side: as scale 2^-127, times G's zero); G masked, its
+  // column sums taken; X's scale bytes as scales
+  auto ready = [&](int64_t c, DwRows& x) __attribute__((always_inline)) {
+    if (c >= chunks - 1) {
+      const int rows = c < chunks ? (int)(p.M - c * 64) - 8 * w.mo : 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j >= rows) x.v[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (G) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (MASK) x.v[j][i] = masked(x.v[j][i], x.s[j] >> (8 * i), p.slope);
+          bs[i] += x.v[j][i];
+        }
+      } else {
+        x.v[j][0] = pow2_of((int)__float_as_uint(x.v[j][0]));
+      }
+    }
+  };
+  auto multiply = [&](const u32x4* b, int ks) __attribute__((always_inline)) {
+    const int o = w.h * 32 + slot32(w.l);
+    const int s = ks * 256 + (w.wave >> 1) * 64 + o, x = 3072 + ks * 256 + (w.wave & 1) * 128 + o;
+    const u32x4 gh = b[s], gm = b[1024 + s], gl = b[2048 + s], x0 = b[x], x1 = b[x + 64];
+    acc[0] = mma(gl, x0, acc[0]), acc[1] = mma(gl, x1, acc[1]);
+    acc[0] = mma(gm, x0, acc[0]), acc[1] = mma(gm, x1, acc[1]);
+    acc[0] = mma(gh, x0, acc[0]), acc[1] = mma(gh, x1, acc[1]);
+  };
+  DwRows xa, xb;
+  dw_load<G, QUADS, MASK>(p, w, ch, chunks, xa);
+  dw_load<G, QUADS, MASK>(p, w, ch + step, chunks, xb);
+  ready(ch, xa);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) dw_stage<G, MASK>(p, w, xa, c, sh);
+  // one chunk: multiply buffer `at`, stage the next chunk (held in x) into the other buffer (behind
+  // the last chunk: zeros nobody reads), with the one after it on its way
+  auto turn = [&](int at, DwRows& x, DwRows& other) __attribute__((always_inline)) {
+    __syncthreads();
+    dw_load<G, QUADS, MASK>(p, w, ch + 2 * step, chunks, other);
+    ready(ch + step, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      multiply(sh + at, i);
+      dw_stage<G, MASK>(p, w, x, i, sh + (DW_BUF - at));
+    }
+    ch += step;
+  };
+  while (ch < chunks) {
+    turn(0, xb, xa);
+    if (ch >= chunks) break;
+    turn(DW_BUF, xa, xb);
+  }
+}
+
+// QUADS: N a multiple of 4, dY's columns are read in fours
+template <bool QUADS, bool MASK>
 __global__ __launch_bounds__(512, 2) void k_dw(DwArgs p) {
   extern __shared__ u32x4 dw_sh[];   // 2 DW_BUF
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int l = lane & 31, h = lane >> 5;
-  const int n0 = blockIdx.x * 128, k0 = blockIdx.y * 128;
-  const bool g_side = tid < 256;
-  const int cq = tid & 31, mo = (tid & 255) >> 5;   // this thread's 4 columns 4 cq .. and 8 rows 8 mo ..
-  const int gc = n0 + 4 * cq, xk = k0 + 4 * cq;
+  const int tid = threadIdx.x, lane = tid & 63, n0 = blockIdx.x * 128, k0 = blockIdx.y * 128;
+  DwAt w{__builtin_amdgcn_readfirstlane(tid >> 6), lane & 31, lane >> 5, tid & 31, (tid & 255) >> 5};
+  const int n = n0 + 4 * w.cq, wave = w.wave, l = w.l, h = w.h, cq = w.cq, mo = w.mo;
+  const bool g_side = wave < 4;
+  w.gc = (uint32_t)(QUADS ? min(n, p.N - 4) : n);
+  w.mc = (uint32_t)min(n, (int)p.ld_mask - 4);
+  w.xc = (uint32_t)min(k0 + 4 * w.cq, (int)p.ld_xc - 4);
   f32x16 acc[2];
 #pragma unroll
   for (int b = 0; b < 2; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
   float bs[4] = {0.f, 0.f, 0.f, 0.f};
-  f32x4 gv[8];        // G rows, or (X' side) codes and scale
-  uint32_t gs[8];
-  const int64_t chunks = (p.M + 63) / 64;
-  auto load = [&](int64_t ch) __attribute__((always_inline)) {
-    const int64_t m0 = ch * 64 + 8 * mo;
-    if (g_side) {
-      const bool full = gc + 4 <= p.N;
-      const int cc = min(gc, p.N - 1);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int64_t m = min(m0 + j, p.M - 1);
-        const float* q = p.dy + m * p.ld_dy;
-        if (full) {
-          gv[j] = *(const typename Octet<float>::half*)(q + gc);
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) gv[j][c] = q[min(gc + c, p.N - 1)];
-        }
-        gs[j] = p.mask ? *(const uint32_t*)(p.mask + m * p.ld_mask + (cc & ~3)) : 0u;
-      }
-    } else if (p.K > 0) {
-      const int kk = min(xk, (int)p.ld_xc - 4);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int64_t m = min(m0 + j, p.M - 1);
-        gs[j] = *(const uint32_t*)(p.xc + m * p.ld_xc + kk);
-        gv[j][0] = __uint_as_float((uint32_t)p.xs[m * p.ss + (kk >> 5)]);
-      }
-    }
-  };
-  auto stage = [&](int64_t ch, u32x4* sh) __attribute__((always_inline)) {
-    const int64_t m0 = ch * 64 + 8 * mo;
-    const int at = (mo >> 1) * 256 + (cq >> 3) * 64 + (mo & 1) * 32;
-    if (g_side) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float g[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float v = masked(gv[j][c], gs[j] >> (8 * c), p.slope);
-          g[j] = m0 + j < p.M && gc + c < p.N ? v : 0.f;
-          bs[c] += g[j];
-        }
-        u32x4 a, b, d;
-        cut3(g, a, b, d);
-        const int s = at + slot32(4 * cq + c);
-        sh[s] = a, sh[1024 + s] = b, sh[2048 + s] = d;
-      }
-    } else {
-      float sc[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        sc[j] = p.K > 0 && m0 + j < p.M ? pow2_of((int)__float_as_uint(gv[j][0])) : 0.f;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        u32x4 x;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {   // q 2^s is exact in the upper 16 bits
-          const float e = q8_value((gs[2 * j] >> (8 * c)) & 0xffu, sc[2 * j]);
-          const float o = q8_value((gs[2 * j + 1] >> (8 * c)) & 0xffu, sc[2 * j + 1]);
-          x[j] = __builtin_amdgcn_perm(__float_as_uint(o), __float_as_uint(e), 0x07060302u);
-        }
-        sh[3072 + at + slot32(4 * cq + c)] = x;
-      }
-    }
-  };
-  int64_t ch = blockIdx.z;
-  int buf = 0;
-  if (ch < chunks) load(ch);
-  for (; ch < chunks; ch += p.splits) {
-    u32x4* sh = dw_sh + buf;
-    stage(ch, sh);
-    __syncthreads();
-    if (ch + p.splits < chunks) load(ch + p.splits);
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const int o = h * 32 + slot32(l);
-      const int s = ks * 256 + (wave >> 1) * 64 + o;
-      const u32x4 gh = sh[s], gm = sh[1024 + s], gl = sh[2048 + s];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const u32x4 xf = sh[3072 + ks * 256 + ((wave & 1) * 2 + b) * 64 + o];
-        f32x16 c = acc[b];
-        c = mma(gl, xf, c), c = mma(gm, xf, c), c = mma(gh, xf, c);
-        acc[b] = c;
-      }
-    }
-    buf ^= DW_BUF;
-  }
+  if (g_side) dw_side<true, QUADS, MASK>(p, w, dw_sh, acc, bs);
+  else dw_side<false, QUADS, MASK>(p, w, dw_sh, acc, bs);
   float* dw = p.dw + (int64_t)blockIdx.z * p.stride;
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
@@ -662,6 +710,31 @@ __global__ __launch_bounds__(512, 2) void k_dw(DwArgs p) {
       for (int j = 0; j < 8; ++j) s += red[j * 128 + tid];
       p.db[(int64_t)blockIdx.z * p.stride + n0 + tid] = s;
     }
+  }
+}
+
+// db alone (a frozen weight under a trained bias): 64 columns a workgroup, the sums in k_dw's order
+__global__ __launch_bounds__(512) void k_db(DwArgs p) {
+  __shared__ float red[512];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), mo = threadIdx.x >> 6;
+  float s = 0.f;
+  if (c < p.N)
+    for (int64_t m0 = (int64_t)blockIdx.z * 64 + 8 * mo; m0 < p.M; m0 += 64 * (int64_t)p.splits) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int64_t m = min(m0 + j, p.M - 1);
+        const float g = p.dy[m * p.ld_dy + c];
+        const float v = p.mask ? masked(g, p.mask[m * p.ld_mask + c], p.slope) : g;
+        s += m0 + j < p.M ? v : 0.f;
+      }
+    }
+  red[threadIdx.x] = s;
+  __syncthreads();
+  if (mo == 0 && c < p.N) {
+    float t = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t += red[64 * j + threadIdx.x];
+    p.db[(int64_t)blockIdx.z * p.stride + c] = t;
   }
 }
 
@@ -756,6 +829,7 @@ int unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, vo
 }
 
 constexpr int64_t MAX_COLS = (int64_t)1 << 20;   // row widths: 32-bit column arithmetic in the kernels
+constexpr int64_t MAX_LD = (int64_t)1 << 24;     // row strides: 64 rows within 32 bits of bytes
 
 // splits of the weight gradient: at most one per chunk of 64 rows, and about one workgroup a CU
 inline int dw_splits(int64_t M, int64_t N, int64_t K) {
@@ -775,7 +849,7 @@ void launch_stream(const RowArgs& a, hipStream_t s) {
 template <bool WT, bool MASK, bool Q8>
 int launch_rows(const RowArgs& a, hipStream_t s) {
   // R < 4, or rows so far apart that a tile of them passes 32 bits of bytes: the general kernel
-  const bool stream = a.R >= 4 && a.R <= 192 && a.ld_in < (1 << 24) && a.ld_out < (1 << 24);
+  const bool stream = a.R >= 4 && a.R <= 192 && a.ld_in < MAX_LD && a.ld_out < MAX_LD;
   if (stream && a.R <= 128 && a.C > 128 && a.C <= 192) launch_stream<WT, MASK, Q8, 4, 12>(a, s);   // rows read once, not twice
   else if (stream && a.R <= 128) launch_stream<WT, MASK, Q8, 4, 8>(a, s);
   else if (stream) launch_stream<WT, MASK, Q8, 6, 8>(a, s);
@@ -850,7 +924,7 @@ extern "C" int apn_q8_linear_bwd_dw(const float* dy, int64_t ld_dy, const uint8_
   if (M < 0 || N < 1 || K < 1 || N > q8::MAX_COLS || K > q8::MAX_COLS || ld_dy < N) return APN_ERR_ARG;
   if (!dw && !db) return APN_OK;
   if (M > 0 && (!dy || !workspace || (dw && (!x_codes || !x_scales)))) return APN_ERR_ARG;
-  if ((uintptr_t)y_codes % 16 || (uintptr_t)x_codes % 16) return APN_ERR_ARG;
+  if ((uintptr_t)y_codes % 16 || (uintptr_t)x_codes % 16 || ld_dy >= q8::MAX_LD) return APN_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   if (M == 0) {   // no rows: zero gradients
     if (dw) APN_TRY(fill_i32((int*)dw, 0, N * K, s));
@@ -859,12 +933,21 @@ extern "C" int apn_q8_linear_bwd_dw(const float* dy, int64_t ld_dy, const uint8_
   const int sp = q8::dw_splits(M, N, K);
   if (!dw) K = 0;   // column sums alone: no product columns
   const int64_t n = N * K + (db ? N : 0);
-  float* part = sp > 1 ? (float*)workspace : dw;
+  float* part = sp > 1 ? (float*)workspace : dw;   // (null with db alone and one split: not used)
   float* bpart = !db ? nullptr : sp > 1 ? part + N * K : db;
-  q8::DwArgs a{dy, y_codes, x_codes, x_scales, part, bpart, M, ld_dy, blocks_of(N) * BLK, blocks_of(K) * BLK, n, (int)N,
-               (int)K, (int)scale_stride(K), sp, slope};
-  hipLaunchKernelGGL(q8::k_dw, dim3((unsigned)ceil_div(N, 128), (unsigned)std::max(1, ceil_div(K, 128)), (unsigned)sp),
-                     dim3(512), 2 * q8::DW_BUF * 16, s, a);
+  q8::DwArgs a{dy, y_codes, x_codes, x_scales, part, bpart, M, n, (uint32_t)ld_dy, (uint32_t)(blocks_of(N) * BLK),
+               (uint32_t)(blocks_of(K) * BLK), (int)N, (int)K, (int)scale_stride(K), sp, slope};
+  const dim3 grid((unsigned)ceil_div(N, 128), (unsigned)ceil_div(K, 128), (unsigned)sp);
+  if (!dw) {
+    hipLaunchKernelGGL(q8::k_db, dim3((unsigned)ceil_div(N, 64), 1, (unsigned)sp), dim3(512), 0, s, a);
+    if (sp > 1)
+      hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)std::min<int64_t>(ceil_div(n, 32), 4096)), dim3(256), 0, s,
+                         part, sp, n, (int64_t)0, dw, db);
+    return launch_status();
+  }
+  const auto kernel = N % 4 ? (y_codes ? q8::k_dw<false, true> : q8::k_dw<false, false>)
+                            : (y_codes ? q8::k_dw<true, true> : q8::k_dw<true, false>);
+  hipLaunchKernelGGL(kernel, grid, dim3(512), 2 * q8::DW_BUF * 16, s, a);
   if (sp > 1)
     hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)std::min<int64_t>(ceil_div(n, 32), 4096)), dim3(256), 0, s,
                        part, sp, n, N * K, dw, db);
