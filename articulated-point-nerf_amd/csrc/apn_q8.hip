@@ -238,16 +238,16 @@ __device__ __forceinline__ void finish_rows(const RowArgs& p, int64_t m0, int c0
 }
 
 // R <= 32 KS, 16 CT columns a workgroup: the columns' weights lie cut in LDS in fragment order, and
-// each of 8 waves streams its own 32 rows (two tiles of 16) from memory straight into fragments of
-// the 16 x 16 x 32 product -- no barrier, every row cut once, and a wave's whole next rows
-// (32 x 32 KS floats) on their way while these are multiplied. The order of the reduction is free:
+// each of 12 waves streams its own 16 rows at a time from memory straight into fragments of the
+// 16 x 16 x 32 product -- no barrier, every row cut once, and a wave's whole next tile
+// (16 x 32 KS floats) on its way while this one is multiplied. The order of the reduction is free:
 // lane (row, q) takes columns 4 q .. 4 q + 3 and 16 + 4 q .. of a step, so that four lanes read 64
 // consecutive bytes of a row with each load, and the weights are laid out to match. (With 32-row
 // tiles and each lane on 64 B of its own, every load touched 64 lines: 77 / 90 us for dX / forward
 // of 203 k x 128 x 128.) A lane's results are 4 of 16 columns of one row.
 // A quad of columns that reaches behind R is read as the row's last four (so R >= 4), and its
 // weights move with it; weights of columns read twice or behind R are zero.
-constexpr int SW = 12, NU = 1;   // waves of a workgroup, 16-row tiles of a wave
+constexpr int SW = 12;   // waves of a workgroup
 __device__ __forceinline__ int quad_start(int r0, int R) { return min(r0, R - 4); }
 __device__ __forceinline__ bool quad_has(int r0, int j, int R) {   // whether element j is this quad's own
   const int c = quad_start(r0, R) + j;
@@ -258,8 +258,21 @@ __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
                                                  0);
 }
 
-// One 32-column block of 16 rows: lane (row, q) holds columns 4 q .. and 16 + 4 q .. (v[0], v[1]).
-// Where things go: addresses of the tile's first row in scalar registers (out, codes, scales), the
+// r[t] of lane (row, q) to r[q] of lane (row, t), q = lane / 16: two exchanges of register halves
+__device__ __forceinline__ void transpose4(uint32_t (&r)[4]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const auto s = __builtin_amdgcn_permlane32_swap(r[i], r[i + 2], false, false);
+    r[i] = s[0], r[i + 2] = s[1];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const auto s = __builtin_amdgcn_permlane16_swap(r[i], r[i + 1], false, false);
+    r[i] = s[0], r[i + 1] = s[1];
+  }
+}
+
+// Where a tile's results go: addresses of its first row in scalar registers (out, codes, scales), the
 // lane's row and quad as 32-bit byte offsets.
 struct Dest {
   char* out;
@@ -268,14 +281,17 @@ struct Dest {
   uint32_t out_at, codes_at, scales_at;
   bool live;   // the lane's row exists
 };
+
+// One 32-column block of 16 rows from c0 on: lane (row, q) holds columns 4 q .. and 16 + 4 q .. . The
+// floats are stored; codes and scale byte are returned.
 template <bool Q8>
-__device__ __forceinline__ void finish_block(const RowArgs& p, const Dest& d, int c0, int q, const f32x4 (&v)[2],
-                                             const float* bias) {
-  if (c0 >= p.C) return;   // uniform
+__device__ __forceinline__ void finish_block(const RowArgs& p, const Dest& d, int c0, int q, const f32x4& v0,
+                                             const f32x4& v1, const float* bias, uint32_t& k0, uint32_t& k1,
+                                             int& byte) {
   const bool whole = c0 + 32 <= p.C;
   float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = v[i >> 2][i & 3];
+  for (int i = 0; i < 4; ++i) y[i] = v0[i], y[4 + i] = v1[i];
   if (Q8) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -314,34 +330,49 @@ __device__ __forceinline__ void finish_block(const RowArgs& p, const Dest& d, in
     for (int i = 0; i < 8; ++i) amax = max(amax, abs_bits(y[i]));
     amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
     amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
-    const int byte = q8_byte(amax);
+    byte = q8_byte(amax);
     const float inv = inv_pow2_of(byte);
-    if (d.live) {
-      uint8_t* c = d.codes + d.codes_at + c0;
-      *(uint32_t*)c = q8_codes4(y, inv);
-      *(uint32_t*)(c + 16) = q8_codes4(y + 4, inv);
-      if (q == 0) {
-        uint8_t* s = d.scales + d.scales_at;
-        s[c0 >> 5] = (uint8_t)byte;
-        if (c0 + 32 >= p.C)
-          for (int i = (c0 >> 5) + 1; i < p.ss; ++i) s[i] = 0;
-      }
-    }
+    k0 = q8_codes4(y, inv), k1 = q8_codes4(y + 4, inv);
+  }
+}
+// Four blocks (NB of them computed) from block b0 on: transposed over the four lanes of a row, lane q
+// stores block q's 32 codes, so that a row's 128 go out as one line (lane by lane as they are
+// computed, 16 B of a row at a time, the stores of 203 k rows took 20 us more), and one lane the
+// scale bytes, with the padding behind the last block.
+template <int NB>
+__device__ __forceinline__ void store_codes(const RowArgs& p, const Dest& d, int b0, int q, uint32_t (&k0)[4],
+                                            uint32_t (&k1)[4], const int (&byte)[4]) {
+  transpose4(k0);
+  transpose4(k1);
+  const int nb = (p.C + 31) / 32;
+  if (!d.live) return;
+  if (q < NB && b0 + q < nb) {
+    uint8_t* c = d.codes + d.codes_at + (b0 + q) * 32;
+    *(u32x4*)c = u32x4{k0[0], k0[1], k0[2], k0[3]};
+    *(u32x4*)(c + 16) = u32x4{k1[0], k1[1], k1[2], k1[3]};
+  }
+  if (q == 0) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) w |= b0 + i < nb ? (uint32_t)byte[i] << (8 * i) : 0u;
+    uint8_t* s = d.scales + d.scales_at + b0;
+    if (b0 % 4 == 0 && (NB == 4 || b0 + NB >= nb)) *(uint32_t*)s = w;   // scale rows are whole words
+    else *(uint16_t*)s = (uint16_t)w;
   }
 }
 
 template <bool WT, bool MASK, bool Q8, int KS, int CT>
 __global__ __launch_bounds__(64 * SW, SW / 4) void k_rows_stream(RowArgs p) {
   extern __shared__ u32x4 ws[];   // [plane][step][column tile][lane], then 16 CT biases
-  constexpr int PLANE = KS * CT * 64;
+  constexpr int PLANE = KS * CT * 64, MG = (KS + 3) / 4;
   float* bias = (float*)(ws + 3 * PLANE);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // the tile's address stays in scalar registers
   const int l = lane & 15, q = lane >> 4;
   const int c0 = blockIdx.y * 16 * CT;
-  const int64_t tiles = (p.M + 16 * NU - 1) / (16 * NU), stride = (int64_t)gridDim.x * SW;
-  f32x4 x[KS][NU][2];   // [step][row tile][half of the step]
-  uint32_t s[MASK ? KS : 1][NU][2];
+  const int64_t tiles = (p.M + 15) / 16, stride = (int64_t)gridDim.x * SW;
+  f32x4 x[KS][2];   // [step][half of the step]
+  u32x4 s[MASK ? MG : 1][2];
   // a quad is at (the tile's rows less 32 columns, in scalar registers) + lane bytes + a constant; in
   // the last step the lane part moves back by `back` where the quad reaches behind R, and stays
   // positive by the 32 columns
@@ -353,21 +384,26 @@ __global__ __launch_bounds__(64 * SW, SW / 4) void k_rows_stream(RowArgs p) {
     back[i] = quad_start(r, p.R) - r;
   }
   const uint32_t out_at = (uint32_t)l * (uint32_t)p.ld_out * 4u + 16u * q;
-  const uint32_t codes_at = (uint32_t)l * (uint32_t)p.ld_codes + 4u * q, scales_at = (uint32_t)(l * p.ss);
-  uint32_t row[NU];
+  const uint32_t codes_at = (uint32_t)l * (uint32_t)p.ld_codes, scales_at = (uint32_t)(l * p.ss);
+  uint32_t row;
   auto load = [&](int64_t tile, int ks) __attribute__((always_inline)) {
-    const char* in = (const char*)(p.in + tile * (16 * NU) * p.ld_in) - 128;
-    const uint8_t* c = MASK ? p.mask + tile * (16 * NU) * p.ld_mask - 32 : nullptr;
+    const char* in = (const char*)(p.in + tile * 16 * p.ld_in) - 128;
+    if (ks == 0) {
+      row = (uint32_t)min((int64_t)l, p.M - 1 - tile * 16);
+      if (MASK) {   // lane q: the 32 codes of step 4 g + q
+        const uint8_t* c = p.mask + tile * 16 * p.ld_mask + row * (uint32_t)p.ld_mask;
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      if (ks == 0) row[u] = (uint32_t)min((int64_t)(16 * u + l), p.M - 1 - tile * (16 * NU));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = (ks == last ? back[i] : 0) + 4 * q + 32;   // back + 4 q >= R - 4 - 32 last - 16 > -20
-        x[ks][u][i] =
-            *(const Octet<float>::half*)(in + (uint32_t)(row[u] * (uint32_t)p.ld_in + at) * 4u + (32 * ks + 16 * i) * 4);
-        if (MASK) __builtin_memcpy(&s[ks][u][i], c + (uint32_t)(row[u] * (uint32_t)p.ld_mask + at) + (32 * ks + 16 * i), 4);
+        for (int g = 0; g < MG; ++g) {
+          const u32x4* at = (const u32x4*)(c + 32 * min(4 * g + q, last));
+          s[g][0] = at[0], s[g][1] = at[1];
+        }
       }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = (ks == last ? back[i] : 0) + 4 * q + 32;   // back + 4 q >= R - 4 - 32 last - 16 > -20
+      x[ks][i] =
+          *(const Octet<float>::half*)(in + (uint32_t)(row * (uint32_t)p.ld_in + at) * 4u + (32 * ks + 16 * i) * 4);
     }
   };
   int64_t tile = blockIdx.x + (int64_t)wave * gridDim.x;
@@ -403,26 +439,39 @@ __global__ __launch_bounds__(64 * SW, SW / 4) void k_rows_stream(RowArgs p) {
   __syncthreads();
   for (; tile < tiles; tile += stride) {
     asm volatile("" : "+v"(back[0]), "+v"(back[1]));   // or every step's lane address is kept (and spilled)
-    f32x4 acc[CT][NU];
+    f32x4 acc[CT];
 #pragma unroll
-    for (int t = 0; t < CT; ++t)
+    for (int t = 0; t < CT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    uint32_t code[MASK ? 4 * MG : 1][2];   // [step][half]: the quads' codes, brought to their lanes
+    if (MASK) {
 #pragma unroll
-      for (int u = 0; u < NU; ++u) acc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int g = 0; g < MG; ++g)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t r[4] = {s[g][i][0], s[g][i][1], s[g][i][2], s[g][i][3]};
+          transpose4(r);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) code[4 * g + k][i] = r[k];
+        }
+    }
     const bool more = tile + stride < tiles;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       if (32 * ks >= p.R) break;
-      u32x4 xh[NU], xm[NU], xl[NU];
+      u32x4 xh, xm, xl;
+      float v[8];
 #pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          v[j] = x[ks][u][j >> 2][j & 3];
-          if (MASK) v[j] = masked(v[j], s[ks][u][j >> 2] >> (8 * (j & 3)), p.slope);
+      for (int i = 0; i < 2; ++i) {
+        uint32_t k = 0;
+        if (MASK) {   // a quad that moved back has its own columns' codes that many bytes up
+          k = code[ks][i];
+          if (ks == last) k <<= 8 * min(-back[i], 3);
         }
-        cut3(v, xh[u], xm[u], xl[u]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[4 * i + j] = MASK ? masked(x[ks][i][j], k >> (8 * j), p.slope) : x[ks][i][j];
       }
+      cut3(v, xh, xm, xl);
       if (more) load(tile + stride, ks);
       // the next weights are read while these are multiplied; the scheduler stays within a step
       // (left alone it hoists all of them and spills)
@@ -432,27 +481,34 @@ __global__ __launch_bounds__(64 * SW, SW / 4) void k_rows_stream(RowArgs p) {
       for (int t = 0; t < CT; ++t) {
         u32x4 nh, nm, nl;
         if (t + 1 < CT) nh = w[64 * (t + 1)], nm = w[PLANE + 64 * (t + 1)], nl = w[2 * PLANE + 64 * (t + 1)];
-#pragma unroll
-        for (int i = 0; i < 6; ++i)   // small products first
-#pragma unroll
-          for (int u = 0; u < NU; ++u)
-            acc[t][u] = mma16(i == 0 ? wl : i == 2 || i == 3 ? wm : wh, i == 1 ? xl[u] : i == 2 || i == 4 ? xm[u] : xh[u],
-                              acc[t][u]);
+        f32x4 a = acc[t];
+        a = mma16(wl, xh, a), a = mma16(wh, xl, a), a = mma16(wm, xm, a);   // small products first
+        a = mma16(wm, xh, a), a = mma16(wh, xm, a), a = mma16(wh, xh, a);
+        acc[t] = a;
         __builtin_amdgcn_sched_barrier(0);
         if (t + 1 < CT) wh = nh, wm = nm, wl = nl;
       }
     }
+    const int64_t m = tile * 16;
+    const Dest d{(char*)(p.out + m * p.ld_out), p.codes + m * p.ld_codes, p.scales + m * p.ss, out_at, codes_at,
+                 scales_at, l < p.M - m};
 #pragma unroll
-    for (int t = 0; t < CT; t += 2)
+    for (int g = 0; g < CT / 2; g += 4) {
+      constexpr int LAST = CT / 2 % 4 ? CT / 2 % 4 : 4;   // blocks of the last group
+      uint32_t k0[4] = {0, 0, 0, 0}, k1[4] = {0, 0, 0, 0};
+      int byte[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        const f32x4 v[2] = {acc[t][u], acc[t + 1][u]};
-        const int64_t m = (tile * NU + u) * 16;
-        const Dest d{(char*)(p.out + m * p.ld_out), p.codes + m * p.ld_codes, p.scales + m * p.ss, out_at, codes_at,
-                     scales_at, l < p.M - m};
-        finish_block<Q8>(p, d, c0 + 16 * t, q, v, bias + 16 * t);
+      for (int t = g; t < g + 4 && t < CT / 2; ++t) {
+        if (c0 + 32 * t < p.C)
+          finish_block<Q8>(p, d, c0 + 32 * t, q, acc[2 * t], acc[2 * t + 1], bias + 32 * t, k0[t - g], k1[t - g],
+                           byte[t - g]);
         __builtin_amdgcn_sched_barrier(0);
       }
+      if (Q8) {
+        if (g + 4 <= CT / 2) store_codes<4>(p, d, c0 / 32 + g, q, k0, k1, byte);
+        else store_codes<LAST>(p, d, c0 / 32 + g, q, k0, k1, byte);
+      }
+    }
   }
 }
 
@@ -512,8 +568,8 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowArgs p) {
   }
 }
 
-// Weight gradient: dW[n][k] = sum_m G[m][n] X'[m][k], db[n] = sum_m G[m][n], 128 x 128 outputs per
-// workgroup of 8 waves, wave (i, j) 32 x 64 of them, the rows in chunks of 64 over the splits
+// Weight gradient: dW[n][k] = sum_m G[m][n] X'[m][k], db[n] = sum_m G[m][n], 128 x 64 KT outputs per
+// workgroup of 8 waves, wave (i, j) 32 x 32 KT of them, the rows in chunks of 64 over the splits
 // (blockIdx.z takes every splits-th chunk), partial sums to the workspace and added in a fixed
 // order. Both operands need 8 consecutive rows m per lane: a thread reads 4 columns of 8 rows of G
 // (threads 0..255) or X' (256..511) and writes the four 8-row pieces in fragment order, column
@@ -535,21 +591,23 @@ struct DwArgs {
 
 __device__ __forceinline__ int slot32(int c) { return (c & 31) ^ ((c >> 3) & 3); }
 
-constexpr int DW_BUF = 3 * 1024 + 1024;   // 16-B pieces: three planes of G, one of X'
+// 16-B pieces of a buffer: three planes of G, one of X'
+template <int KT> constexpr int DW_BUF = 3 * 1024 + 512 * KT;
 
 // One thread's part of a chunk: 8 rows of 4 columns of dY and Y's codes, or of X's codes and scales
+// (v[j][0]; with KT = 3 two more columns' in the upper halves: codes t[j], scale v[j][1])
 struct DwRows {
   f32x4 v[8];
-  uint32_t s[8];
+  uint32_t s[8], t[8];
 };
 struct DwAt {   // where a thread works
   int wave, l, h, cq, mo;
-  uint32_t gc, mc, xc;   // its first column of dY, of Y's codes, of X's codes
+  uint32_t gc, mc, xc, xd;   // its first column of dY, of Y's codes, of X's codes (and of the two more)
 };
 
 // Loads of chunk ch (one behind the last: the last one's again). Columns behind the ends are read
 // somewhere in the row: their results are not stored. G: this wave's side.
-template <bool G, bool QUADS, bool MASK>
+template <bool G, bool QUADS, bool MASK, int KT>
 __device__ __forceinline__ void dw_load(const DwArgs& p, const DwAt& w, int64_t ch, int64_t chunks, DwRows& x) {
   const int64_t m0 = min(ch, chunks - 1) * 64;
   const uint32_t lim = (uint32_t)min((int64_t)63, p.M - 1 - m0);
@@ -579,35 +637,47 @@ __device__ __forceinline__ void dw_load(const DwArgs& p, const DwAt& w, int64_t 
       const uint32_t row = min((uint32_t)(8 * w.mo + j), lim);
       x.s[j] = *(const uint32_t*)(c + (__umul24(row, p.ld_xc) + w.xc));
       x.v[j][0] = __uint_as_float((uint32_t)s[__umul24(row, (uint32_t)p.ss) + (w.xc >> 5)]);
+      if (KT == 3) {
+        x.t[j] = *(const uint16_t*)(c + (__umul24(row, p.ld_xc) + w.xd));
+        x.v[j][1] = __uint_as_float((uint32_t)s[__umul24(row, (uint32_t)p.ss) + (w.xd >> 5)]);
+      }
     }
   }
 }
-// Column c of the thread's four, cut, as one 8-row piece per plane
-template <bool G, bool MASK>
-__device__ __forceinline__ void dw_stage(const DwArgs& p, const DwAt& w, const DwRows& x, int c, u32x4* sh) {
-  const int s = (w.mo >> 1) * 256 + (w.cq >> 3) * 64 + (w.mo & 1) * 32 + slot32(4 * w.cq + c);
+// byte c of 8 rows' codes with their scales as bf16 values: q 2^s is exact in the upper 16 bits; the
+// signs go in pairs
+__device__ __forceinline__ u32x4 dw_values(const uint32_t (&s)[8], const f32x4 (&v)[8], int c, int k) {
+  u32x4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float e = (float)((s[2 * j] >> (8 * c)) & 0x7fu) * v[2 * j][k];
+    const float o = (float)((s[2 * j + 1] >> (8 * c)) & 0x7fu) * v[2 * j + 1][k];
+    const uint32_t sign = __builtin_amdgcn_perm(s[2 * j + 1], s[2 * j], 0x040c000cu + 0x01000100u * c);
+    r[j] = __builtin_amdgcn_perm(__float_as_uint(o), __float_as_uint(e), 0x07060302u) | (sign & 0x80008000u);
+  }
+  return r;
+}
+// Column c of the thread's four, cut, as one 8-row piece per plane (and, c < 2, of the two more)
+template <bool G, int KT>
+__device__ __forceinline__ void dw_stage(const DwAt& w, const DwRows& x, int c, u32x4* sh) {
+  const int row = (w.mo & 1) * 32, ks = w.mo >> 1, col = (w.cq >> 3) * 64 + row + slot32(4 * w.cq + c);
   if (G) {
     float g[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) g[j] = x.v[j][c];
     u32x4 a, b, d;
     cut3(g, a, b, d);
+    const int s = ks * 256 + col;
     sh[s] = a, sh[1024 + s] = b, sh[2048 + s] = d;
   } else {
-    u32x4 v;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {   // q 2^s is exact in the upper 16 bits; the signs go in pairs
-      const float e = (float)((x.s[2 * j] >> (8 * c)) & 0x7fu) * x.v[2 * j][0];
-      const float o = (float)((x.s[2 * j + 1] >> (8 * c)) & 0x7fu) * x.v[2 * j + 1][0];
-      const uint32_t sign = __builtin_amdgcn_perm(x.s[2 * j + 1], x.s[2 * j], 0x040c000cu + 0x01000100u * c);
-      v[j] = __builtin_amdgcn_perm(__float_as_uint(o), __float_as_uint(e), 0x07060302u) | (sign & 0x80008000u);
-    }
-    sh[3072 + s] = v;
+    u32x4* xs = sh + 3072 + ks * (128 * KT);
+    xs[col] = dw_values(x.s, x.v, c, 0);
+    if (KT == 3 && c < 2) xs[256 + (w.cq >> 4) * 64 + row + slot32(2 * w.cq + c)] = dw_values(x.t, x.v, c, 1);
   }
 }
 // One side's waves: both sides' meet the same barriers.
-template <bool G, bool QUADS, bool MASK>
-__device__ __forceinline__ void dw_side(const DwArgs& p, const DwAt& w, u32x4* sh, f32x16 (&acc)[2], float (&bs)[4]) {
+template <bool G, bool QUADS, bool MASK, int KT>
+__device__ __forceinline__ void dw_side(const DwArgs& p, const DwAt& w, u32x4* sh, f32x16 (&acc)[KT], float (&bs)[4]) {
   const int64_t chunks = (p.M + 63) / 64, step = p.splits;
   int64_t ch = blockIdx.z;
   // rows behind the last one as zeros (X's side: as scale 2^-127, times G's zero); G masked, its
@@ -628,67 +698,74 @@ __device__ __forceinline__ void dw_side(const DwArgs& p, const DwAt& w, u32x4* s
           bs[i] += x.v[j][i];
         }
       } else {
-        x.v[j][0] = pow2_of((int)__float_as_uint(x.v[j][0]));
+#pragma unroll
+        for (int i = 0; i < KT - 1; ++i) x.v[j][i] = pow2_of((int)__float_as_uint(x.v[j][i]));
       }
     }
   };
   auto multiply = [&](const u32x4* b, int ks) __attribute__((always_inline)) {
     const int o = w.h * 32 + slot32(w.l);
-    const int s = ks * 256 + (w.wave >> 1) * 64 + o, x = 3072 + ks * 256 + (w.wave & 1) * 128 + o;
-    const u32x4 gh = b[s], gm = b[1024 + s], gl = b[2048 + s], x0 = b[x], x1 = b[x + 64];
-    acc[0] = mma(gl, x0, acc[0]), acc[1] = mma(gl, x1, acc[1]);
-    acc[0] = mma(gm, x0, acc[0]), acc[1] = mma(gm, x1, acc[1]);
-    acc[0] = mma(gh, x0, acc[0]), acc[1] = mma(gh, x1, acc[1]);
+    const int s = ks * 256 + (w.wave >> 1) * 64 + o;
+    const u32x4* x = b + 3072 + (ks * 2 + (w.wave & 1)) * (64 * KT) + o;
+    const u32x4 g[3] = {b[2048 + s], b[1024 + s], b[s]};   // small products first
+    u32x4 xf[KT];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) xf[t] = x[64 * t];
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+      for (int t = 0; t < KT; ++t) acc[t] = mma(g[i], xf[t], acc[t]);
   };
   DwRows xa, xb;
-  dw_load<G, QUADS, MASK>(p, w, ch, chunks, xa);
-  dw_load<G, QUADS, MASK>(p, w, ch + step, chunks, xb);
+  dw_load<G, QUADS, MASK, KT>(p, w, ch, chunks, xa);
+  dw_load<G, QUADS, MASK, KT>(p, w, ch + step, chunks, xb);
   ready(ch, xa);
 #pragma unroll
-  for (int c = 0; c < 4; ++c) dw_stage<G, MASK>(p, w, xa, c, sh);
+  for (int c = 0; c < 4; ++c) dw_stage<G, KT>(w, xa, c, sh);
   // one chunk: multiply buffer `at`, stage the next chunk (held in x) into the other buffer (behind
   // the last chunk: zeros nobody reads), with the one after it on its way
   auto turn = [&](int at, DwRows& x, DwRows& other) __attribute__((always_inline)) {
     __syncthreads();
-    dw_load<G, QUADS, MASK>(p, w, ch + 2 * step, chunks, other);
+    dw_load<G, QUADS, MASK, KT>(p, w, ch + 2 * step, chunks, other);
     ready(ch + step, x);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       multiply(sh + at, i);
-      dw_stage<G, MASK>(p, w, x, i, sh + (DW_BUF - at));
+      dw_stage<G, KT>(w, x, i, sh + (DW_BUF<KT> - at));
     }
     ch += step;
   };
   while (ch < chunks) {
     turn(0, xb, xa);
     if (ch >= chunks) break;
-    turn(DW_BUF, xa, xb);
+    turn(DW_BUF<KT>, xa, xb);
   }
 }
 
 // QUADS: N a multiple of 4, dY's columns are read in fours
-template <bool QUADS, bool MASK>
+template <bool QUADS, bool MASK, int KT>
 __global__ __launch_bounds__(512, 2) void k_dw(DwArgs p) {
   extern __shared__ u32x4 dw_sh[];   // 2 DW_BUF
-  const int tid = threadIdx.x, lane = tid & 63, n0 = blockIdx.x * 128, k0 = blockIdx.y * 128;
+  const int tid = threadIdx.x, lane = tid & 63, n0 = blockIdx.x * 128, k0 = blockIdx.y * (64 * KT);
   DwAt w{__builtin_amdgcn_readfirstlane(tid >> 6), lane & 31, lane >> 5, tid & 31, (tid & 255) >> 5};
   const int n = n0 + 4 * w.cq, wave = w.wave, l = w.l, h = w.h, cq = w.cq, mo = w.mo;
   const bool g_side = wave < 4;
   w.gc = (uint32_t)(QUADS ? min(n, p.N - 4) : n);
   w.mc = (uint32_t)min(n, (int)p.ld_mask - 4);
   w.xc = (uint32_t)min(k0 + 4 * w.cq, (int)p.ld_xc - 4);
-  f32x16 acc[2];
+  w.xd = (uint32_t)min(k0 + 128 + 2 * w.cq, (int)p.ld_xc - 2);
+  f32x16 acc[KT];
 #pragma unroll
-  for (int b = 0; b < 2; ++b)
+  for (int b = 0; b < KT; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
   float bs[4] = {0.f, 0.f, 0.f, 0.f};
-  if (g_side) dw_side<true, QUADS, MASK>(p, w, dw_sh, acc, bs);
-  else dw_side<false, QUADS, MASK>(p, w, dw_sh, acc, bs);
+  if (g_side) dw_side<true, QUADS, MASK, KT>(p, w, dw_sh, acc, bs);
+  else dw_side<false, QUADS, MASK, KT>(p, w, dw_sh, acc, bs);
   float* dw = p.dw + (int64_t)blockIdx.z * p.stride;
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    const int k = k0 + (wave & 1) * 64 + b * 32 + l;
+  for (int b = 0; b < KT; ++b) {
+    const int k = k0 + (wave & 1) * (32 * KT) + b * 32 + l;
     if (k >= p.K) continue;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -739,22 +816,26 @@ __global__ __launch_bounds__(512) void k_db(DwArgs p) {
 }
 
 // dw and db from their partial sums: output o (the first `split_at` of them dw's) is the sum over z
-// of part[z * n + o], 8 lanes each every 8th split, then a fixed tree
-__global__ __launch_bounds__(256) void k_add_splits(const float* __restrict__ part, int splits, int64_t n,
-                                                    int64_t split_at, float* __restrict__ dw,
-                                                    float* __restrict__ db) {
-  const int z0 = threadIdx.x & 7;
-  for (int64_t o = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 3; o < n; o += (int64_t)gridDim.x * 32) {
-    float s = 0.f;
+// of part[z * n + o]. 64 outputs a workgroup (256-B reads), 16 waves each every 16th split, all its
+// loads in flight together, joined in order.
+__global__ __launch_bounds__(1024) void k_add_splits(const float* __restrict__ part, int splits, int64_t n,
+                                                     int64_t split_at, float* __restrict__ dw,
+                                                     float* __restrict__ db) {
+  __shared__ float red[1024];
+  const int64_t o = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  float s = 0.f;
+  if (o < n) {
 #pragma unroll 8
-    for (int z = z0; z < splits; z += 8) s += part[(int64_t)z * n + o];
-    s += __shfl_xor(s, 1, 8);
-    s += __shfl_xor(s, 2, 8);
-    s += __shfl_xor(s, 4, 8);
-    if (z0 == 0) {
-      if (o < split_at) dw[o] = s;
-      else db[o - split_at] = s;
-    }
+    for (int z = threadIdx.x >> 6; z < splits; z += 16) s += part[(int64_t)z * n + o];
+  }
+  red[threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.x < 64 && o < n) {
+    float t = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) t += red[64 * j + threadIdx.x];
+    if (o < split_at) dw[o] = t;
+    else db[o - split_at] = t;
   }
 }
 
@@ -831,26 +912,56 @@ int unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, vo
 constexpr int64_t MAX_COLS = (int64_t)1 << 20;   // row widths: 32-bit column arithmetic in the kernels
 constexpr int64_t MAX_LD = (int64_t)1 << 24;     // row strides: 64 rows within 32 bits of bytes
 
-// splits of the weight gradient: at most one per chunk of 64 rows, and about one workgroup a CU
+// The weight gradient's tiles are 192 columns wide where one such tile takes the place of two of 128
+// (dY is read once instead of twice).
+inline int dw_width(int64_t K) { return K > 128 && K <= 192 ? 192 : 128; }
+inline int64_t dw_tiles(int64_t N, int64_t K) {
+  const int64_t kw = dw_width(K);
+  return ((N + 127) / 128) * ((K + kw - 1) / kw);
+}
+// Splits of the weight gradient: each takes c chunks of 64 rows, about 2.5 us each, one workgroup a
+// CU at most; a split's partial sums are written and read once, at about 4 TB/s together. The c with
+// the smallest sum of both.
 inline int dw_splits(int64_t M, int64_t N, int64_t K) {
-  const int64_t chunks = (M + 63) / 64, tiles = ((N + 127) / 128) * ((K + 127) / 128);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(chunks, 256 / std::max<int64_t>(1, tiles)));
+  const int64_t chunks = (M + 63) / 64, tiles = dw_tiles(N, K), most = std::max<int64_t>(1, 256 / tiles);
+  const int64_t first = std::max<int64_t>(1, (chunks + most - 1) / most);
+  const double per_split = 8e-6 / 4.0 * (double)(N * (K + 1));   // us
+  int64_t best = first;
+  double cost = 1e30;
+  for (int64_t c = first; c < 4 * first + 8 && c <= chunks; ++c) {
+    const double t = 2.5 * (double)c + per_split * (double)((chunks + c - 1) / c);
+    if (t < cost) cost = t, best = c;
+  }
+  return (int)std::max<int64_t>(1, (chunks + best - 1) / best);
+}
+
+template <int KT>
+void launch_dw(const DwArgs& a, dim3 grid, hipStream_t s) {
+  const auto kernel = a.N % 4 ? (a.mask ? k_dw<false, true, KT> : k_dw<false, false, KT>)
+                              : (a.mask ? k_dw<true, true, KT> : k_dw<true, false, KT>);
+  hipLaunchKernelGGL(kernel, grid, dim3(512), 2 * DW_BUF<KT> * 16, s, a);
 }
 
 template <bool WT, bool MASK, bool Q8, int KS, int CT>
 void launch_stream(const RowArgs& a, hipStream_t s) {
   const int cols = ceil_div(a.C, 16 * CT);
-  const int64_t tiles = (a.M + 16 * NU - 1) / (16 * NU);   // one workgroup a CU, at first one tile each
+  const int64_t tiles = (a.M + 15) / 16;   // one workgroup a CU, at first one tile each
   hipLaunchKernelGGL((k_rows_stream<WT, MASK, Q8, KS, CT>),
                      dim3((unsigned)std::min<int64_t>(tiles, std::max(1, 256 / cols)), (unsigned)cols), dim3(64 * SW),
                      3 * KS * CT * 64 * 16 + 16 * CT * 4, s, a);
 }
 
+constexpr int64_t FEW_TILES = 3072;
+
 template <bool WT, bool MASK, bool Q8>
 int launch_rows(const RowArgs& a, hipStream_t s) {
   // R < 4, or rows so far apart that a tile of them passes 32 bits of bytes: the general kernel
   const bool stream = a.R >= 4 && a.R <= 192 && a.ld_in < MAX_LD && a.ld_out < MAX_LD;
-  if (stream && a.R <= 128 && a.C > 128 && a.C <= 192) launch_stream<WT, MASK, Q8, 4, 12>(a, s);   // rows read once, not twice
+  const bool few = (a.M + 15) / 16 <= FEW_TILES;
+  if (stream && few && a.R <= 128) launch_stream<WT, MASK, Q8, 4, 4>(a, s);
+  else if (stream && few) launch_stream<WT, MASK, Q8, 6, 4>(a, s);
+  else if (stream && a.R <= 128 && a.C > 128 && a.C <= 192)
+    launch_stream<WT, MASK, Q8, 4, 12>(a, s);   // rows read once, not twice
   else if (stream && a.R <= 128) launch_stream<WT, MASK, Q8, 4, 8>(a, s);
   else if (stream) launch_stream<WT, MASK, Q8, 6, 8>(a, s);
   else
@@ -937,20 +1048,18 @@ extern "C" int apn_q8_linear_bwd_dw(const float* dy, int64_t ld_dy, const uint8_
   float* bpart = !db ? nullptr : sp > 1 ? part + N * K : db;
   q8::DwArgs a{dy, y_codes, x_codes, x_scales, part, bpart, M, n, (uint32_t)ld_dy, (uint32_t)(blocks_of(N) * BLK),
                (uint32_t)(blocks_of(K) * BLK), (int)N, (int)K, (int)scale_stride(K), sp, slope};
-  const dim3 grid((unsigned)ceil_div(N, 128), (unsigned)ceil_div(K, 128), (unsigned)sp);
   if (!dw) {
     hipLaunchKernelGGL(q8::k_db, dim3((unsigned)ceil_div(N, 64), 1, (unsigned)sp), dim3(512), 0, s, a);
     if (sp > 1)
-      hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)std::min<int64_t>(ceil_div(n, 32), 4096)), dim3(256), 0, s,
-                         part, sp, n, (int64_t)0, dw, db);
+      hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)ceil_div(n, 64)), dim3(1024), 0, s, part, sp, n, (int64_t)0, dw, db);
     return launch_status();
   }
-  const auto kernel = N % 4 ? (y_codes ? q8::k_dw<false, true> : q8::k_dw<false, false>)
-                            : (y_codes ? q8::k_dw<true, true> : q8::k_dw<true, false>);
-  hipLaunchKernelGGL(kernel, grid, dim3(512), 2 * q8::DW_BUF * 16, s, a);
+  const int width = q8::dw_width(K);
+  const dim3 grid((unsigned)ceil_div(N, 128), (unsigned)ceil_div(K, width), (unsigned)sp);
+  if (width == 192) q8::launch_dw<3>(a, grid, s);
+  else q8::launch_dw<2>(a, grid, s);
   if (sp > 1)
-    hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)std::min<int64_t>(ceil_div(n, 32), 4096)), dim3(256), 0, s,
-                       part, sp, n, N * K, dw, db);
+    hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)ceil_div(n, 64)), dim3(1024), 0, s, part, sp, n, N * K, dw, db);
   return launch_status();
 }
 

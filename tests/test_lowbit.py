@@ -773,7 +773,9 @@ def test_c_entries_refuse_without_gpu():
     assert lib.apn_q8_linear_bwd_dw(p, 8, p, 0.0, None, None, 4, 8, 32, p, p, p, None) == 1
     assert lib.apn_q8_linear_bwd_dw(p, 8, p, 0.0, p, p, 4, 8, 32, p, p, None, None) == 1
     assert lib.apn_q8_linear_bwd_dw(p, 8, p, 0.0, p, p, 4, 8, 32, None, None, None, None) == 0   # nothing asked for
-    assert lib.apn_q8_linear_bwd_dw_workspace_bytes(100000, 128, 128) >= 128 * 129 * 4
+    for M in (0, 1, 63, 64, 65, 1000, 100000, 1 << 40):
+        for N, K in ((1, 1), (128, 128), (128, 191), (1 << 20, 1), (513, 4096)):
+            assert lib.apn_q8_linear_bwd_dw_workspace_bytes(M, N, K) >= N * (K + 1) * 4
     assert lib.apn_q8_idw_sum_bwd(4, 0, p, p, p, p, p, p, None) == 1
     assert lib.apn_mx4_quantize(p, 5, 4, 32, 32, p, p, None) == 1
     assert lib.apn_mx4_dequantize(p, p, 4, 32, p, 0, 16, None) == 1
