@@ -476,17 +476,16 @@ __global__ __launch_bounds__(64 * SW, SW / 4) void k_rows_stream(RowArgs p) {
       // the next weights are read while these are multiplied; the scheduler stays within a step
       // (left alone it hoists all of them and spills)
       const u32x4* w = ws + ks * CT * 64 + lane;
-      u32x4 wh = w[0], wm = w[PLANE], wl = w[2 * PLANE];
 #pragma unroll
-      for (int t = 0; t < CT; ++t) {
-        u32x4 nh, nm, nl;
-        if (t + 1 < CT) nh = w[64 * (t + 1)], nm = w[PLANE + 64 * (t + 1)], nl = w[2 * PLANE + 64 * (t + 1)];
-        f32x4 a = acc[t];
-        a = mma16(wl, xh, a), a = mma16(wh, xl, a), a = mma16(wm, xm, a);   // small products first
-        a = mma16(wm, xh, a), a = mma16(wh, xm, a), a = mma16(wh, xh, a);
-        acc[t] = a;
-        __builtin_amdgcn_sched_barrier(0);
-        if (t + 1 < CT) wh = nh, wm = nm, wl = nl;
+      for (int t = 0; t < CT; t += 2) {
+        const u32x4 wh = w[64 * t], wm = w[PLANE + 64 * t], wl = w[2 * PLANE + 64 * t];
+        const u32x4 vh = w[64 * t + 64], vm = w[PLANE + 64 * t + 64], vl = w[2 * PLANE + 64 * t + 64];
+        f32x4 a = acc[t], b = acc[t + 1];
+        a = mma16(wl, xh, a), b = mma16(vl, xh, b), a = mma16(wh, xl, a), b = mma16(vh, xl, b);
+        a = mma16(wm, xm, a), b = mma16(vm, xm, b), a = mma16(wm, xh, a), b = mma16(vm, xh, b);
+        a = mma16(wh, xm, a), b = mma16(vh, xm, b), a = mma16(wh, xh, a), b = mma16(vh, xh, b);
+        acc[t] = a, acc[t + 1] = b;
+        if (t % 4 == 2) __builtin_amdgcn_sched_barrier(0);
       }
     }
     const int64_t m = tile * 16;
