@@ -104,6 +104,7 @@ SIGNATURES = {
     "apn_mx4_quantize": (C.c_int, [P, I32, I64, I64, I64, P, P, P]),
     "apn_mx4_dequantize": (C.c_int, [P, P, I64, I64, P, I32, I64, P]),
     "apn_mx4_linear": (C.c_int, [P, P, P, P, P, I64, I64, I64, I32, F32, P, I32, I64, P]),
+    "apn_mx4_linear_few": (C.c_int, [P, I32, I64, P, P, P, I64, I64, I64, I32, F32, P, I32, I64, P]),
     "apn_gemm_f32_splitk": (C.c_int, [P, P, P, P, P, I64, I64, I64, I64, I64, I32, I32, F32, I32, P, P]),
 }
 

@@ -31,6 +31,7 @@ __all__ = ["Q8Rows", "q8_pack", "linear_q8", "linear_q8_backward", "sequential_q
 BLOCK = 32
 MAX_COLS = 1 << 20
 MAX_LD = 1 << 24     # rows further apart are copied
+FEW_ROWS = 4         # mx4_linear of so many float rows quantizes them inside the product
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -384,7 +385,14 @@ def mx4_linear(x, weight: MX4Rows, bias: torch.Tensor | None = None, slope: floa
     act, sl = _act(slope, what)
     dev = _device(what, x.codes if isinstance(x, MX4Rows) else x, wc, b)
     if not isinstance(x, MX4Rows):
-        x = mx4_quantize(x)
+        xt = _type(x.dtype, what)
+        rows, M, _, ldx = _rows(x, what)
+        if M <= FEW_ROWS:   # quantized on the way
+            out = torch.empty((M, N), dtype=out_dtype, device=wc.device)
+            _launch(dev, "apn_mx4_linear_few", rows.data_ptr(), xt, ldx, wc.data_ptr(), weight.scales.data_ptr(),
+                    _addr(b), M, N, K, act, sl, out.data_ptr(), t, N)
+            return out
+        x = mx4_quantize(rows)
     M = x.codes.shape[0]
     out = torch.empty((M, N), dtype=out_dtype, device=wc.device)
     _launch(dev, "apn_mx4_linear", x.codes.data_ptr(), x.scales.data_ptr(), wc.data_ptr(), weight.scales.data_ptr(),

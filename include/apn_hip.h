@@ -527,6 +527,10 @@ int apn_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t M, i
 int apn_mx4_linear(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes, const uint8_t* b_scales,
                    const float* bias, int64_t M, int64_t N, int64_t K, int32_t act, float slope, void* out,
                    int32_t type, int64_t ld_out, void* stream);
+/* The same from up to 16 float rows x [M, K] (x_type, row stride ldx), quantized on the way. */
+int apn_mx4_linear_few(const void* x, int32_t x_type, int64_t ldx, const uint8_t* b_codes, const uint8_t* b_scales,
+                       const float* bias, int64_t M, int64_t N, int64_t K, int32_t act, float slope, void* out,
+                       int32_t type, int64_t ld_out, void* stream);
 
 /* Utilities */
 size_t apn_scan_workspace_bytes(int64_t n);
