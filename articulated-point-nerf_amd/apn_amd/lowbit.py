@@ -144,8 +144,8 @@ class _BlockRows:
                 (codes.shape[1], scales.shape[1]) != want:
             raise ValueError(f"{what}: codes [M, {want[0]}] and scales [M, {want[1]}] for {cols} columns, got "
                              f"{tuple(codes.shape)} and {tuple(scales.shape)}")
-        if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() % 16:
-            raise ValueError(f"{what}: contiguous codes (16-byte aligned) and scales")
+        if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() % 16 or scales.data_ptr() % 4:
+            raise ValueError(f"{what}: contiguous codes (16-byte aligned) and scales (4-byte aligned)")
         _device(what, codes, scales)
         self.codes, self.scales, self.cols = codes, scales, cols
 

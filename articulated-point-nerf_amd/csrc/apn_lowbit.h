@@ -130,6 +130,27 @@ __device__ __forceinline__ void store4(typename Elem<T>::type* x, int n, const f
   }
 }
 
+// r[t] of lane (row, q) to r[q] of lane (row, t), q = lane / 16: two exchanges of register halves
+__device__ __forceinline__ void transpose4(uint32_t (&r)[4]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const auto s = __builtin_amdgcn_permlane32_swap(r[i], r[i + 2], false, false);
+    r[i] = s[0], r[i + 2] = s[1];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const auto s = __builtin_amdgcn_permlane16_swap(r[i], r[i + 1], false, false);
+    r[i] = s[0], r[i + 1] = s[1];
+  }
+}
+// the largest of the four lanes of a row (lanes l, l + 16, l + 32, l + 48), in all of them
+__device__ __forceinline__ uint32_t row_max(uint32_t a) {
+  const auto s = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  a = max(s[0], s[1]);
+  const auto t = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  return max(t[0], t[1]);
+}
+
 // activation of the layers' epilogue: v > 0 ? v : slope v; slope 0 (ReLU) gives +0 for -inf and keeps NaN
 __device__ __forceinline__ float leaky(float v, float slope) {
   return v > 0.f ? v : (slope == 0.f ? (v != v ? v : 0.f) : v * slope);

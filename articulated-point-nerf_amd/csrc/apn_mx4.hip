@@ -98,9 +98,82 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, int sa, u32x4 b, int sb, f32x4 c) 
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 4, 4, I, sa, I, sb);
 }
 
+// This workgroup's tile. XCD x (workgroup b: b % 8) takes a run of tiles of its own, in groups of 8
+// row tiles by all column tiles, so that its L2 sees the same operands again.
+template <int RM, int RN>
+__device__ __forceinline__ void tile_of(const Args& p, int64_t& m0, int& n0) {
+  const int64_t tm = (p.M + RM - 1) / RM;
+  const int tn = (p.N + RN - 1) / RN;
+  const int64_t total = tm * tn, b = blockIdx.x, per = total / 8, rest = total % 8, x = b % 8;
+  const int64_t lin = x * per + min(x, rest) + b / 8;
+  const int64_t group = lin / (8 * tn), in_group = lin % (8 * tn), gm = min((int64_t)8, tm - group * 8);
+  m0 = (group * 8 + in_group % gm) * RM;
+  n0 = (int)(in_group / gm) * RN;
+}
+__device__ __forceinline__ f32x4 bias4(const Args& p, int n) {
+  f32x4 b = {0.f, 0.f, 0.f, 0.f};
+  if (p.bias) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) b[r] = p.bias[min(n + r, p.N - 1)];
+  }
+  return b;
+}
+__device__ __forceinline__ void finish4(const Args& p, const f32x4& v, const f32x4& bias, float (&y)[4]) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    y[r] = v[r] + bias[r];
+    if (p.act) y[r] = leaky(y[r], p.slope);
+  }
+}
+// The results of TN column tiles of one row tile, four tiles at a time: 16-bit types are transposed
+// over the four lanes of a row, so that lane q stores the 32 B of tile q and a row's 128 B go out
+// together; floats go out as they are (64 B of a row together). All biases come before any store:
+// a load waited for behind a store waits for the store too.
+template <int T, int TN>
+__device__ __forceinline__ void store_row(const Args& p, int64_t m, int n0, int q, const f32x4 (&acc)[TN],
+                                          const f32x4 (&bias)[TN]) {
+  typedef typename Elem<T>::type E;
+  E* o = (E*)p.out + m * p.ld_out + n0;
+  const int left = p.N - n0;
+#pragma unroll
+  for (int g = 0; g < TN; g += 4) {
+    bool whole = false;
+    if constexpr (T != APN_F32) {
+      whole = g + 4 <= TN && left >= 16 * g + 64;   // uniform
+      if (whole) {
+        typedef E e2 __attribute__((ext_vector_type(2)));
+        typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
+        uint32_t a[4], b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float y[4];
+          finish4(p, acc[(g + j) % TN], bias[(g + j) % TN], y);
+          a[j] = __builtin_bit_cast(uint32_t, e2{(E)y[0], (E)y[1]});
+          b[j] = __builtin_bit_cast(uint32_t, e2{(E)y[2], (E)y[3]});
+        }
+        transpose4(a);
+        transpose4(b);
+        if (m < p.M) {
+          E* d = o + 16 * (g + q);
+          *(u32x4u*)d = u32x4{a[0], b[0], a[1], b[1]};
+          *(u32x4u*)(d + 8) = u32x4{a[2], b[2], a[3], b[3]};
+        }
+      }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int j = g; j < g + 4 && j < TN; ++j) {
+        float y[4];
+        finish4(p, acc[j], bias[j], y);
+        if (m < p.M) store4<T>(o + 16 * j + 4 * q, left - 16 * j - 4 * q, y);
+      }
+    }
+  }
+}
+
 // Tile kernel: WM x WN waves of TM x TN 16 x 16 tiles. Both operands go through LDS in fragment
-// order, one step of 4 blocks (64 B of a row) at a time, double-buffered, the step after the next on
-// its way in registers: 16-B piece (row tile, block, row), the row xor-ed with twice the block so that
+// order, one step of 4 blocks (64 B of a row) at a time, double-buffered, the two steps after the
+// next on their way in registers: 16-B piece (row tile, block, row), the row xor-ed with twice the block so that
 // the lanes that write (4 blocks of 2 rows) and those that read (8 rows of a block) meet all bank
 // groups. Scale bytes go by four steps: a thread reads 16 of one row and writes them transposed, so
 // that a lane's word holds its own block's scales of the four steps and the instruction picks the
@@ -110,71 +183,87 @@ template <int WM, int WN, int TM, int TN, int T>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(Args p) {
   constexpr int THREADS = 64 * WM * WN, RM = 16 * WM * TM, RN = 16 * WN * TN, ROWS = RM + RN;
   constexpr int PIECES = ROWS * 4 / THREADS, BUF = ROWS * 4;
-  static_assert(ROWS * 4 % THREADS == 0 && ROWS <= THREADS && RM % 16 == 0, "piece per thread");
+  static_assert(RM * 4 % THREADS == 0 && RN * 4 % THREADS == 0 && (ROWS < THREADS || ROWS % THREADS == 0) && TN <= TM,
+                "whole passes");
   __shared__ u32x4 sh[2 * BUF];
   __shared__ u32x4 sc[2 * ROWS];
   const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
-  // XCD x (workgroup b: b % 8) takes a run of tiles of its own, in groups of 8 row tiles by all
-  // column tiles, so that its L2 sees the same operands again
-  const int64_t tm = (p.M + RM - 1) / RM;
-  const int tn = (p.N + RN - 1) / RN;
-  const int64_t total = tm * tn, b = blockIdx.x, per = total / 8, rest = total % 8, x = b % 8;
-  const int64_t lin = x * per + min(x, rest) + b / 8;
-  const int64_t group = lin / (8 * tn), in_group = lin % (8 * tn), gm = min((int64_t)8, tm - group * 8);
-  const int64_t m0 = (group * 8 + in_group % gm) * RM;
-  const int n0 = (int)(in_group / gm) * RN;
+  int64_t m0;
+  int n0;
+  tile_of<RM, RN>(p, m0, n0);
   const int steps = (p.nb + 3) / 4;
-  const uint8_t* src[PIECES];
+  // Everything in the loop is read without a branch around it: from a step behind the last one the
+  // last one's again, from a block behind the last one the step's first (and zeroed when stored), so
+  // that no load is waited for before its own store.
+  const int last = steps - 1, c = tid & 3, blocks = p.nb - 4 * last;   // a thread's block; blocks of the last step
+  const uint8_t* const xrow = p.ac + m0 * (p.nb * 16);
+  const uint8_t* const wrow = p.bc + (int64_t)n0 * (p.nb * 16);
+  const uint32_t back = c < blocks ? 0u : 16u * c;
+  uint32_t src[PIECES];
   int dst[PIECES];
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
-    const int f = tid + THREADS * i, row = f >> 2, c = f & 3;
-    const uint8_t* base = row < RM ? p.ac + min(m0 + row, p.M - 1) * (p.nb * 16)
-                                   : p.bc + (int64_t)min(n0 + row - RM, p.N - 1) * (p.nb * 16);
-    src[i] = base + c * 16;
+    const int row = (tid + THREADS * i) >> 2;   // (whole passes: X's rows or B's)
+    const int r = row < RM ? (int)min((int64_t)row, p.M - 1 - m0) : min(row - RM, p.N - 1 - n0);
+    src[i] = (uint32_t)r * (uint32_t)(p.nb * 16) + 16u * c;
     dst[i] = (row >> 4) * 64 + c * 16 + ((row & 15) ^ (2 * c));
   }
-  const uint8_t* scales = tid < RM ? p.as + min(m0 + tid, p.M - 1) * p.ss
-                                   : p.bs + (int64_t)min(n0 + tid - RM, p.N - 1) * p.ss;
   u32x4 piece[PIECES];
+  auto load_piece = [&](int s, int i) __attribute__((always_inline)) {
+    const int at = min(s, last);
+    piece[i] = *(const u32x4*)((THREADS * i < RM * 4 ? xrow : wrow) + (int64_t)at * 64 +
+                               (src[i] - (at == last ? back : 0u)));
+  };
+  auto store_piece = [&](int s, int buf, int i) __attribute__((always_inline)) {
+    if (s == last && blocks < 4) {
+      if (c >= blocks) piece[i] = u32x4{0u, 0u, 0u, 0u};
+    }
+    sh[buf + dst[i]] = piece[i];
+  };
   auto load = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) {   // a block behind the last one: the row's first instead
-      const int c = (tid + THREADS * i) & 3;
-      piece[i] = *(const u32x4*)(src[i] + (4 * s + c < p.nb ? s * 64 : -c * 16));
-    }
+    for (int i = 0; i < PIECES; ++i) load_piece(s, i);
   };
   auto store = [&](int s, int buf) __attribute__((always_inline)) {
-    if (4 * s + 4 > p.nb) {
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i)
-        if (4 * s + ((tid + THREADS * i) & 3) >= p.nb) piece[i] = u32x4{0u, 0u, 0u, 0u};
-    }
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) sh[buf + dst[i]] = piece[i];
+    for (int i = 0; i < PIECES; ++i) store_piece(s, buf, i);
   };
-  u32x4 sv;
+  constexpr int SR = (ROWS + THREADS - 1) / THREADS;   // scale rows of a thread
+  const uint8_t* scales[SR];
+#pragma unroll
+  for (int r = 0; r < SR; ++r) {
+    const int row = min(tid + THREADS * r, ROWS - 1);
+    scales[r] = row < RM ? p.as + min(m0 + row, p.M - 1) * p.ss
+                         : p.bs + (int64_t)min(n0 + row - RM, p.N - 1) * p.ss;
+  }
+  u32x4 sv[SR];
   auto load_scales = [&](int s) __attribute__((always_inline)) {   // of steps s .. s + 3
-    if (ROWS < THREADS && tid >= ROWS) return;
-    if (4 * s + 16 <= p.nb) {
-      __builtin_memcpy(&sv, scales + 4 * s, 16);   // (4-B aligned)
-    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int at = 4 * (s + i), n = p.nb - at;
-        uint32_t w = *(const uint32_t*)(scales + min(at, p.ss - 4));
-        sv[i] = n >= 4 ? w : n <= 0 ? 0u : w & ((1u << (8 * n)) - 1u);
-      }
-    }
+    for (int r = 0; r < SR; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sv[r][i] = *(const uint32_t*)(scales[r] + min(4 * (s + i), p.ss - 4));
   };
-  auto store_scales = [&](int buf) __attribute__((always_inline)) {
-    if (ROWS < THREADS && tid >= ROWS) return;
-    // bytes (step i, block c) to (block c, step i)
-    const uint32_t a = __builtin_amdgcn_perm(sv[1], sv[0], 0x05010400u), b = __builtin_amdgcn_perm(sv[3], sv[2], 0x05010400u);
-    const uint32_t c = __builtin_amdgcn_perm(sv[1], sv[0], 0x07030602u), d = __builtin_amdgcn_perm(sv[3], sv[2], 0x07030602u);
-    sc[buf + tid] = u32x4{__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(b, a, 0x07060302u),
-                          __builtin_amdgcn_perm(d, c, 0x05040100u), __builtin_amdgcn_perm(d, c, 0x07060302u)};
+  auto store_scales = [&](int s, int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < SR; ++r) {   // bytes (step i, block c) to (block c, step i)
+      u32x4 v = sv[r];
+      if (4 * s + 16 > p.nb) {   // zeros behind the last block, whatever the padding holds
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = p.nb - 4 * (s + i);
+          v[i] = n >= 4 ? v[i] : n <= 0 ? 0u : v[i] & ((1u << (8 * n)) - 1u);
+        }
+      }
+      const uint32_t a = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u);
+      const uint32_t b = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u);
+      const uint32_t d = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u);
+      const uint32_t e = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
+      if (ROWS >= THREADS || tid < ROWS)
+        sc[buf + tid + THREADS * r] =
+            u32x4{__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(b, a, 0x07060302u),
+                  __builtin_amdgcn_perm(e, d, 0x05040100u), __builtin_amdgcn_perm(e, d, 0x07060302u)};
+    }
   };
   f32x4 acc[TM][TN];
 #pragma unroll
@@ -182,40 +271,56 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(Args p) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   int sm[TM], sn[TN];
+  u32x4 xf[2][TM], wf[2][TN];   // this step's fragments and the next one's
   const int frag = q * 16 + (l ^ (2 * q));
-  auto multiply = [&](int buf, auto I) __attribute__((always_inline)) {
-    u32x4 w[TN];
+  auto fetch_part = [&](int buf, int m, u32x4 (&x)[TM], u32x4 (&w)[TN]) __attribute__((always_inline)) {
+    x[m] = sh[buf + (wm * TM + m) * 64 + frag];
+    if (m < TN) w[m] = sh[buf + RM * 4 + (wn * TN + m) * 64 + frag];
+  };
+  auto fetch_scales = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j) w[j] = sh[buf + RM * 4 + (wn * TN + j) * 64 + frag];
+    for (int j = 0; j < TM; ++j) sm[j] = ((const int*)(sc + buf + (wm * TM + j) * 16 + l))[q];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const u32x4 x = sh[buf + (wm * TM + i) * 64 + frag];
-#pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = mma<decltype(I)::value>(w[j], sn[j], x, sm[i], acc[i][j]);
-    }
+    for (int j = 0; j < TN; ++j) sn[j] = ((const int*)(sc + buf + RM + (wn * TN + j) * 16 + l))[q];
   };
   load_scales(0);
   load(0);
-  store_scales(0);
+  store_scales(0, 0);
   store(0, 0);
-  if (steps > 1) load(1);
+  load(1);
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < TM; ++m) fetch_part(0, m, xf[0], wf[0]);
+  fetch_scales(0);
+  store(1, BUF);
+  load(2);
   int sbuf = 0;
+  // Step s multiplies the fragments in registers; meanwhile the fragments of s + 1 come from the
+  // buffer that the barrier has just closed, the pieces of s + 2 go into the other one (whose
+  // fragments every wave took before the barrier) and those of s + 3 set out.
   for (int s = 0; s < steps; s += 4) {
     auto turn = [&](auto I) __attribute__((always_inline)) {
       constexpr int i = decltype(I)::value;
       if (i && s + i >= steps) return;
       __syncthreads();
-      if (i == 0) {
+      if (i == 0) load_scales(s + 4);
+      if (i == 2) store_scales(s + 4, sbuf ^ ROWS);
+      // in TM parts, each with its products first in line: a wave issues in order, so a wait for a
+      // piece must not stand before them
 #pragma unroll
-        for (int j = 0; j < TM; ++j) sm[j] = ((const int*)(sc + sbuf + (wm * TM + j) * 16 + l))[q];
+      for (int m = 0; m < TM; ++m) {
+        fetch_part((i & 1) ? 0 : BUF, m, xf[(i & 1) ^ 1], wf[(i & 1) ^ 1]);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) sn[j] = ((const int*)(sc + sbuf + RM + (wn * TN + j) * 16 + l))[q];
-        if (s + 4 < steps) load_scales(s + 4);
+        for (int n = 0; n < TN; ++n) acc[m][n] = mma<i>(wf[i & 1][n], sn[n], xf[i & 1][m], sm[m], acc[m][n]);
+        constexpr int PP = (PIECES + TM - 1) / TM;
+#pragma unroll
+        for (int f = m * PP; f < (m + 1) * PP && f < PIECES; ++f) {
+          store_piece(s + i + 2, (i & 1) ? BUF : 0, f);
+          load_piece(s + i + 3, f);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if (s + i + 1 < steps) store(s + i + 1, (i & 1) ? 0 : BUF);
-      if (s + i + 2 < steps) load(s + i + 2);
-      multiply((i & 1) ? BUF : 0, I);
-      if (i == 3 && s + 4 < steps) store_scales(sbuf ^ ROWS);
+      if (i == 3) fetch_scales(sbuf ^ ROWS);   // (behind the last step: not used)
     };
     turn(std::integral_constant<int, 0>());
     turn(std::integral_constant<int, 1>());
@@ -223,24 +328,171 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(Args p) {
     turn(std::integral_constant<int, 3>());
     sbuf ^= ROWS;
   }
-  typedef typename Elem<T>::type E;
+  f32x4 bias[TN];
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int64_t m = m0 + (wm * TM + i) * 16 + l;
-    E* o = (E*)p.out + m * p.ld_out;
+  for (int j = 0; j < TN; ++j) bias[j] = bias4(p, n0 + (wn * TN + j) * 16 + 4 * q);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int n = n0 + (wn * TN + j) * 16 + 4 * q;
-      float y[4];
+  for (int i = 0; i < TM; ++i)
+    store_row<T, TN>(p, m0 + (wm * TM + i) * 16 + l, n0 + wn * TN * 16, q, acc[i], bias);
+}
+
+// 256 x 256 tile for large products: 4 waves, one per SIMD, each 128 x 128 (256 accumulators), both
+// operands straight from memory into LDS (no registers on the way), four buffers of one step (32 KB)
+// so that three steps are on their way: a step is 0.43 us of matrix work and L2 answers in about 1 us
+// (with one step on its way in registers the 8192 x 4096 x 4096 product took 150 us, with two 119).
+// The LDS side of such a load is lane by lane, so the lanes choose what they read: row lane / 4, and
+// of its four blocks the one that lands conflict-free -- slot 4 r + (c ^ r / 4) of a 16-row tile. The
+// next step's fragments come from LDS while this step's are multiplied.
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+// 64 lanes x W bytes from base + lane bytes to LDS byte address `to` + W lane; arrives under vmcnt
+// (no register is written, so nothing waits for it but the kernel's own s_waitcnt; m0 is set for the
+// load alone, the compiler keeps nothing in it; one wait state between m0 and its use)
+template <int W>
+__device__ __forceinline__ void to_lds(const uint8_t* base, uint32_t lane_bytes, uint32_t to) {
+  if (W == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(lane_bytes), "s"(base)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(lane_bytes), "s"(base)
+                 : "memory");
+}
+// at most N loads out, LDS reads done, all waves here
+template <int N>
+__device__ __forceinline__ void arrive() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+constexpr int TILE256_LDS = 4 * 2 * 256 * 64 + 2 * 2 * 256 * 16;
+
+template <int T>
+__global__ __launch_bounds__(256, 1) void k_tile256(Args p) {
+  constexpr int R = 256, STAGE = 2 * R * 64, SCALES = 2 * R * 16;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // 4 STAGE of codes, 2 SCALES
+  const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave & 1, wn = wave >> 1;
+  int64_t m0;
+  int n0;
+  tile_of<R, R>(p, m0, n0);
+  const int steps = (p.nb + 3) / 4, last = steps - 1, blocks = p.nb - 4 * last;
+  // a wave loads row tiles 8 wave .. 8 wave + 7 of the 32 (X's 16, then B's 16) of a step
+  const int r = lane >> 2, c = (lane & 3) ^ (r >> 2);
+  const uint32_t row_bytes = (uint32_t)p.nb * 16, back = c < blocks ? 0u : 16u * c;
+  const bool xs_side = wave < 2;
+  const uint8_t* const base = xs_side ? p.ac + m0 * row_bytes : p.bc + (int64_t)n0 * row_bytes;
+  const int rows = xs_side ? (int)min((int64_t)R, p.M - m0) : min(R, p.N - n0);   // that exist
+  uint32_t src[8];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        y[r] = acc[i][j][r];
-        if (p.bias) y[r] += p.bias[min(n + r, p.N - 1)];
-        if (p.act) y[r] = leaky(y[r], p.slope);
+  for (int i = 0; i < 8; ++i) src[i] = (uint32_t)min((wave & 1) * 128 + 16 * i + r, rows - 1) * row_bytes + 16u * c;
+  const uint32_t lds0 = lds_at(lds);
+  auto load = [&](int s, int i) __attribute__((always_inline)) {   // (behind the last step: it again)
+    const int at = min(s, last);
+    to_lds<16>(base + (int64_t)at * 64, src[i] - (at == last ? back : 0u), lds0 + (s & 3) * STAGE + (wave * 8 + i) * 1024);
+  };
+  // scales of steps s .. s + 3: 16 B of a row, 64 rows an instruction, where rows of scales are whole
+  // 16-B pieces (K a multiple of 512), else the four words one by one (word j of all rows together)
+  const uint8_t* const sbase = xs_side ? p.as + m0 * p.ss : p.bs + (int64_t)n0 * p.ss;
+  const bool wide = p.ss % 16 == 0 && ((uintptr_t)p.as | (uintptr_t)p.bs) % 16 == 0;
+  uint32_t ssrc[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) ssrc[i] = (uint32_t)min((wave & 1) * 128 + 64 * i + lane, rows - 1) * (uint32_t)p.ss;
+  auto load_scales = [&](int s) __attribute__((always_inline)) {
+    const uint32_t to = lds0 + 4 * STAGE + ((s >> 2) & 1) * SCALES;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (wide) {
+        to_lds<16>(sbase + min(4 * s, p.ss - 16), ssrc[i], to + (wave * 2 + i) * 1024);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          to_lds<4>(sbase + min(4 * (s + j), p.ss - 4), ssrc[i], to + j * 2048 + (wave * 2 + i) * 256);
       }
-      if (m < p.M) store4<T>(o + n, p.N - n, y);
     }
+  };
+  f32x4 acc[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  u32x4 xf[2][8], wf[2][8];
+  int sm[8], sn[8];
+  const int frag = (l * 4 + (q ^ (l >> 2))) * 16;
+  auto fetch = [&](int s, int i, u32x4 (&x)[8], u32x4 (&w)[8]) __attribute__((always_inline)) {
+    const uint8_t* b = lds + (s & 3) * STAGE + frag;
+    x[i] = *(const u32x4*)(b + (wm * 8 + i) * 1024);
+    w[i] = *(const u32x4*)(b + (16 + wn * 8 + i) * 1024);
+  };
+  // byte q of the four steps' words of a row; zero behind the last block, whatever the padding holds
+  const uint32_t pick = 0x0c0c0400u + 0x0101u * q;
+  auto scale_of = [&](const uint8_t* at, int row, int s) __attribute__((always_inline)) {
+    u32x4 v;
+    if (wide) {
+      v = *(const u32x4*)(at + 16 * row);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = *(const uint32_t*)(at + j * 2048 + 4 * row);
+    }
+    uint32_t a = __builtin_amdgcn_perm(v[1], v[0], pick) | __builtin_amdgcn_perm(v[3], v[2], pick) << 16;
+    if (4 * s + 16 > p.nb) {
+      const int n = (p.nb - 4 * s - q + 3) / 4;   // steps whose block q exists
+      a = n >= 4 ? a : n <= 0 ? 0u : a & ((1u << (8 * n)) - 1u);
+    }
+    return (int)a;
+  };
+  auto fetch_scales = [&](int s) __attribute__((always_inline)) {
+    const uint8_t* b = lds + 4 * STAGE + ((s >> 2) & 1) * SCALES;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sm[i] = scale_of(b, (wm * 8 + i) * 16 + l, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sn[i] = scale_of(b, 256 + (wn * 8 + i) * 16 + l, s);
+  };
+  load_scales(0);
+#pragma unroll
+  for (int s = 0; s < 3; ++s)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) load(s, i);
+  arrive<16>();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) fetch(0, i, xf[0], wf[0]);
+  fetch_scales(0);
+  for (int s = 0; s < steps; s += 4) {
+    auto turn = [&](auto I) __attribute__((always_inline)) {
+      constexpr int i = decltype(I)::value;
+      if (i && s + i >= steps) return;
+      // Step s + i + 1 has arrived when no more are out than the last step sent: 8, and the scales
+      // with step 0's. Every wave then has its fragments of the buffer that is written next.
+      if (i != 1) arrive<8>();
+      else if (wide) arrive<10>();
+      else arrive<16>();
+      if (i == 0) load_scales(s + 4);
+      if (s + i == last && blocks < 4) {   // blocks behind the last one: X's codes as zeros
+        asm volatile("");                  // (a branch: as selects they would run in every step)
+#pragma unroll
+        for (int m = 0; m < 8; ++m)
+          if (q >= blocks) xf[i & 1][m] = u32x4{0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+      for (int m = 0; m < 8; ++m) {
+        fetch(s + i + 1, m, xf[(i & 1) ^ 1], wf[(i & 1) ^ 1]);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) acc[m][n] = mma<i>(wf[i & 1][n], sn[n], xf[i & 1][m], sm[m], acc[m][n]);
+        load(s + i + 3, m);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (i == 3) fetch_scales(s + 4);
+    };
+    turn(std::integral_constant<int, 0>());
+    turn(std::integral_constant<int, 1>());
+    turn(std::integral_constant<int, 2>());
+    turn(std::integral_constant<int, 3>());
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in LDS after the end
+  f32x4 bias[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) bias[j] = bias4(p, n0 + (wn * 8 + j) * 16 + 4 * q);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) store_row<T, 8>(p, m0 + (wm * 8 + i) * 16 + l, n0 + wn * 128, q, acc[i], bias);
 }
 
 // Up to 16 rows: 16 columns a workgroup, K over its 8 waves -- two steps (128 B of a row of B, a
@@ -324,12 +576,7 @@ __global__ __launch_bounds__(512) void k_few(FewArgs f) {
     for (int j = 1; j < 8; ++j) t += red[64 * j + lane];
     float y[4];
     const int c = n0 + 4 * q;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      y[r] = t[r];
-      if (p.bias) y[r] += p.bias[min(c + r, p.N - 1)];
-      if (p.act) y[r] = leaky(y[r], p.slope);
-    }
+    finish4(p, t, bias4(p, c), y);
     typedef typename Elem<T>::type E;
     store4<T>((E*)p.out + l * p.ld_out + c, p.N - c, y);
   }
@@ -383,7 +630,8 @@ void launch_linear(const Args& a, hipStream_t s) {
     hipLaunchKernelGGL((k_few<-1, T>), dim3((unsigned)ceil_div(a.N, 16)), dim3(512), 0, s, FewArgs{a, nullptr, 0, 0});
     return;
   }
-  if (tiles_of<2, 4, 8, 4, T>(a) >= 192) launch_tile<2, 4, 8, 4, T>(a, s);
+  if (a.N > 128 && tiles_of<2, 2, 8, 8, T>(a) >= 192)
+    hipLaunchKernelGGL((k_tile256<T>), dim3((unsigned)tiles_of<2, 2, 8, 8, T>(a)), dim3(256), TILE256_LDS, s, a);
   else if (tiles_of<2, 2, 4, 4, T>(a) >= 128) launch_tile<2, 2, 4, 4, T>(a, s);
   else launch_tile<2, 2, 2, 2, T>(a, s);
 }
@@ -406,7 +654,7 @@ extern "C" int apn_mx4_quantize(const void* x, int32_t type, int64_t M, int64_t 
                                 uint8_t* scales, void* stream) {
   if (M < 0 || K < 1 || K > mx4::MAX_COLS || ldx < K || !ok_type(type)) return APN_ERR_ARG;
   if (M == 0) return APN_OK;
-  if (!x || !codes || !scales || (uintptr_t)codes % 16) return APN_ERR_ARG;
+  if (!x || !codes || !scales || (uintptr_t)codes % 16 || (uintptr_t)scales % 4) return APN_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   if (type == APN_F32) return mx4::quantize<APN_F32>(x, M, K, ldx, codes, scales, s);
   if (type == APN_BF16) return mx4::quantize<APN_BF16>(x, M, K, ldx, codes, scales, s);
@@ -417,7 +665,7 @@ extern "C" int apn_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, i
                                   int32_t type, int64_t ldo, void* stream) {
   if (M < 0 || K < 1 || K > mx4::MAX_COLS || ldo < K || !ok_type(type)) return APN_ERR_ARG;
   if (M == 0) return APN_OK;
-  if (!out || !codes || !scales || (uintptr_t)codes % 16) return APN_ERR_ARG;
+  if (!out || !codes || !scales || (uintptr_t)codes % 16 || (uintptr_t)scales % 4) return APN_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   if (type == APN_F32) return mx4::dequantize<APN_F32>(codes, scales, M, K, out, ldo, s);
   if (type == APN_BF16) return mx4::dequantize<APN_BF16>(codes, scales, M, K, out, ldo, s);
@@ -431,6 +679,7 @@ extern "C" int apn_mx4_linear(const uint8_t* a_codes, const uint8_t* a_scales, c
     return APN_ERR_ARG;
   if (M == 0) return APN_OK;
   if (!a_codes || !a_scales || !b_codes || !b_scales || !out) return APN_ERR_ARG;
+  if ((uintptr_t)a_scales % 4 || (uintptr_t)b_scales % 4) return APN_ERR_ARG;
   if ((uintptr_t)a_codes % 16 || (uintptr_t)b_codes % 16) return APN_ERR_ARG;
   // rows per launch: fewer than 2^24 tiles of 64 x 64 (a launch has at most 2^32 threads)
   const int64_t piece = std::max<int64_t>(256, ((int64_t)1 << 35) / (N + 256) / 256 * 256);
@@ -454,7 +703,7 @@ extern "C" int apn_mx4_linear_few(const void* x, int32_t x_type, int64_t ldx, co
       !ok_type(x_type) || !ok_type(type))
     return APN_ERR_ARG;
   if (M == 0) return APN_OK;
-  if (!x || !b_codes || !b_scales || !out || (uintptr_t)b_codes % 16) return APN_ERR_ARG;
+  if (!x || !b_codes || !b_scales || !out || (uintptr_t)b_codes % 16 || (uintptr_t)b_scales % 4) return APN_ERR_ARG;
   const mx4::FewArgs a{{nullptr, nullptr, b_codes, b_scales, bias, out, M, ld_out, (int)N, (int)blocks_of(K),
                         (int)scale_stride(K), act, slope}, x, ldx, (int)K};
   hipStream_t s = (hipStream_t)stream;

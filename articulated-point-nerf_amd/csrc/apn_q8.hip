@@ -258,20 +258,6 @@ __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
                                                  0);
 }
 
-// r[t] of lane (row, q) to r[q] of lane (row, t), q = lane / 16: two exchanges of register halves
-__device__ __forceinline__ void transpose4(uint32_t (&r)[4]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const auto s = __builtin_amdgcn_permlane32_swap(r[i], r[i + 2], false, false);
-    r[i] = s[0], r[i + 2] = s[1];
-  }
-#pragma unroll
-  for (int i = 0; i < 4; i += 2) {
-    const auto s = __builtin_amdgcn_permlane16_swap(r[i], r[i + 1], false, false);
-    r[i] = s[0], r[i + 1] = s[1];
-  }
-}
-
 // Where a tile's results go: addresses of its first row in scalar registers (out, codes, scales), the
 // lane's row and quad as 32-bit byte offsets.
 struct Dest {
@@ -328,9 +314,7 @@ __device__ __forceinline__ void finish_block(const RowArgs& p, const Dest& d, in
     uint32_t amax = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) amax = max(amax, abs_bits(y[i]));
-    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
-    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
-    byte = q8_byte(amax);
+    byte = q8_byte(row_max(amax));
     const float inv = inv_pow2_of(byte);
     k0 = q8_codes4(y, inv), k1 = q8_codes4(y + 4, inv);
   }
@@ -980,7 +964,7 @@ extern "C" int apn_q8_pack(const void* x, int32_t type, int64_t M, int64_t K, in
                            uint8_t* scales, void* stream) {
   if (M < 0 || K < 1 || K > q8::MAX_COLS || ldx < K || !ok_type(type)) return APN_ERR_ARG;
   if (M == 0) return APN_OK;
-  if (!x || !codes || !scales || (uintptr_t)codes % 16) return APN_ERR_ARG;
+  if (!x || !codes || !scales || (uintptr_t)codes % 16 || (uintptr_t)scales % 4) return APN_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   if (type == APN_F32) return q8::pack<APN_F32>(x, M, K, ldx, codes, scales, s);
   if (type == APN_BF16) return q8::pack<APN_BF16>(x, M, K, ldx, codes, scales, s);
@@ -991,7 +975,7 @@ extern "C" int apn_q8_unpack(const uint8_t* codes, const uint8_t* scales, int64_
                              int32_t type, int64_t ldo, void* stream) {
   if (M < 0 || K < 1 || K > q8::MAX_COLS || ldo < K || !ok_type(type)) return APN_ERR_ARG;
   if (M == 0) return APN_OK;
-  if (!out || !codes || !scales || (uintptr_t)codes % 16) return APN_ERR_ARG;
+  if (!out || !codes || !scales || (uintptr_t)codes % 16 || (uintptr_t)scales % 4) return APN_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   if (type == APN_F32) return q8::unpack<APN_F32>(codes, scales, M, K, out, ldo, s);
   if (type == APN_BF16) return q8::unpack<APN_BF16>(codes, scales, M, K, out, ldo, s);
@@ -1004,7 +988,7 @@ extern "C" int apn_q8_linear_fwd(const float* x, int64_t ldx, const float* w, in
   if (M < 0 || N < 1 || K < 1 || N > q8::MAX_COLS || K > q8::MAX_COLS || ldx < K || ldw < K || ldy < N)
     return APN_ERR_ARG;
   if (M == 0) return APN_OK;
-  if (!x || !w || !y || !codes || !scales || (uintptr_t)codes % 16) return APN_ERR_ARG;
+  if (!x || !w || !y || !codes || !scales || (uintptr_t)codes % 16 || (uintptr_t)scales % 4) return APN_ERR_ARG;
   q8::RowArgs a{x,   nullptr, w, bias, y, codes, scales, M, ldx, 0, ldw, ldy, blocks_of(N) * BLK, (int)K, (int)N,
                 (int)scale_stride(N), act, slope};
   return q8::launch_rows<false, false, true>(a, (hipStream_t)stream);

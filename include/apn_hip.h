@@ -483,7 +483,7 @@ int apn_cloud_bbox(const float* xyz, int64_t N, float* out6, int32_t* ord8, void
  * Narrow block formats of the Linear layers. A row of K values is stored in blocks of 32
  * consecutive columns (the last may be shorter), each with one scale 2^(byte - 127) (byte 255:
  * the block held an infinity or NaN and reads back as NaN). Scale rows are padded with zero bytes
- * to 4 ceil(ceil(K / 32) / 4) bytes. Code arrays are 16-B aligned. K, N <= 2^20.
+ * to 4 ceil(ceil(K / 32) / 4) bytes. Code arrays are 16-B aligned, scale arrays 4-B. K, N <= 2^20.
  *   q8:  32 ceil(K / 32) bytes a row, code = (x > 0 ? 0 : 0x80) | min(rint(|x| / scale), 127)
  *        (pad: 0x80); the scale is the smallest that holds the block's largest magnitude, and the
  *        sign bit says "not positive" also where the magnitude rounds to 0.

@@ -535,6 +535,27 @@ def test_mx4_linear_vs_float64(dev, M, K, N, out_dtype):
 
 
 @gpu
+@pytest.mark.parametrize("M,K,N", [(3500, 33, 3600), (3300, 100, 3800), (3500, 700, 3700), (3841, 1000, 3585),
+                                   (2048, 4096, 1536), (33000, 96, 100), (1500, 520, 1600)])
+def test_mx4_linear_many_tiles_vs_float64(dev, M, K, N):
+    """Enough tiles for every tile shape, K with whole and partial steps, scale rows of whole and
+    partial 16-byte pieces; padding bytes of the scales that are not zero are not read."""
+    from apn_amd import lowbit as lb
+    x, w, b, _ = _rand(M, N, K, M + K + N, dev)
+    xq, wq = lb.mx4_quantize(x), lb.mx4_quantize(w)
+    xv, wv = xq.dequantize().double(), wq.dequantize().double()   # (equal to the definition: above)
+    ref = xv @ wv.t() + b.double()
+    S = xv.abs() @ wv.abs().t() + b.double().abs()
+    y = lb.mx4_linear(xq, wq, b)
+    _within(y, ref, (K + 16) * U * S)
+    nb = -(-K // BLOCK)
+    for r in (xq, wq):
+        r.scales[:, nb:] = 255
+    assert torch.equal(lb.mx4_linear(xq, wq, b), y)
+    assert torch.equal(lb.mx4_linear(xq, wq, b, 0.01, torch.bfloat16), _act64(y, 0.01).to(torch.bfloat16))
+
+
+@gpu
 def test_mx4_linear_non_finite_and_empty(dev):
     from apn_amd import lowbit as lb
     x, w, b, _ = _rand(70, 40, 96, 3, dev)
