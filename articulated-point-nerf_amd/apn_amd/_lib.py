@@ -21,6 +21,11 @@ I32 = C.c_int32
 F32 = C.c_float
 SZ = C.c_size_t
 
+class MX4LayerArg(C.Structure):
+    """apn_mx4_layer"""
+    _fields_ = [("codes", P), ("scales", P), ("bias", P), ("N", I64), ("K", I64), ("act", I32), ("slope", F32)]
+
+
 # name -> (restype, argtypes); must match include/apn_hip.h
 SIGNATURES = {
     "apn_sample_pts_on_rays_workspace_bytes": (SZ, [I64]),
@@ -105,6 +110,8 @@ SIGNATURES = {
     "apn_mx4_dequantize": (C.c_int, [P, P, I64, I64, P, I32, I64, P]),
     "apn_mx4_linear": (C.c_int, [P, P, P, P, P, I64, I64, I64, I32, F32, P, I32, I64, P]),
     "apn_mx4_linear_few": (C.c_int, [P, I32, I64, P, P, P, I64, I64, I64, I32, F32, P, I32, I64, P]),
+    "apn_mx4_network_lds_bytes": (SZ, [I32, P]),
+    "apn_mx4_network": (C.c_int, [P, I32, I64, I64, I32, P, P, I32, I64, P]),
     "apn_gemm_f32_splitk": (C.c_int, [P, P, P, P, P, I64, I64, I64, I64, I64, I32, I32, F32, I32, P, P]),
 }
 

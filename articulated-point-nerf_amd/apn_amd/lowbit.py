@@ -409,7 +409,9 @@ class MX4Layer:
         _device("MX4Layer", weight.codes, bias)
         self.weight, self.slope = weight, slope
         self.bias = _bias(bias, weight.shape[0], "MX4Layer")
-        _act(slope, "MX4Layer")
+        act, sl = _act(slope, "MX4Layer")
+        self._arg = L.MX4LayerArg(weight.codes.data_ptr(), weight.scales.data_ptr(), _addr(self.bias), *weight.shape,
+                                  act, sl)
 
 
 def mx4_layers(layers, col_pos=None, width=None):
@@ -428,11 +430,29 @@ def mx4_layers(layers, col_pos=None, width=None):
 
 
 def mx4_sequential(layers, x: torch.Tensor, out_dtype=torch.float32) -> torch.Tensor:
-    """A stack of MX4Layers on x [..., K]; the rows between the layers are 4-bit. Returns [M, N]."""
+    """A stack of MX4Layers on x [..., K] (float32, bfloat16, float16); the rows between the layers are
+    4-bit. Returns [M, N] of ``out_dtype``. Stacks whose weights fit one CU's LDS (depth <= 8, widths
+    <= 256: feat_net) run in one launch, others layer by layer."""
+    what = "mx4_sequential"
     layers = list(layers)
     if not layers:
-        raise ValueError("mx4_sequential: no layers")
-    h = x
-    for layer in layers[:-1]:
-        h = mx4_linear(h, layer.weight, layer.bias, layer.slope)
+        raise ValueError(f"{what}: no layers")
+    if any(not isinstance(y, MX4Layer) for y in layers):
+        raise TypeError(f"{what}: MX4Layer expected")
+    for a, b in zip(layers, layers[1:]):
+        if b.weight.cols != a.weight.shape[0]:
+            raise ValueError(f"{what}: a layer of width {b.weight.cols} behind {a.weight.shape[0]} outputs")
+    t, xt = _type(out_dtype, what), _type(x.dtype, what)
+    rows, M, K, ldx = _rows(x, what)
+    if K != layers[0].weight.cols:
+        raise ValueError(f"{what}: input width {K} vs weight {layers[0].weight.shape}")
+    dev = _device(what, rows, *(y.weight.codes for y in layers))
+    args = (L.MX4LayerArg * len(layers))(*(y._arg for y in layers))
+    if len(layers) > 1 and L.load().apn_mx4_network_lds_bytes(len(layers), args):
+        out = torch.empty((M, layers[-1].weight.shape[0]), dtype=out_dtype, device=rows.device)
+        _launch(dev, "apn_mx4_network", rows.data_ptr(), xt, ldx, M, len(layers), args, out.data_ptr(), t, out.shape[1])
+        return out
+    h = rows
+    for y in layers[:-1]:
+        h = mx4_linear(h, y.weight, y.bias, y.slope)
     return mx4_linear(h, layers[-1].weight, layers[-1].bias, layers[-1].slope, out_dtype=out_dtype)

@@ -87,8 +87,8 @@ struct Args {
   const float* bias;
   void* out;
   int64_t M, ld_out;
-  int N, nb, ss, act;   // nb: blocks of K; ss: bytes per scale row
-  float slope;
+  int N, nb, ss, relu;   // nb: blocks of K; ss: bytes per scale row
+  float below;           // factor of results that are not positive
 };
 
 template <int I>   // the scales are byte I of sa and sb
@@ -110,6 +110,11 @@ __device__ __forceinline__ void tile_of(const Args& p, int64_t& m0, int& n0) {
   m0 = (group * 8 + in_group % gm) * RM;
   n0 = (int)(in_group / gm) * RN;
 }
+// without a branch per value: p.below is 1 without an activation, the slope with one
+__device__ __forceinline__ float activate(const Args& p, float v) {
+  const float b = p.relu ? (v != v ? v : 0.f) : v * p.below;
+  return v > 0.f ? v : b;
+}
 __device__ __forceinline__ f32x4 bias4(const Args& p, int n) {
   f32x4 b = {0.f, 0.f, 0.f, 0.f};
   if (p.bias) {
@@ -120,10 +125,7 @@ __device__ __forceinline__ f32x4 bias4(const Args& p, int n) {
 }
 __device__ __forceinline__ void finish4(const Args& p, const f32x4& v, const f32x4& bias, float (&y)[4]) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    y[r] = v[r] + bias[r];
-    if (p.act) y[r] = leaky(y[r], p.slope);
-  }
+  for (int r = 0; r < 4; ++r) y[r] = activate(p, v[r] + bias[r]);
 }
 // The results of TN column tiles of one row tile, four tiles at a time: 16-bit types are transposed
 // over the four lanes of a row, so that lane q stores the 32 B of tile q and a row's 128 B go out
@@ -375,38 +377,37 @@ __global__ __launch_bounds__(256, 1) void k_tile256(Args p) {
   int64_t m0;
   int n0;
   tile_of<R, R>(p, m0, n0);
+  m0 = min(m0, p.M - R), n0 = min(n0, p.N - R);   // (M, N >= R) the last tiles reach back: same values twice
   const int steps = (p.nb + 3) / 4, last = steps - 1, blocks = p.nb - 4 * last;
   // a wave loads row tiles 8 wave .. 8 wave + 7 of the 32 (X's 16, then B's 16) of a step
   const int r = lane >> 2, c = (lane & 3) ^ (r >> 2);
   const uint32_t row_bytes = (uint32_t)p.nb * 16, back = c < blocks ? 0u : 16u * c;
   const bool xs_side = wave < 2;
-  const uint8_t* const base = xs_side ? p.ac + m0 * row_bytes : p.bc + (int64_t)n0 * row_bytes;
-  const int rows = xs_side ? (int)min((int64_t)R, p.M - m0) : min(R, p.N - n0);   // that exist
-  uint32_t src[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) src[i] = (uint32_t)min((wave & 1) * 128 + 16 * i + r, rows - 1) * row_bytes + 16u * c;
+  const int64_t row0 = (xs_side ? m0 : n0) + (wave & 1) * 128;   // the wave's first row
+  const uint8_t* const base = (xs_side ? p.ac : p.bc) + row0 * row_bytes;
+  const uint32_t src = (uint32_t)r * row_bytes + 16u * c;
   const uint32_t lds0 = lds_at(lds);
   auto load = [&](int s, int i) __attribute__((always_inline)) {   // (behind the last step: it again)
     const int at = min(s, last);
-    to_lds<16>(base + (int64_t)at * 64, src[i] - (at == last ? back : 0u), lds0 + (s & 3) * STAGE + (wave * 8 + i) * 1024);
+    to_lds<16>(base + (int64_t)at * 64 + (int64_t)i * 16 * row_bytes, src - (at == last ? back : 0u),
+               lds0 + (s & 3) * STAGE + (wave * 8 + i) * 1024);
   };
   // scales of steps s .. s + 3: 16 B of a row, 64 rows an instruction, where rows of scales are whole
   // 16-B pieces (K a multiple of 512), else the four words one by one (word j of all rows together)
-  const uint8_t* const sbase = xs_side ? p.as + m0 * p.ss : p.bs + (int64_t)n0 * p.ss;
+  const uint8_t* const sbase = (xs_side ? p.as : p.bs) + row0 * p.ss;
   const bool wide = p.ss % 16 == 0 && ((uintptr_t)p.as | (uintptr_t)p.bs) % 16 == 0;
-  uint32_t ssrc[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) ssrc[i] = (uint32_t)min((wave & 1) * 128 + 64 * i + lane, rows - 1) * (uint32_t)p.ss;
   auto load_scales = [&](int s) __attribute__((always_inline)) {
     const uint32_t to = lds0 + 4 * STAGE + ((s >> 2) & 1) * SCALES;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+      const uint8_t* const b = sbase + (int64_t)i * 64 * p.ss;
       if (wide) {
-        to_lds<16>(sbase + min(4 * s, p.ss - 16), ssrc[i], to + (wave * 2 + i) * 1024);
+        to_lds<16>(b + min(4 * s, p.ss - 16), (uint32_t)lane * (uint32_t)p.ss, to + (wave * 2 + i) * 1024);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          to_lds<4>(sbase + min(4 * (s + j), p.ss - 4), ssrc[i], to + j * 2048 + (wave * 2 + i) * 256);
+          to_lds<4>(b + min(4 * (s + j), p.ss - 4), (uint32_t)lane * (uint32_t)p.ss,
+                    to + j * 2048 + (wave * 2 + i) * 256);
       }
     }
   };
@@ -423,29 +424,31 @@ __global__ __launch_bounds__(256, 1) void k_tile256(Args p) {
     x[i] = *(const u32x4*)(b + (wm * 8 + i) * 1024);
     w[i] = *(const u32x4*)(b + (16 + wn * 8 + i) * 1024);
   };
-  // byte q of the four steps' words of a row; zero behind the last block, whatever the padding holds
+  // a row's scales of four steps: byte q of the four words
   const uint32_t pick = 0x0c0c0400u + 0x0101u * q;
-  auto scale_of = [&](const uint8_t* at, int row, int s) __attribute__((always_inline)) {
+  auto raw_scale = [&](int s, int row) __attribute__((always_inline)) {
+    const uint8_t* b = lds + 4 * STAGE + ((s >> 2) & 1) * SCALES;
     u32x4 v;
     if (wide) {
-      v = *(const u32x4*)(at + 16 * row);
+      v = *(const u32x4*)(b + 16 * row);
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = *(const uint32_t*)(at + j * 2048 + 4 * row);
+      for (int j = 0; j < 4; ++j) v[j] = *(const uint32_t*)(b + j * 2048 + 4 * row);
     }
-    uint32_t a = __builtin_amdgcn_perm(v[1], v[0], pick) | __builtin_amdgcn_perm(v[3], v[2], pick) << 16;
+    return v;
+  };
+  auto scale_of = [&](const u32x4& v) __attribute__((always_inline)) {
+    return (int)(__builtin_amdgcn_perm(v[1], v[0], pick) | __builtin_amdgcn_perm(v[3], v[2], pick) << 16);
+  };
+  // zero behind the last block, whatever the padding holds
+  auto trim_scales = [&](int s) __attribute__((always_inline)) {
     if (4 * s + 16 > p.nb) {
       const int n = (p.nb - 4 * s - q + 3) / 4;   // steps whose block q exists
-      a = n >= 4 ? a : n <= 0 ? 0u : a & ((1u << (8 * n)) - 1u);
+      const uint32_t keep = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+      asm volatile("");
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sm[i] &= keep, sn[i] &= keep;
     }
-    return (int)a;
-  };
-  auto fetch_scales = [&](int s) __attribute__((always_inline)) {
-    const uint8_t* b = lds + 4 * STAGE + ((s >> 2) & 1) * SCALES;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sm[i] = scale_of(b, (wm * 8 + i) * 16 + l, s);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sn[i] = scale_of(b, 256 + (wn * 8 + i) * 16 + l, s);
   };
   load_scales(0);
 #pragma unroll
@@ -454,8 +457,12 @@ __global__ __launch_bounds__(256, 1) void k_tile256(Args p) {
     for (int i = 0; i < 8; ++i) load(s, i);
   arrive<16>();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) fetch(0, i, xf[0], wf[0]);
-  fetch_scales(0);
+  for (int i = 0; i < 8; ++i) {
+    fetch(0, i, xf[0], wf[0]);
+    sm[i] = scale_of(raw_scale(0, (wm * 8 + i) * 16 + l));
+    sn[i] = scale_of(raw_scale(0, 256 + (wn * 8 + i) * 16 + l));
+  }
+  trim_scales(0);
   for (int s = 0; s < steps; s += 4) {
     auto turn = [&](auto I) __attribute__((always_inline)) {
       constexpr int i = decltype(I)::value;
@@ -472,15 +479,26 @@ __global__ __launch_bounds__(256, 1) void k_tile256(Args p) {
         for (int m = 0; m < 8; ++m)
           if (q >= blocks) xf[i & 1][m] = u32x4{0u, 0u, 0u, 0u};
       }
+      u32x4 a, b;
+      int next[8];
 #pragma unroll
       for (int m = 0; m < 8; ++m) {
         fetch(s + i + 1, m, xf[(i & 1) ^ 1], wf[(i & 1) ^ 1]);
+        if (i == 3) {   // the next group's scales
+          a = raw_scale(s + 4, (wm * 8 + m) * 16 + l);
+          b = raw_scale(s + 4, 256 + (wn * 8 + m) * 16 + l);
+        }
 #pragma unroll
         for (int n = 0; n < 8; ++n) acc[m][n] = mma<i>(wf[i & 1][n], sn[n], xf[i & 1][m], sm[m], acc[m][n]);
         load(s + i + 3, m);
+        if (i == 3) sm[m] = scale_of(a), next[m] = scale_of(b);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (i == 3) fetch_scales(s + 4);
+      if (i == 3) {
+#pragma unroll
+        for (int m = 0; m < 8; ++m) sn[m] = next[m];
+        trim_scales(s + 4);
+      }
     };
     turn(std::integral_constant<int, 0>());
     turn(std::integral_constant<int, 1>());
@@ -582,6 +600,195 @@ __global__ __launch_bounds__(512) void k_few(FewArgs f) {
   }
 }
 
+// A stack of layers on 16 rows a wave, everything between the input rows and the output in registers.
+// All layers' weights (fragment order), scales and biases lie in LDS. A layer's results -- lane
+// (row, q) holds columns 4 q .. 4 q + 3 of every 16 -- are quantized where they are: a 32-column block
+// is 8 values of each of a row's four lanes, its codes 32 bits a lane, and four blocks transposed over
+// the four lanes are the next product's operand: lane q the 16 B of block 4 s + q. The input's floats
+// come in the same arrangement (four lanes on 64 B of a row), the next tile's while this one is
+// computed. Bound by the input and output rows.
+struct NetLayer {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  const float* bias;
+  int N, nb, ss, relu;
+  float below;
+  int at;   // byte offset of its LDS part: codes [column tile][step][lane] 16 B, scales [tile][lane], biases
+};
+constexpr int NET_DEPTH = 8, NET_COLS = 256;
+struct NetArgs {
+  NetLayer layer[NET_DEPTH];
+  const void* x;
+  void* out;
+  int64_t M, ldx, ld_out;
+  int depth, K, bytes;
+};
+// LDS bytes of a layer: column tiles of 16, padded to whole blocks of 32 columns
+inline int net_bytes(int N, int nb) {
+  const int tiles = (N + 31) / 32 * 2;
+  return tiles * (((nb + 3) / 4) * 1024 + 256 + 64);
+}
+
+// one block's 8 values of a lane (columns 4 q .. and 16 + 4 q ..): 4 + 4 nibbles, and the scale byte
+__device__ __forceinline__ uint32_t quant_block(const float (&v)[8], int& byte) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a = max(a, abs_bits(v[j]));
+  byte = mx4_byte(row_max(a));
+  return quant8(v, byte);
+}
+// four blocks' nibbles as the operand of a step: lane q's block, its columns in order
+__device__ __forceinline__ u32x4 to_operand(uint32_t (&r)[4]) {
+  transpose4(r);   // r[p]: columns 4 p .. (lower half) and 16 + 4 p .. (upper half) of the lane's block
+  return u32x4{__builtin_amdgcn_perm(r[1], r[0], 0x05040100u), __builtin_amdgcn_perm(r[3], r[2], 0x05040100u),
+               __builtin_amdgcn_perm(r[1], r[0], 0x07060302u), __builtin_amdgcn_perm(r[3], r[2], 0x07060302u)};
+}
+
+// KB: blocks of the input's columns at most; NT: column tiles of any layer at most; SW waves
+template <int TX, int T, int KB, int NT, int SW>
+__global__ __launch_bounds__(64 * SW, SW / 4) void k_network(NetArgs f) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t net_lds[];
+  constexpr int STEPS = (KB > NT / 2 ? KB + 3 : NT / 2 + 3) / 4;
+  typedef typename Elem<TX>::type E;
+  typedef E quad __attribute__((ext_vector_type(4), aligned(sizeof(E))));
+  const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t tiles = (f.M + 15) / 16, stride = (int64_t)gridDim.x * SW;
+  quad x[KB][2];
+  const int last = (f.K - 1) / 32, whole = f.K % 32 == 0;
+  // (the tile's first row in scalar registers, the lane's row and quad as 32-bit offsets)
+  uint32_t row = 0, quad_at = 4 * q;
+  auto load = [&](int64_t tile, int b) __attribute__((always_inline)) {
+    const E* in = (const E*)f.x + tile * 16 * f.ldx;
+    if (b == 0) row = (uint32_t)min((int64_t)l, f.M - 1 - tile * 16) * (uint32_t)f.ldx;
+    if (b < last || whole) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        x[b][i] = *(const quad*)((const char*)(in + 32 * b + 16 * i) + (row + quad_at) * (uint32_t)sizeof(E));
+    } else {   // the last, short block: element by element, the row's last one behind its end
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t c = min(32 * b + 16 * i + quad_at + j, (uint32_t)f.K - 1);
+          x[b][i][j] = *(const E*)((const char*)in + (row + c) * (uint32_t)sizeof(E));
+        }
+    }
+  };
+  int64_t tile = blockIdx.x + (int64_t)wave * gridDim.x;
+  if (tile < tiles) {
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+      if (b <= last) load(tile, b);
+  }
+  for (int d = 0; d < f.depth; ++d) {
+    const NetLayer& y = f.layer[d];
+    const int nt = (y.N + 31) / 32 * 2, steps = (y.nb + 3) / 4;
+    u32x4* codes = (u32x4*)(net_lds + y.at);
+    uint32_t* scales = (uint32_t*)(codes + nt * steps * 64);
+    float* bias = (float*)(scales + nt * 64);
+    for (int i = tid; i < nt * steps * 64; i += 64 * SW) {
+      const int ln = i & 63, s = (i >> 6) % steps, n = (i >> 6) / steps * 16 + (ln & 15), b = 4 * s + (ln >> 4);
+      const u32x4 w = *(const u32x4*)(y.codes + ((int64_t)min(n, y.N - 1) * y.nb + min(b, y.nb - 1)) * 16);
+      codes[i] = n < y.N && b < y.nb ? w : u32x4{0u, 0u, 0u, 0u};
+    }
+    for (int i = tid; i < nt * 64; i += 64 * SW) {   // byte s: step s
+      const int n = (i >> 6) * 16 + (i & 15), k = (i & 63) >> 4;
+      uint32_t w = 0;
+      for (int s = 0; s < steps; ++s)
+        if (n < y.N && 4 * s + k < y.nb) w |= (uint32_t)y.scales[(int64_t)n * y.ss + 4 * s + k] << (8 * s);
+      scales[i] = w;
+    }
+    for (int i = tid; i < nt * 16; i += 64 * SW) bias[i] = y.bias && i < y.N ? y.bias[i] : 0.f;
+  }
+  __syncthreads();
+  for (; tile < tiles; tile += stride) {
+    asm volatile("" : "+v"(quad_at));   // or every block's lane offsets are kept (and spilled)
+    u32x4 op[STEPS];     // the product's row operand
+    uint32_t os = 0;     // its scale bytes by step
+    const bool more = tile + stride < tiles;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) op[s] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int s = 0; s < (KB + 3) / 4; ++s) {   // the input
+      uint32_t r[4] = {0u, 0u, 0u, 0u}, sb = 0;
+#pragma unroll
+      for (int k = 0; k < 4 && 4 * s + k < KB; ++k) {
+        const int b = 4 * s + k;
+        if (b <= last) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = (float)x[b][j >> 2][j & 3];
+          if (b == last && !whole) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = 32 * b + 16 * (j >> 2) + 4 * q + (j & 3) < f.K ? v[j] : 0.f;
+          }
+          int byte;
+          r[k] = quant_block(v, byte);
+          sb |= (uint32_t)byte << (8 * k);
+          if (more) load(tile + stride, b);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      op[s] = to_operand(r);
+      os |= ((sb >> (8 * q)) & 0xffu) << (8 * s);
+    }
+    for (int d = 0; d < f.depth; ++d) {
+      const NetLayer& y = f.layer[d];
+      const int nt = (y.N + 31) / 32 * 2, steps = (y.nb + 3) / 4;
+      const u32x4* codes = (const u32x4*)(net_lds + y.at) + lane;
+      const int* scales = (const int*)(net_lds + y.at + nt * steps * 1024) + lane;
+      const float* bias = (const float*)(net_lds + y.at + nt * (steps * 1024 + 256)) + 4 * q;
+      f32x4 acc[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        if (t < nt) {
+          const int ws = scales[64 * t];
+          f32x4 a = *(const f32x4*)(bias + 16 * t);
+          a = mma<0>(codes[t * steps * 64], ws, op[0], (int)os, a);
+          if (STEPS > 1 && steps > 1) a = mma<1>(codes[(t * steps + 1) * 64], ws, op[STEPS > 1 ? 1 : 0], (int)os, a);
+          acc[t] = a;
+        }
+      const bool end = d + 1 == f.depth;
+      typedef typename Elem<T>::type O;
+      O* const out = (O*)f.out + tile * 16 * f.ld_out;
+      const uint32_t out_at = (uint32_t)l * (uint32_t)f.ld_out + quad_at;
+      const bool live = l < f.M - tile * 16;
+      os = 0;
+#pragma unroll
+      for (int s = 0; s < NT / 8; ++s) {
+        uint32_t r[4] = {0u, 0u, 0u, 0u}, sb = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int t = 8 * s + 2 * k;
+          if (t < nt) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float z = acc[t + (j >> 2)][j & 3], b = y.relu ? (z != z ? z : 0.f) : z * y.below;
+              v[j] = z > 0.f ? z : b;
+            }
+            if (end) {
+              O* o = (O*)((char*)(out + 16 * t) + out_at * (uint32_t)sizeof(O));
+              if (live) {
+                store4<T>(o, y.N - 16 * t - 4 * q, v);
+                store4<T>(o + 16, y.N - 16 * t - 16 - 4 * q, v + 4);
+              }
+            } else {
+              int byte;
+              r[k] = quant_block(v, byte);   // (columns behind N are zeros: zero weights and bias)
+              sb |= (uint32_t)byte << (8 * k);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        op[s] = to_operand(r);
+        os |= ((sb >> (8 * q)) & 0xffu) << (8 * s);
+      }
+    }
+  }
+}
+
 inline int64_t row_piece(int64_t upr) { return std::max<int64_t>(1, ((int64_t)1 << 30) / upr); }
 
 template <int T>
@@ -612,7 +819,7 @@ int dequantize(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K
   return launch_status();
 }
 
-constexpr int64_t MAX_COLS = (int64_t)1 << 20;
+constexpr int64_t MAX_COLS = (int64_t)1 << 20, MAX_LD = (int64_t)1 << 24;
 
 template <int WM, int WN, int TM, int TN, int T>
 int64_t tiles_of(const Args& a) {
@@ -630,7 +837,7 @@ void launch_linear(const Args& a, hipStream_t s) {
     hipLaunchKernelGGL((k_few<-1, T>), dim3((unsigned)ceil_div(a.N, 16)), dim3(512), 0, s, FewArgs{a, nullptr, 0, 0});
     return;
   }
-  if (a.N > 128 && tiles_of<2, 2, 8, 8, T>(a) >= 192)
+  if (a.N >= 256 && a.M >= 256 && tiles_of<2, 2, 8, 8, T>(a) >= 192)
     hipLaunchKernelGGL((k_tile256<T>), dim3((unsigned)tiles_of<2, 2, 8, 8, T>(a)), dim3(256), TILE256_LDS, s, a);
   else if (tiles_of<2, 2, 4, 4, T>(a) >= 128) launch_tile<2, 2, 4, 4, T>(a, s);
   else launch_tile<2, 2, 2, 2, T>(a, s);
@@ -642,6 +849,25 @@ void launch_few(const FewArgs& a, int32_t type, hipStream_t s) {
   if (type == APN_F32) hipLaunchKernelGGL((k_few<TX, APN_F32>), grid, dim3(512), 0, s, a);
   else if (type == APN_BF16) hipLaunchKernelGGL((k_few<TX, APN_BF16>), grid, dim3(512), 0, s, a);
   else hipLaunchKernelGGL((k_few<TX, APN_F16>), grid, dim3(512), 0, s, a);
+}
+
+template <int TX, int T, int KB, int NT, int SW>
+void launch_net_as(const NetArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((k_network<TX, T, KB, NT, SW>), dim3((unsigned)std::min<int64_t>((a.M + 15) / 16, 256)),
+                     dim3(64 * SW), a.bytes, s, a);
+}
+template <int TX, int T>
+void launch_net(const NetArgs& a, hipStream_t s) {
+  int cols = 0;
+  for (int d = 0; d < a.depth; ++d) cols = std::max(cols, a.layer[d].N);
+  if (a.K <= 192 && cols <= 128) launch_net_as<TX, T, 6, 8, 16>(a, s);
+  else launch_net_as<TX, T, 8, 16, 8>(a, s);
+}
+template <int TX>
+void launch_net_in(const NetArgs& a, int32_t type, hipStream_t s) {
+  if (type == APN_F32) launch_net<TX, APN_F32>(a, s);
+  else if (type == APN_BF16) launch_net<TX, APN_BF16>(a, s);
+  else launch_net<TX, APN_F16>(a, s);
 }
 
 }  // namespace mx4
@@ -688,7 +914,7 @@ extern "C" int apn_mx4_linear(const uint8_t* a_codes, const uint8_t* a_scales, c
   for (int64_t m = 0; m < M; m += piece) {
     char* o = (char*)out + m * ld_out * (type == APN_F32 ? 4 : 2);
     mx4::Args a{a_codes + m * row, a_scales + m * ss, b_codes, b_scales, bias, o, std::min(piece, M - m), ld_out, (int)N,
-                (int)blocks_of(K), (int)ss, act, slope};
+                (int)blocks_of(K), (int)ss, act && slope == 0.f, act ? slope : 1.f};
     if (type == APN_F32) mx4::launch_linear<APN_F32>(a, s);
     else if (type == APN_BF16) mx4::launch_linear<APN_BF16>(a, s);
     else mx4::launch_linear<APN_F16>(a, s);
@@ -705,10 +931,45 @@ extern "C" int apn_mx4_linear_few(const void* x, int32_t x_type, int64_t ldx, co
   if (M == 0) return APN_OK;
   if (!x || !b_codes || !b_scales || !out || (uintptr_t)b_codes % 16 || (uintptr_t)b_scales % 4) return APN_ERR_ARG;
   const mx4::FewArgs a{{nullptr, nullptr, b_codes, b_scales, bias, out, M, ld_out, (int)N, (int)blocks_of(K),
-                        (int)scale_stride(K), act, slope}, x, ldx, (int)K};
+                        (int)scale_stride(K), act && slope == 0.f, act ? slope : 1.f}, x, ldx, (int)K};
   hipStream_t s = (hipStream_t)stream;
   if (x_type == APN_F32) mx4::launch_few<APN_F32>(a, type, s);
   else if (x_type == APN_BF16) mx4::launch_few<APN_BF16>(a, type, s);
   else mx4::launch_few<APN_F16>(a, type, s);
+  return launch_status();
+}
+
+extern "C" size_t apn_mx4_network_lds_bytes(int32_t depth, const apn_mx4_layer* layers) {
+  if (depth < 1 || depth > mx4::NET_DEPTH || !layers) return 0;
+  size_t bytes = 0;
+  for (int d = 0; d < depth; ++d) {
+    const apn_mx4_layer& y = layers[d];
+    if (y.N < 1 || y.K < 1 || y.N > mx4::NET_COLS || y.K > mx4::NET_COLS || (d && y.K != layers[d - 1].N)) return 0;
+    bytes += (size_t)mx4::net_bytes((int)y.N, (int)blocks_of(y.K));
+  }
+  return bytes <= 160 * 1024 ? bytes : 0;
+}
+
+extern "C" int apn_mx4_network(const void* x, int32_t x_type, int64_t ldx, int64_t M, int32_t depth,
+                               const apn_mx4_layer* layers, void* out, int32_t type, int64_t ld_out, void* stream) {
+  const size_t bytes = apn_mx4_network_lds_bytes(depth, layers);
+  if (M < 0 || bytes == 0 || !ok_type(x_type) || !ok_type(type) || ldx < layers[0].K || ld_out < layers[depth - 1].N ||
+      ldx >= mx4::MAX_LD || ld_out >= mx4::MAX_LD)
+    return APN_ERR_ARG;
+  if (M == 0) return APN_OK;
+  if (!x || !out) return APN_ERR_ARG;
+  mx4::NetArgs a{};
+  a.x = x, a.out = out, a.M = M, a.ldx = ldx, a.ld_out = ld_out, a.depth = depth, a.K = (int)layers[0].K;
+  for (int d = 0; d < depth; ++d) {
+    const apn_mx4_layer& y = layers[d];
+    if (!y.codes || !y.scales || (uintptr_t)y.codes % 16) return APN_ERR_ARG;
+    a.layer[d] = {y.codes, y.scales, y.bias, (int)y.N, (int)blocks_of(y.K), (int)scale_stride(y.K),
+                  y.act && y.slope == 0.f, y.act ? y.slope : 1.f, a.bytes};
+    a.bytes += mx4::net_bytes((int)y.N, (int)blocks_of(y.K));
+  }
+  hipStream_t s = (hipStream_t)stream;
+  if (x_type == APN_F32) mx4::launch_net_in<APN_F32>(a, type, s);
+  else if (x_type == APN_BF16) mx4::launch_net_in<APN_BF16>(a, type, s);
+  else mx4::launch_net_in<APN_F16>(a, type, s);
   return launch_status();
 }

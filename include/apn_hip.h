@@ -531,6 +531,21 @@ int apn_mx4_linear(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_
 int apn_mx4_linear_few(const void* x, int32_t x_type, int64_t ldx, const uint8_t* b_codes, const uint8_t* b_scales,
                        const float* bias, int64_t M, int64_t N, int64_t K, int32_t act, float slope, void* out,
                        int32_t type, int64_t ld_out, void* stream);
+/* A stack of such layers on float rows x [M, K0] in one launch, the rows between them in mx4:
+ * h = x; h = act(mx4(h) b^T + bias) for each layer; out [M, N of the last]. Layers in a host array;
+ * K of each but the first = N of the one before; apn_mx4_network_lds_bytes says whether the stack
+ * fits (depth <= 8, K and N <= 256, the weights' bytes): 0 = no. ldx, ld_out < 2^24. */
+typedef struct {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  const float* bias;   /* [N] or NULL */
+  int64_t N, K;
+  int32_t act;
+  float slope;
+} apn_mx4_layer;
+size_t apn_mx4_network_lds_bytes(int32_t depth, const apn_mx4_layer* layers);
+int apn_mx4_network(const void* x, int32_t x_type, int64_t ldx, int64_t M, int32_t depth,
+                    const apn_mx4_layer* layers, void* out, int32_t type, int64_t ld_out, void* stream);
 
 /* Utilities */
 size_t apn_scan_workspace_bytes(int64_t n);

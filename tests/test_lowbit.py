@@ -606,12 +606,51 @@ def test_mx4_sequential_vs_float64(dev, M, sizes):
     assert float((y - h).norm() / h.norm()) < 1e-3
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,sizes,slope", [(1, [1, 1], 0.0), (17, [31, 33, 5], 0.01), (5000, [192, 128, 128], 0.0),
+                                           (333, [256, 256, 256, 256, 256], 0.01), (100, [129, 130, 1, 7], -0.5),
+                                           (40, [8] * 9, None), (65, [191, 64, 255, 30], None)])
+def test_mx4_stack_in_one_launch(dev, M, sizes, slope, dtype, out_dtype):
+    """A stack that fits one launch (several layers, widths up to 256) equals the same layers one by one
+    up to flips of inner codes (see above), for every type, padded rows and short blocks; a row that is
+    not finite stays its own."""
+    from apn_amd import lowbit as lb
+    g = torch.Generator(device=dev).manual_seed(sum(sizes) + M)
+    packed = [lb.MX4Layer(lb.mx4_quantize(torch.randn(n, k, device=dev, generator=g) / k ** 0.5),
+                          torch.randn(n, device=dev, generator=g) if i != 1 else None, slope)
+              for i, (k, n) in enumerate(zip(sizes[:-1], sizes[1:]))]
+    x = torch.randn(M, sizes[0] + 3, device=dev, generator=g).to(dtype)[:, 1:sizes[0] + 1]
+    y = lb.mx4_sequential(packed, x, out_dtype)
+    h = x
+    for p in packed[:-1]:
+        h = lb.mx4_linear(h, p.weight, p.bias, p.slope)
+    h = lb.mx4_linear(h, packed[-1].weight, packed[-1].bias, packed[-1].slope)
+    # one flip in a few rows is a larger share of a small output: 1e-3 of many rows, 0.1 of few
+    half = 0.0 if out_dtype == torch.float32 else torch.finfo(out_dtype).eps / 2
+    assert y.dtype == out_dtype
+    bound = (1e-3 if M * sizes[-1] > 1000 else 0.1) + half
+    assert float((y.double() - h.double()).norm()) <= bound * float(h.double().norm())
+    assert torch.equal(y, lb.mx4_sequential(packed, x.clone(), out_dtype))
+    if M > 20:
+        x = x.clone()
+        x[3, 0], x[19, -1] = math.inf, math.nan
+        bad = torch.zeros(M, dtype=torch.bool, device=dev)
+        bad[[3, 19]] = True
+        z = lb.mx4_sequential(packed, x, out_dtype)
+        assert torch.isnan(z[bad]).all() and torch.equal(z[~bad], y[~bad])
+    assert lb.mx4_sequential(packed, x[:0], out_dtype).shape == (0, sizes[-1])
+
+
 # --- streams, graphs, the model ------------------------------------------------------------------------
 
 def _functional_step(lb, x, w, b, dy, packed):
     y, k = lb.linear_q8(x, w, b, 0.01)
     grads = lb.linear_q8_backward(dy, w, lb.q8_pack(x), k, 0.01)
-    return (y, *grads, lb.mx4_linear(x, packed, b, 0.01), lb.mx4_sequential([lb.MX4Layer(packed, b, 0.0)], x))
+    square = lb.mx4_quantize(w[:, :1].expand(-1, w.shape[0]).contiguous())
+    return (y, *grads, lb.mx4_linear(x, packed, b, 0.01), lb.mx4_linear(x[:3], packed, b, 0.01),
+            lb.mx4_sequential([lb.MX4Layer(packed, b, 0.0), lb.MX4Layer(square, b)], x))
 
 
 @gpu
@@ -803,6 +842,18 @@ def test_c_entries_refuse_without_gpu():
     assert lib.apn_mx4_linear(p, p, p, p, None, 4, 0, 32, 0, 0.0, p, 0, 32, None) == 1
     assert lib.apn_mx4_linear(p, p, p + 1, p, None, 4, 8, 32, 0, 0.0, p, 0, 32, None) == 1
     assert lib.apn_mx4_linear(p, p, p, p, None, 4, 8, 32, 0, 0.0, p, 4, 32, None) == 1
+    assert lib.apn_mx4_linear(p, p + 2, p, p, None, 4, 8, 32, 0, 0.0, p, 0, 32, None) == 1
+    assert lib.apn_mx4_linear_few(p, 0, 32, p, p, None, 17, 8, 32, 0, 0.0, p, 0, 8, None) == 1
+    assert lib.apn_mx4_linear_few(p, 0, 31, p, p, None, 4, 8, 32, 0, 0.0, p, 0, 8, None) == 1
+    arg = _lib.MX4LayerArg
+    two = (arg * 2)(arg(p, p, None, 64, 32, 0, 0.0), arg(p, p, None, 64, 64, 1, 0.5))
+    assert lib.apn_mx4_network_lds_bytes(2, two) > 2 * 64 * 16
+    assert lib.apn_mx4_network(p, 0, 31, 4, 2, two, p, 0, 64, None) == 1
+    assert lib.apn_mx4_network(p, 0, 32, 4, 9, two, p, 0, 64, None) == 1
+    two[1].K = 32
+    assert lib.apn_mx4_network_lds_bytes(2, two) == 0 and lib.apn_mx4_network(p, 0, 32, 4, 2, two, p, 0, 64, None) == 1
+    wide = (arg * 1)(arg(p, p, None, 257, 32, 0, 0.0))
+    assert lib.apn_mx4_network_lds_bytes(1, wide) == 0 and lib.apn_mx4_network_lds_bytes(0, None) == 0
 
 
 @gpu
@@ -845,3 +896,12 @@ def test_refusals_gpu(dev):
         lb.mx4_linear(x, lb.mx4_quantize(w), out_dtype=torch.float64)
     with pytest.raises(TypeError, match="MX4Rows"):
         lb.mx4_linear(x, xk)
+    layer = lb.MX4Layer(lb.mx4_quantize(w))
+    with pytest.raises(ValueError, match="behind 5 outputs"):
+        lb.mx4_sequential([layer, layer], x)
+    with pytest.raises(ValueError, match="input width"):
+        lb.mx4_sequential([layer], x[:, :32])
+    with pytest.raises(TypeError, match="MX4Layer"):
+        lb.mx4_sequential([w], x)
+    with pytest.raises(TypeError, match="float"):
+        lb.mx4_sequential([layer], x.double())
