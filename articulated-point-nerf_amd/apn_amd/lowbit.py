@@ -147,35 +147,53 @@ class _BlockRows:
         if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() % 16 or scales.data_ptr() % 4:
             raise ValueError(f"{what}: contiguous codes (16-byte aligned) and scales (4-byte aligned)")
         _device(what, codes, scales)
-        self.codes, self.scales, self.cols = codes, scales, cols
+        self._buf, self._codes, self._scales = None, codes, scales
+        self.rows, self.cols, self.device = codes.shape[0], cols, codes.device
+        self._at = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
     def _empty(cls, rows, cols, device):
-        """Rows for a kernel to fill (their layout needs no check)."""
+        """Rows for a kernel to fill: one allocation, their layout needs no check."""
         self = cls.__new__(cls)
-        self.codes = torch.empty((rows, cls._BYTES * _blocks(cols)), dtype=torch.uint8, device=device)
-        self.scales = torch.empty((rows, _scale_bytes(cols)), dtype=torch.uint8, device=device)
-        self.cols = cols
+        n = rows * cls._BYTES * _blocks(cols)
+        self._buf = torch.empty(n + rows * _scale_bytes(cols), dtype=torch.uint8, device=device)
+        self._codes = self._scales = None
+        self.rows, self.cols, self.device = rows, cols, device
+        p = self._buf.data_ptr()
+        self._at = p, p + n
         return self
 
     @property
-    def shape(self):
-        return self.codes.shape[0], self.cols
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            w = self._BYTES * _blocks(self.cols)
+            self._codes = self._buf[:self.rows * w].view(self.rows, w)
+        return self._codes
 
     @property
-    def device(self):
-        return self.codes.device
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            w = _scale_bytes(self.cols)
+            self._scales = self._buf[self._buf.numel() - self.rows * w:].view(self.rows, w)
+        return self._scales
+
+    @property
+    def shape(self):
+        return self.rows, self.cols
 
     @property
     def nbytes(self):
-        return self.codes.numel() + self.scales.numel()
+        return self.rows * (self._BYTES * _blocks(self.cols) + _scale_bytes(self.cols))
+
+    def _index(self, what, dev):
+        """Checks that these rows are on device index ``dev``."""
+        if self.device.index != dev:
+            raise RuntimeError(f"{what}: tensors on different devices: {self.device} and cuda:{dev}")
 
     def _read(self, entry, dtype):
         t = _type(dtype, f"{type(self).__name__}.dequantize")
-        codes, K = self.codes, self.cols
-        M = codes.shape[0]
-        out = torch.empty((M, K), dtype=dtype, device=codes.device)
-        _launch(codes.get_device(), entry, codes.data_ptr(), self.scales.data_ptr(), M, K, out.data_ptr(), t, K)
+        out = torch.empty((self.rows, self.cols), dtype=dtype, device=self.device)
+        _launch(out.get_device(), entry, *self._at, self.rows, self.cols, out.data_ptr(), t, self.cols)
         return out
 
 
@@ -204,7 +222,7 @@ def _pack(cls, entry, x, what):
     x, M, K, ld = _rows(x, what)
     dev = _device(what, x)
     out = cls._empty(M, K, x.device)
-    _launch(dev, entry, x.data_ptr(), t, M, K, ld, out.codes.data_ptr(), out.scales.data_ptr())
+    _launch(dev, entry, x.data_ptr(), t, M, K, ld, *out._at)
     return out
 
 
@@ -229,7 +247,7 @@ def linear_q8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
     y = torch.empty((M, N), dtype=torch.float32, device=x.device)
     kept = Q8Rows._empty(M, N, x.device)
     _launch(dev, "apn_q8_linear_fwd", x.data_ptr(), ldx, w.data_ptr(), ldw, _addr(b), M, N, K, act, sl, y.data_ptr(), N,
-            kept.codes.data_ptr(), kept.scales.data_ptr())
+            *kept._at)
     return y, kept
 
 
@@ -260,15 +278,18 @@ def linear_q8_backward(dy: torch.Tensor, weight: torch.Tensor, x_kept: Q8Rows | 
     _, sl = _act(slope, what)
     if slope is not None and y_kept is None:
         raise ValueError(f"{what}: an activation needs y_kept")
-    mask = y_kept.codes if slope is not None else None
-    xc, xs = (x_kept.codes, x_kept.scales) if want_w else (None, None)
-    dev = _device(what, dy, w, mask, xc)
+    dev = _device(what, dy, w)
+    for kept in (x_kept, y_kept):
+        if kept is not None:
+            kept._index(what, dev)
+    mask = y_kept._at[0] if slope is not None else None
+    xc, xs = x_kept._at if want_w else (None, None)
     empty = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dy.device)  # noqa: E731
     dx = dw = db = None
     if want_x:
         Kp = -(-K // 4) * 4   # rows of whole 16-byte pieces, as linear's: odd rows written 1.5 x as slowly
         dx = empty(M, Kp)
-        _launch(dev, "apn_q8_linear_bwd_dx", dy.data_ptr(), ld_dy, _addr(mask), sl, w.data_ptr(), ldw, M, N, K,
+        _launch(dev, "apn_q8_linear_bwd_dx", dy.data_ptr(), ld_dy, mask, sl, w.data_ptr(), ldw, M, N, K,
                 dx.data_ptr(), Kp)
         if Kp != K:
             dx = dx[:, :K]
@@ -276,7 +297,7 @@ def linear_q8_backward(dy: torch.Tensor, weight: torch.Tensor, x_kept: Q8Rows | 
         dw = empty(N, K) if want_w else None
         db = empty(N) if want_b else None
         ws = empty(max(int(L.load().apn_q8_linear_bwd_dw_workspace_bytes(M, N, K)) // 4, 1))
-        _launch(dev, "apn_q8_linear_bwd_dw", dy.data_ptr(), ld_dy, _addr(mask), sl, _addr(xc), _addr(xs), M, N, K,
+        _launch(dev, "apn_q8_linear_bwd_dw", dy.data_ptr(), ld_dy, mask, sl, xc, xs, M, N, K,
                 _addr(dw), _addr(db), ws.data_ptr())
     return dx, dw, db
 
@@ -374,29 +395,36 @@ def mx4_linear(x, weight: MX4Rows, bias: torch.Tensor | None = None, slope: floa
     if not isinstance(weight, MX4Rows):
         raise TypeError(f"{what}: weight must be MX4Rows, got {type(weight).__name__}")
     t = _type(out_dtype, what)
-    wc, K = weight.codes, weight.cols
-    width = x.cols if isinstance(x, MX4Rows) else x.shape[-1] if x.dim() else 0
+    N, K = weight.rows, weight.cols
+    own = isinstance(x, MX4Rows)
+    width = x.cols if own else x.shape[-1] if x.dim() else 0
     if width != K:
         raise ValueError(f"{what}: input width {width} vs weight {weight.shape}")
-    N = wc.shape[0]
     if N == 0:
         raise ValueError(f"{what}: weight without rows {weight.shape}")
     b = _bias(bias, N, what)
     act, sl = _act(slope, what)
-    dev = _device(what, x.codes if isinstance(x, MX4Rows) else x, wc, b)
-    if not isinstance(x, MX4Rows):
+    if not own:
         xt = _type(x.dtype, what)
         rows, M, _, ldx = _rows(x, what)
+        dev = _device(what, rows)
+        weight._index(what, dev)
+        if b is not None:
+            _device(what, rows, b)
         if M <= FEW_ROWS:   # quantized on the way
-            out = torch.empty((M, N), dtype=out_dtype, device=wc.device)
-            _launch(dev, "apn_mx4_linear_few", rows.data_ptr(), xt, ldx, wc.data_ptr(), weight.scales.data_ptr(),
-                    _addr(b), M, N, K, act, sl, out.data_ptr(), t, N)
+            out = torch.empty((M, N), dtype=out_dtype, device=weight.device)
+            _launch(dev, "apn_mx4_linear_few", rows.data_ptr(), xt, ldx, *weight._at, _addr(b), M, N, K, act, sl,
+                    out.data_ptr(), t, N)
             return out
         x = mx4_quantize(rows)
-    M = x.codes.shape[0]
-    out = torch.empty((M, N), dtype=out_dtype, device=wc.device)
-    _launch(dev, "apn_mx4_linear", x.codes.data_ptr(), x.scales.data_ptr(), wc.data_ptr(), weight.scales.data_ptr(),
-            _addr(b), M, N, K, act, sl, out.data_ptr(), t, N)
+    else:
+        dev = x.device.index
+        weight._index(what, dev)
+        if b is not None and b.get_device() != dev:
+            _device(what, x.codes, b)
+    M = x.rows
+    out = torch.empty((M, N), dtype=out_dtype, device=weight.device)
+    _launch(dev, "apn_mx4_linear", *x._at, *weight._at, _addr(b), M, N, K, act, sl, out.data_ptr(), t, N)
     return out
 
 
@@ -406,12 +434,12 @@ class MX4Layer:
     def __init__(self, weight: MX4Rows, bias: torch.Tensor | None = None, slope: float | None = None):
         if not isinstance(weight, MX4Rows):
             raise TypeError(f"MX4Layer: weight must be MX4Rows, got {type(weight).__name__}")
-        _device("MX4Layer", weight.codes, bias)
+        if bias is not None:
+            _device("MX4Layer", weight.codes, bias)
         self.weight, self.slope = weight, slope
         self.bias = _bias(bias, weight.shape[0], "MX4Layer")
         act, sl = _act(slope, "MX4Layer")
-        self._arg = L.MX4LayerArg(weight.codes.data_ptr(), weight.scales.data_ptr(), _addr(self.bias), *weight.shape,
-                                  act, sl)
+        self._arg = L.MX4LayerArg(*weight._at, _addr(self.bias), *weight.shape, act, sl)
 
 
 def mx4_layers(layers, col_pos=None, width=None):
@@ -446,7 +474,9 @@ def mx4_sequential(layers, x: torch.Tensor, out_dtype=torch.float32) -> torch.Te
     rows, M, K, ldx = _rows(x, what)
     if K != layers[0].weight.cols:
         raise ValueError(f"{what}: input width {K} vs weight {layers[0].weight.shape}")
-    dev = _device(what, rows, *(y.weight.codes for y in layers))
+    dev = _device(what, rows)
+    for y in layers:
+        y.weight._index(what, dev)
     args = (L.MX4LayerArg * len(layers))(*(y._arg for y in layers))
     if len(layers) > 1 and L.load().apn_mx4_network_lds_bytes(len(layers), args):
         out = torch.empty((M, layers[-1].weight.shape[0]), dtype=out_dtype, device=rows.device)
