@@ -749,11 +749,15 @@ __global__ __launch_bounds__(64 * SW, SW / 4) void k_network(NetArgs f) {
           if (STEPS > 1 && steps > 1) a = mma<1>(codes[(t * steps + 1) * 64], ws, op[STEPS > 1 ? 1 : 0], (int)os, a);
           acc[t] = a;
         }
-      const bool end = d + 1 == f.depth;
-      typedef typename Elem<T>::type O;
-      O* const out = (O*)f.out + tile * 16 * f.ld_out;
-      const uint32_t out_at = (uint32_t)l * (uint32_t)f.ld_out + quad_at;
-      const bool live = l < f.M - tile * 16;
+      if (d + 1 == f.depth) {
+        f32x4 none[NT];   // (the biases are in the sums)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) none[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        Args p{};
+        p.out = f.out, p.M = f.M, p.ld_out = f.ld_out, p.N = y.N, p.relu = y.relu, p.below = y.below;
+        store_row<T, NT>(p, tile * 16 + l, 0, q, acc, none);
+        break;
+      }
       os = 0;
 #pragma unroll
       for (int s = 0; s < NT / 8; ++s) {
@@ -768,17 +772,9 @@ __global__ __launch_bounds__(64 * SW, SW / 4) void k_network(NetArgs f) {
               const float z = acc[t + (j >> 2)][j & 3], b = y.relu ? (z != z ? z : 0.f) : z * y.below;
               v[j] = z > 0.f ? z : b;
             }
-            if (end) {
-              O* o = (O*)((char*)(out + 16 * t) + out_at * (uint32_t)sizeof(O));
-              if (live) {
-                store4<T>(o, y.N - 16 * t - 4 * q, v);
-                store4<T>(o + 16, y.N - 16 * t - 16 - 4 * q, v + 4);
-              }
-            } else {
-              int byte;
-              r[k] = quant_block(v, byte);   // (columns behind N are zeros: zero weights and bias)
-              sb |= (uint32_t)byte << (8 * k);
-            }
+            int byte;
+            r[k] = quant_block(v, byte);   // (columns behind N are zeros: zero weights and bias)
+            sb |= (uint32_t)byte << (8 * k);
             __builtin_amdgcn_sched_barrier(0);
           }
         }
@@ -913,8 +909,8 @@ extern "C" int apn_mx4_linear(const uint8_t* a_codes, const uint8_t* a_scales, c
   const int64_t row = blocks_of(K) * 16, ss = scale_stride(K);
   for (int64_t m = 0; m < M; m += piece) {
     char* o = (char*)out + m * ld_out * (type == APN_F32 ? 4 : 2);
-    mx4::Args a{a_codes + m * row, a_scales + m * ss, b_codes, b_scales, bias, o, std::min(piece, M - m), ld_out, (int)N,
-                (int)blocks_of(K), (int)ss, act && slope == 0.f, act ? slope : 1.f};
+    mx4::Args a{a_codes + m * row, a_scales + m * ss, b_codes, b_scales, bias, o, std::min(piece, M - m), ld_out,
+                (int)N, (int)blocks_of(K), (int)ss, act && slope == 0.f, act ? slope : 1.f};
     if (type == APN_F32) mx4::launch_linear<APN_F32>(a, s);
     else if (type == APN_BF16) mx4::launch_linear<APN_BF16>(a, s);
     else mx4::launch_linear<APN_F16>(a, s);
