@@ -57,7 +57,8 @@ __device__ __forceinline__ uint32_t q8_codes4(const float* x, float inv) {
     t[j] = __float_as_uint(fminf(fabsf(x[j]) * inv, 127.f) + 8388608.f);
     s |= x[j] > 0.f ? 0u : 0x80u << (8 * j);
   }
-  const uint32_t lo = __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(t[3], t[2], 0x04000c0cu);
+  const uint32_t lo = __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(t[3], t[2], 0x04000c0cu);
   return lo | hi | s;
 }
 __device__ __forceinline__ float q8_value(uint32_t code, float scale) {

@@ -94,15 +94,10 @@ __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
 }
 
 // Rows kernel: out[m][c] = sum_r in[m][r] Wop[c][r], the forward (r = input column, c = output
-// column) and dX (r = output column, c = input column, Wop = W^T, `in` masked by Y's signs).
-// 64 rows x 32 NW columns per workgroup of NW waves. The matrix operands are swapped -- A = W's
-// rows, B = the data rows -- so a lane's 16 results of a 32 x 32 tile are 16 of the 32 columns of
-// ONE data row (columns 8 j + 4 h + i; the other half in lane ^ 32), which makes the q8 block
-// maximum 15 in-lane maxima and one exchange. Data rows are staged through LDS once per workgroup,
-// cut into their three planes, in fragment order: 16-B piece (plane, k step, row tile, half, row),
-// the row slot xor-ed with the 8-column unit so that the 8 lanes which write one row's units and
-// the 8 lanes which read neighbouring rows both meet all 8 bank groups.
-constexpr int BM = 64;   // rows of a workgroup's tile; the reduction is staged 64 columns at a time
+// column) and dX (r = output column, c = input column, Wop = W^T, `in` masked by Y's signs). The
+// matrix operands are swapped -- A = W's rows, B = the data rows -- so that a lane's results are
+// columns of ONE data row (of a 32 x 32 tile 16 of its 32 columns, 8 j + 4 h + i, the other half in
+// lane ^ 32; of a 16 x 16 tile 4), which makes a q8 block's maximum mostly in-lane.
 
 struct RowArgs {
   const float* in;
@@ -117,76 +112,9 @@ struct RowArgs {
   float slope;
 };
 
-template <bool WT>   // WT: W stored [r][c], else [c][r]
-__device__ __forceinline__ void load_w(const RowArgs& p, int c, int r, float (&v)[8]) {
-  const int cc = min(c, p.C - 1);
-  if (!WT && r + 8 <= p.R) {
-    load8<APN_F32>(p.w + (int64_t)cc * p.ldw + r, 8, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int rr = min(r + j, p.R - 1);
-      v[j] = p.w[WT ? (int64_t)rr * p.ldw + cc : (int64_t)cc * p.ldw + rr];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = r + j < p.R ? v[j] : 0.f;
-  }
-  if (c >= p.C) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.f;
-  }
-}
-
 // the gradient through the activation; slope 0 gives 0 whatever g holds
 __device__ __forceinline__ float masked(float g, uint32_t code, float slope) {
   return code & 0x80u ? (slope == 0.f ? 0.f : g * slope) : g;
-}
-
-// One thread's 8-column unit of a staged chunk: the loads, and later the cut into LDS. Rows and
-// columns behind the ends are read at the last one and zeroed: no lane branches around a load.
-struct Unit {
-  float v[8];
-  u32x2 s;
-};
-template <bool MASK>
-__device__ __forceinline__ void load_unit(const RowArgs& p, int64_t m, int r, bool full, Unit& u) {
-  const int64_t mm = min(m, p.M - 1);
-  const float* q = p.in + mm * p.ld_in;
-  if (full) {
-    load8<APN_F32>(q + r, 8, u.v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) u.v[j] = q[min(r + j, p.R - 1)];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) u.v[j] = m < p.M && r + j < p.R ? u.v[j] : 0.f;
-  }
-  if (MASK) u.s = *(const u32x2*)(p.mask + mm * p.ld_mask + min(r, (int)p.ld_mask - 8));
-}
-template <bool MASK>
-__device__ __forceinline__ void stage_unit(const RowArgs& p, int row, int u, Unit& x, u32x4* sh) {
-  if (MASK) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x.v[j] = masked(x.v[j], x.s[j >> 2] >> (8 * (j & 3)), p.slope);
-  }
-  u32x4 a, b, c;
-  cut3(x.v, a, b, c);
-  const int at = (u >> 1) * 128 + (row >> 5) * 64 + (u & 1) * 32 + ((row & 31) ^ u);
-  sh[at] = a, sh[512 + at] = b, sh[1024 + at] = c;
-}
-
-// six products of one 16-column step for the wave's NT row tiles from t0 on, small ones first
-template <int NT>
-__device__ __forceinline__ void step(const u32x4* sh, int ks, int t0, int l, int h, u32x4 wh, u32x4 wm, u32x4 wl,
-                                     f32x16 (&acc)[NT]) {
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int at = ks * 128 + (t0 + t) * 64 + h * 32 + (l ^ (2 * ks + h));
-    const u32x4 xh = sh[at], xm = sh[512 + at], xl = sh[1024 + at];
-    f32x16 a = acc[t];
-    a = mma(wl, xh, a), a = mma(wh, xl, a), a = mma(wm, xm, a);
-    a = mma(wm, xh, a), a = mma(wh, xm, a), a = mma(wh, xh, a);
-    acc[t] = a;
-  }
 }
 
 template <bool Q8, int NT>
@@ -495,59 +423,184 @@ __global__ __launch_bounds__(64 * SW, SW / 4) void k_rows_stream(RowArgs p) {
   }
 }
 
-// Any R: the weights are read (from the caches) and cut at each use, one step ahead.
+// Any R: 128 rows x 128 columns a workgroup of 8 waves (64 x 32 each), rows and weights in chunks of
+// 32 columns of the reduction cut once per workgroup into LDS (fragment order), the next chunk's on
+// their way to registers. A thread cuts one octet of each; rows and columns behind the ends are read
+// at the last one and zeroed, so that no lane branches around a load. One buffer, so that a CU holds
+// two workgroups and one multiplies while the other cuts: 77 us for 20000 x 400 x 400 and 250 for dX
+// of 60000 x 512 x 512; with two buffers and one workgroup a CU 85 and 290 (and 27 against 31 where
+// the workgroups are few, 1000 x 512 x 512). Bound by the matrix and vector units in turn.
 template <bool WT, bool MASK, bool Q8>
-__global__ __launch_bounds__(256, 2) void k_rows(RowArgs p) {
-  __shared__ u32x4 sh[2 * 1536];
+__global__ __launch_bounds__(512, 4) void k_rows(RowArgs p) {
+  __shared__ u32x4 rsh[2 * 1536];   // (rows, weights) x [plane][step][tile of 32][half, slot]
+  constexpr int PLANE = 512, SIDE = 3 * PLANE;
   __shared__ float bias[128];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int l = lane & 31, h = lane >> 5;
-  const int c0 = (blockIdx.y * 4 + wave) * 32;
-  if (Q8 && tid < 128) {   // read behind the first chunk's barrier
-    const int c = blockIdx.y * 128 + tid;
-    bias[tid] = p.bias && c < p.C ? p.bias[c] : 0.f;
-  }
-  const int nch = (p.R + 63) / 64, last = (p.R - 1) / 16;
-  int buf = 0;
-  for (int64_t m0 = (int64_t)blockIdx.x * BM; m0 < p.M; m0 += (int64_t)gridDim.x * BM) {
-    f32x16 acc[2];
+  const int tid = threadIdx.x, lane = tid & 63, l = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave & 1, wc = wave >> 1;
+  const int64_t m0 = (int64_t)blockIdx.x * 128;
+  const int c0 = blockIdx.y * 128;
+  if (Q8 && tid < 128) bias[tid] = p.bias && c0 + tid < p.C ? p.bias[c0 + tid] : 0.f;   // (read behind a barrier)
+  // the thread's octets: row xr, columns 8 xu .. of a chunk; weight column wcol, reduction 8 wu ..
+  const int xr = tid >> 2, xu = tid & 3, wcol = WT ? tid & 127 : tid >> 2, wu = WT ? tid >> 7 : tid & 3;
+  const int64_t xm = min(m0 + xr, p.M - 1);
+  const float* const in = p.in + xm * p.ld_in;
+  const uint8_t* const mask = MASK ? p.mask + xm * p.ld_mask : nullptr;
+  const int cw = min(c0 + wcol, p.C - 1);
+  const float* const w = WT ? p.w + cw : p.w + (int64_t)cw * p.ldw;
+  float xv[8], wv[8];
+  u32x2 xs = {0u, 0u};
+  auto load = [&](int r0) __attribute__((always_inline)) {
+    const int r = r0 + 8 * xu, s = r0 + 8 * wu;
+    if (r0 + 32 <= p.R) {
+      load8<APN_F32>(in + r, 8, xv);
+    } else {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
-    Unit x[2];
-    float wv[8];
-    auto load = [&](int ch) __attribute__((always_inline)) {
-      const bool full = m0 + BM <= p.M && 64 * ch + 64 <= p.R;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int f = tid + 256 * i;
-        load_unit<MASK>(p, m0 + (f >> 3), 64 * ch + 8 * (f & 7), full, x[i]);
+      for (int j = 0; j < 8; ++j) {   // (the weights' zeros alone would leave inf x 0)
+        const float x = in[min(r + j, p.R - 1)];
+        xv[j] = r + j < p.R ? x : 0.f;
       }
-    };
-    load(0);
-    load_w<WT>(p, c0 + l, 8 * h, wv);
-    for (int ch = 0; ch < nch; ++ch) {
-      u32x4* s = sh + buf;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int f = tid + 256 * i;
-        stage_unit<MASK>(p, f >> 3, f & 7, x[i], s);
-      }
-      __syncthreads();
-      if (ch + 1 < nch) load(ch + 1);
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        u32x4 wh, wm, wl;
-        cut3(wv, wh, wm, wl);
-        const int g = 4 * ch + ks;
-        if (g >= last + 1) break;
-        load_w<WT>(p, c0 + l, 16 * min(g + 1, last) + 8 * h, wv);
-        step<2>(s, ks, 0, l, h, wh, wm, wl, acc);
-      }
-      buf ^= 1536;
     }
-    finish_rows<Q8, 2>(p, m0, c0, l, h, acc, Q8 ? bias + 32 * wave : nullptr);
+    if (MASK) xs = *(const u32x2*)(mask + min(r, (int)p.ld_mask - 8));
+    if (!WT && r0 + 32 <= p.R) {
+      load8<APN_F32>(w + s, 8, wv);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = min(s + j, p.R - 1);
+        const float x = WT ? w[(int64_t)i * p.ldw] : w[i];
+        wv[j] = s + j < p.R ? x : 0.f;
+      }
+    }
+  };
+  auto stage = [&](u32x4* sh) __attribute__((always_inline)) {
+    // (registers of their own: left in the loads' tuple, the compiler lets the cut parts overwrite an
+    // octet's elements before their use)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(xv[j]), "+v"(wv[j]));
+    if (MASK) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) xv[j] = masked(xv[j], xs[j >> 2] >> (8 * (j & 3)), p.slope);
+    }
+    u32x4 a, b, c;
+    cut3(xv, a, b, c);
+    const int x = ((xu >> 1) * 4 + (xr >> 5)) * 64 + (xu & 1) * 32 + ((xr & 31) ^ (2 * xu));
+    sh[x] = a, sh[PLANE + x] = b, sh[2 * PLANE + x] = c;
+    cut3(wv, a, b, c);
+    const int y = SIDE + ((wu >> 1) * 4 + (wcol >> 5)) * 64 + (wu & 1) * 32 + ((wcol & 31) ^ (2 * wu));
+    sh[y] = a, sh[PLANE + y] = b, sh[2 * PLANE + y] = c;
+  };
+  f32x16 acc[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
+  load(0);
+  for (int r0 = 0; r0 < p.R; r0 += 32) {
+    stage(rsh);
+    __syncthreads();
+    load(min(r0 + 32, (p.R - 1) / 32 * 32));
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const int at = ks * 256 + h * 32 + (l ^ (2 * (2 * ks + h)));
+      const u32x4* y = rsh + SIDE + at + wc * 64;
+      const u32x4 wh = y[0], wm = y[PLANE], wl = y[2 * PLANE];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const u32x4* x = rsh + at + (wr * 2 + t) * 64;
+        const u32x4 xh = x[0], xm = x[PLANE], xl = x[2 * PLANE];
+        f32x16 a = acc[t];
+        a = mma(wl, xh, a), a = mma(wh, xl, a), a = mma(wm, xm, a);   // small products first
+        a = mma(wm, xh, a), a = mma(wh, xm, a), a = mma(wh, xh, a);
+        acc[t] = a;
+      }
+    }
+    __syncthreads();
+  }
+  finish_rows<Q8, 2>(p, m0 + 64 * wr, c0 + 32 * wc, l, h, acc, Q8 ? bias + 32 * wc : nullptr);
+}
+
+// A few rows: f32 products, bound by the latency of W. Forward: 32 columns a workgroup, 16 lanes
+// each, four rows at a time (blockIdx.y).
+__global__ __launch_bounds__(512) void k_few_fwd(RowArgs p) {
+  __shared__ float ys[4][32];
+  const int tid = threadIdx.x, c0 = blockIdx.x * 32, c = min(c0 + (tid >> 4), p.C - 1), part = tid & 15;
+  const int64_t m0 = (int64_t)blockIdx.y * 4;
+  const float* w = p.w + (int64_t)c * p.ldw;
+  const float* x[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) x[r] = p.in + min(m0 + r, p.M - 1) * p.ld_in;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int k = 4 * part; k < p.R; k += 64) {
+    if (k + 4 <= p.R) {
+      const f32x4 a = *(const Octet<float>::half*)(w + k);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 b = *(const Octet<float>::half*)(x[r] + k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[r] = fmaf(a[j], b[j], s[r]);
+      }
+    } else {
+      for (int j = k; j < p.R; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = fmaf(w[j], x[r][j], s[r]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) s[r] += __shfl_xor(s[r], d);
+    if (part == 0) ys[r][tid >> 4] = s[r];
+  }
+  __syncthreads();
+  if (tid >= 128) return;
+  const int r = tid >> 5, o = tid & 31;
+  const int64_t m = m0 + r;
+  float y = ys[r][o];
+  if (c0 + o < p.C) {
+    if (p.bias) y += p.bias[c0 + o];
+    if (p.act) y = leaky(y, p.slope);
+  } else {
+    y = 0.f;
+  }
+  uint32_t a = abs_bits(y);
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) a = max(a, (uint32_t)__shfl_xor((int)a, d));
+  const int byte = q8_byte(a);
+  if (m >= p.M) return;
+  if (c0 + o < p.C) p.out[m * p.ld_out + c0 + o] = y;
+  const float v[4] = {y, 0.f, 0.f, 0.f};
+  p.codes[m * p.ld_codes + c0 + o] = (uint8_t)q8_codes4(v, inv_pow2_of(byte));
+  uint8_t* q = p.scales + m * p.ss + (c0 >> 5);
+  if (o == 0) *q = (uint8_t)byte;
+  else if (c0 + 32 >= p.C && (c0 >> 5) + o < p.ss) q[o] = 0;
+}
+// dX: 64 columns a workgroup, the reduction over its 8 waves, four rows at a time.
+template <bool MASK>
+__global__ __launch_bounds__(512) void k_few_dx(RowArgs p) {
+  __shared__ float red[8][4][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = blockIdx.x * 64 + lane, cc = min(c, p.C - 1);
+  const int64_t m0 = (int64_t)blockIdx.y * 4;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int r = wave; r < p.R; r += 8) {
+    const float w = p.w[(int64_t)r * p.ldw + cc];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t m = min(m0 + i, p.M - 1);
+      const float g = p.in[m * p.ld_in + r];
+      s[i] = fmaf(MASK ? masked(g, p.mask[m * p.ld_mask + r], p.slope) : g, w, s[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) red[wave][i][lane] = s[i];
+  __syncthreads();
+  if (wave < 4 && c < p.C && m0 + wave < p.M) {
+    float t = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t += red[j][wave][lane];
+    p.out[(m0 + wave) * p.ld_out + c] = t;
   }
 }
 
@@ -575,7 +628,8 @@ struct DwArgs {
 __device__ __forceinline__ int slot32(int c) { return (c & 31) ^ ((c >> 3) & 3); }
 
 // 16-B pieces of a buffer: three planes of G, one of X'
-template <int KT> constexpr int DW_BUF = 3 * 1024 + 512 * KT;
+constexpr int DW_G = 3 * 1024;   // G's three planes, then X'
+template <int KT> constexpr int DW_BUF = DW_G + 512 * KT;
 
 // One thread's part of a chunk: 8 rows of 4 columns of dY and Y's codes, or of X's codes and scales
 // (v[j][0]; with KT = 3 two more columns' in the upper halves: codes t[j], scale v[j][1])
@@ -653,7 +707,7 @@ __device__ __forceinline__ void dw_stage(const DwAt& w, const DwRows& x, int c, 
     const int s = ks * 256 + col;
     sh[s] = a, sh[1024 + s] = b, sh[2048 + s] = d;
   } else {
-    u32x4* xs = sh + 3072 + ks * (128 * KT);
+    u32x4* xs = sh + DW_G + ks * (128 * KT);
     xs[col] = dw_values(x.s, x.v, c, 0);
     if (KT == 3 && c < 2) xs[256 + (w.cq >> 4) * 64 + row + slot32(2 * w.cq + c)] = dw_values(x.t, x.v, c, 1);
   }
@@ -689,7 +743,7 @@ __device__ __forceinline__ void dw_side(const DwArgs& p, const DwAt& w, u32x4* s
   auto multiply = [&](const u32x4* b, int ks) __attribute__((always_inline)) {
     const int o = w.h * 32 + slot32(w.l);
     const int s = ks * 256 + (w.wave >> 1) * 64 + o;
-    const u32x4* x = b + 3072 + (ks * 2 + (w.wave & 1)) * (64 * KT) + o;
+    const u32x4* x = b + DW_G + (ks * 2 + (w.wave & 1)) * (64 * KT) + o;
     const u32x4 g[3] = {b[2048 + s], b[1024 + s], b[s]};   // small products first
     u32x4 xf[KT];
 #pragma unroll
@@ -934,10 +988,19 @@ void launch_stream(const RowArgs& a, hipStream_t s) {
                      3 * KS * CT * 64 * 16 + 16 * CT * 4, s, a);
 }
 
-constexpr int64_t FEW_TILES = 3072;
+// Few tiles: at most one for each wave of a full launch, so the columns are split finer. Few rows:
+// one row of 256 x 256 forward 4.6 us and dX 6.9 us, against 15 us in k_rows; 16 rows of 128 x 128
+// 5.3 and 4.9 us, 17 rows in the streaming kernel 8.2 and 5.3 us.
+constexpr int64_t FEW_TILES = SW * 256, FEW_ROWS = 16;
 
 template <bool WT, bool MASK, bool Q8>
 int launch_rows(const RowArgs& a, hipStream_t s) {
+  if (a.M <= FEW_ROWS) {
+    const unsigned rows = (unsigned)((a.M + 3) / 4);
+    if constexpr (Q8) hipLaunchKernelGGL(k_few_fwd, dim3((unsigned)ceil_div(a.C, 32), rows), dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((k_few_dx<MASK>), dim3((unsigned)ceil_div(a.C, 64), rows), dim3(512), 0, s, a);
+    return launch_status();
+  }
   // R < 4, or rows so far apart that a tile of them passes 32 bits of bytes: the general kernel
   const bool stream = a.R >= 4 && a.R <= 192 && a.ld_in < MAX_LD && a.ld_out < MAX_LD;
   const bool few = (a.M + 15) / 16 <= FEW_TILES;
@@ -947,10 +1010,19 @@ int launch_rows(const RowArgs& a, hipStream_t s) {
     launch_stream<WT, MASK, Q8, 4, 12>(a, s);   // rows read once, not twice
   else if (stream && a.R <= 128) launch_stream<WT, MASK, Q8, 4, 8>(a, s);
   else if (stream) launch_stream<WT, MASK, Q8, 6, 8>(a, s);
-  else
-    hipLaunchKernelGGL((k_rows<WT, MASK, Q8>),
-                       dim3((unsigned)std::min<int64_t>((a.M + BM - 1) / BM, 1 << 20), (unsigned)ceil_div(a.C, 128)),
-                       dim3(256), 0, s, a);
+  else {
+    const unsigned cols = (unsigned)ceil_div(a.C, 128);
+    const int64_t most = (int64_t)1 << 21;   // workgroups a launch (2^32 threads at most)
+    const int64_t tiles = std::max<int64_t>(1, most / cols);
+    for (int64_t m = 0; m < a.M; m += tiles * 128) {
+      RowArgs b = a;
+      b.M = std::min(a.M - m, tiles * 128);
+      b.in += m * a.ld_in, b.out += m * a.ld_out;
+      if (MASK) b.mask += m * a.ld_mask;
+      if (Q8) b.codes += m * a.ld_codes, b.scales += m * a.ss;
+      hipLaunchKernelGGL((k_rows<WT, MASK, Q8>), dim3((unsigned)((b.M + 127) / 128), cols), dim3(512), 0, s, b);
+    }
+  }
   return launch_status();
 }
 
@@ -1034,7 +1106,8 @@ extern "C" int apn_q8_linear_bwd_dw(const float* dy, int64_t ld_dy, const uint8_
   if (!dw) {
     hipLaunchKernelGGL(q8::k_db, dim3((unsigned)ceil_div(N, 64), 1, (unsigned)sp), dim3(512), 0, s, a);
     if (sp > 1)
-      hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)ceil_div(n, 64)), dim3(1024), 0, s, part, sp, n, (int64_t)0, dw, db);
+      hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)ceil_div(n, 64)), dim3(1024), 0, s, part, sp, n, (int64_t)0, dw,
+                         db);
     return launch_status();
   }
   const int width = q8::dw_width(K);
