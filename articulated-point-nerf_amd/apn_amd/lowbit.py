@@ -11,11 +11,13 @@
   between the layers in 4 bits (``TemporalPoints.feat_format``: preview renders).
 
 Both formats store a row of K values in blocks of 32 consecutive columns (include/apn_hip.h has the
-layout). A block that holds an infinity or NaN reads back as NaN, whole.
+layout). A block that holds an infinity or NaN reads back as NaN, whole; an infinite operand of
+``linear_q8`` makes the results it reaches infinite or NaN.
 
 Device tensors only. Rows are the last dimension; leading dimensions are flattened. Every call runs
 on the current stream of its tensors' device and allocates only through torch, so the functional
-forms (not the autograd one) can be captured into a graph.
+forms (not the autograd one) can be captured into a graph. The functional forms are outside
+autograd: their results carry no gradient.
 """
 from __future__ import annotations
 
@@ -128,7 +130,8 @@ def _act(slope, what):
 
 class _BlockRows:
     """Codes and scales of [rows, cols] values; ``codes`` uint8 [rows, _BYTES ceil(cols / 32)],
-    ``scales`` uint8 [rows, 4 ceil(ceil(cols / 32) / 4)], both contiguous."""
+    ``scales`` uint8 [rows, 4 ceil(ceil(cols / 32) / 4)], both contiguous; codes behind column cols
+    are zeros (q8: 0x80)."""
 
     _BYTES = 0
 
@@ -149,7 +152,6 @@ class _BlockRows:
         _device(what, codes, scales)
         self._buf, self._codes, self._scales = None, codes, scales
         self.rows, self.cols, self.device = codes.shape[0], cols, codes.device
-        self._at = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
     def _empty(cls, rows, cols, device):
@@ -159,9 +161,15 @@ class _BlockRows:
         self._buf = torch.empty(n + rows * _scale_bytes(cols), dtype=torch.uint8, device=device)
         self._codes = self._scales = None
         self.rows, self.cols, self.device = rows, cols, device
-        p = self._buf.data_ptr()
-        self._at = p, p + n
         return self
+
+    @property
+    def _at(self):
+        """The addresses of codes and scales."""
+        if self._buf is None:
+            return self._codes.data_ptr(), self._scales.data_ptr()
+        p = self._buf.data_ptr()
+        return p, p + self.rows * self._BYTES * _blocks(self.cols)
 
     @property
     def codes(self) -> torch.Tensor:
@@ -302,6 +310,11 @@ def linear_q8_backward(dy: torch.Tensor, weight: torch.Tensor, x_kept: Q8Rows | 
     return dx, dw, db
 
 
+def _not_captured(what):
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what}: autograd steps cannot be captured; capture linear_q8 / linear_q8_backward")
+
+
 class _Q8Stack(torch.autograd.Function):
     """A stack of Linear layers: f32 forward, everything the backward needs kept in 8 bits (the
     stack's input and each layer's output, once)."""
@@ -333,6 +346,7 @@ class _Q8Stack(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _not_captured("sequential_q8")
         n = len(ctx.slopes)
         saved = ctx.saved_tensors
         ws, rest = saved[n:2 * n], saved[2 * n:]
@@ -372,8 +386,7 @@ def sequential_q8(layers, x: torch.Tensor, col_pos=None, keep_output=False):
     if not layers:
         raise ValueError(f"{what}: no layers")
     L.require_cuda(x, what=what)
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"{what}: autograd steps cannot be captured; capture linear_q8 / linear_q8_backward")
+    _not_captured(what)
     params = [p for layer, _ in layers for p in (layer.weight, layer.bias)]
     holder = [] if keep_output else None
     y = _Q8Stack.apply(x, tuple(s for _, s in layers), col_pos, holder, *params)
@@ -436,10 +449,13 @@ class MX4Layer:
             raise TypeError(f"MX4Layer: weight must be MX4Rows, got {type(weight).__name__}")
         if bias is not None:
             _device("MX4Layer", weight.codes, bias)
+        bias = _bias(bias, weight.shape[0], "MX4Layer")
         self.weight, self.slope = weight, slope
-        self.bias = _bias(bias, weight.shape[0], "MX4Layer")
-        act, sl = _act(slope, "MX4Layer")
-        self._arg = L.MX4LayerArg(*weight._at, _addr(self.bias), *weight.shape, act, sl)
+        self.bias = None if bias is None else bias.detach().clone()   # (a parameter's storage may be replaced)
+        self._act = _act(slope, "MX4Layer")
+
+    def _arg(self):
+        return L.MX4LayerArg(*self.weight._at, _addr(self.bias), *self.weight.shape, *self._act)
 
 
 def mx4_layers(layers, col_pos=None, width=None):
@@ -477,7 +493,7 @@ def mx4_sequential(layers, x: torch.Tensor, out_dtype=torch.float32) -> torch.Te
     dev = _device(what, rows)
     for y in layers:
         y.weight._index(what, dev)
-    args = (L.MX4LayerArg * len(layers))(*(y._arg for y in layers))
+    args = (L.MX4LayerArg * len(layers))(*(y._arg() for y in layers))
     if len(layers) > 1 and L.load().apn_mx4_network_lds_bytes(len(layers), args):
         out = torch.empty((M, layers[-1].weight.shape[0]), dtype=out_dtype, device=rows.device)
         _launch(dev, "apn_mx4_network", rows.data_ptr(), xt, ldx, M, len(layers), args, out.data_ptr(), t, out.shape[1])

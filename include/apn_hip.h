@@ -489,7 +489,8 @@ int apn_cloud_bbox(const float* xyz, int64_t N, float* out6, int32_t* ord8, void
  *        sign bit says "not positive" also where the magnitude rounds to 0.
  *   mx4: 16 ceil(K / 32) bytes a row, low nibble first, nibble = sign << 3 | index into
  *        {0, 0.5, 1, 1.5, 2, 3, 4, 6}; scale = 2^(floor(log2 max|x|) - 2), nearest, ties to even,
- *        saturating at 6 (the OCP microscaling conversion).
+ *        saturating at 6 (the OCP microscaling conversion). Pad: 0; the products rely on it within
+ *        the last block.
  * ------------------------------------------------------------------------------------- */
 
 /* rows x [M, K] (type, row stride ldx) -> codes, scales; and back into out [M, K] (stride ldo) */
@@ -499,7 +500,7 @@ int apn_q8_unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_
                   int64_t ldo, void* stream);
 /* Training Linear with its output kept in 8 bits: y [M, N] = act(x w^T + bias) in f32 accuracy
  * (x [M, K], w [N, K], bias [N] or NULL; act: LeakyReLU(slope), slope 0 = ReLU), and the q8 codes
- * and scales of y. */
+ * and scales of y. An infinite operand makes the results it reaches infinite or NaN. */
 int apn_q8_linear_fwd(const float* x, int64_t ldx, const float* w, int64_t ldw, const float* bias, int64_t M,
                       int64_t N, int64_t K, int32_t act, float slope, float* y, int64_t ldy, uint8_t* codes,
                       uint8_t* scales, void* stream);
