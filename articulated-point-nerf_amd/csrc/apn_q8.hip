@@ -375,9 +375,12 @@ __global__ __launch_bounds__(64 * SW, SW / 4) void k_rows_stream(RowArgs p) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t k = 0;
-        if (MASK) {   // a quad that moved back has its own columns' codes that many bytes up
-          k = code[ks][i];
-          if (ks == last) k <<= 8 * min(-back[i], 3);
+        if (MASK) {   // a quad that moved back has its own columns' codes that many bytes up, and the
+          k = code[ks][i];   // columns before them, whose weights are 0, masked (they may hold NaN)
+          if (ks == last) {
+            const int up = 8 * min(-back[i], 3);
+            k = k << up | (0x80808080u & ((1u << up) - 1u));
+          }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)

@@ -241,6 +241,47 @@ def test_linear_q8_backward_vs_float64(dev, M, K, N, slope):
         assert torch.equal(one[i], (dx, dw, db)[i]) and all(one[j] is None for j in range(3) if j != i)
 
 
+# sizes around the kernels' limits: 16 | 17 rows, 192 | 193 columns of the reduction, 128-row and
+# 128-column tiles, chunks of 32 columns, many tiles
+EDGES = [(4, 300, 31), (5, 65, 100), (15, 4, 130), (16, 513, 63), (16, 7, 1), (17, 193, 193), (18, 1, 300), (128, 224, 128),
+         (129, 225, 129), (700, 400, 260), (3000, 193, 1), (2500, 193, 700), (49200, 64, 33)]
+
+
+@gpu
+@pytest.mark.parametrize("slope", [None, 0.01])
+@pytest.mark.parametrize("M,K,N", EDGES)
+def test_linear_q8_kernel_edges(dev, M, K, N, slope):
+    test_linear_q8_vs_float64(dev, M, K, N, slope)
+    test_linear_q8_backward_vs_float64(dev, M, K, N, slope)
+
+
+@gpu
+@pytest.mark.parametrize("M", [3, 16, 40])
+@pytest.mark.parametrize("K", [30, 250])
+def test_linear_q8_masked_and_short_rows(dev, M, K):
+    """Small and general row kernels: padded rows whose padding is NaN, gradients that are not finite
+    where slope 0 masks them, one row that holds an infinity beside finite ones."""
+    from apn_amd import lowbit as lb
+    N = 70
+    x, w, b, dy = _rand(M, N, K, M + K, dev)
+    wide = torch.full((M, K + 3), math.nan, device=dev)
+    wide[:, :K] = x
+    y, kept = lb.linear_q8(wide[:, :K], w, b, 0.0)
+    y1, kept1 = lb.linear_q8(x, w, b, 0.0)
+    assert torch.equal(y, y1) and torch.equal(kept.codes, kept1.codes) and torch.equal(kept.scales, kept1.scales)
+    x2 = x.clone()
+    x2[1, K - 1] = math.inf
+    y2, _ = lb.linear_q8(x2, w, b, None)
+    y3, _ = lb.linear_q8(x, w, b, None)
+    rest = torch.arange(M, device=dev) != 1
+    assert torch.equal(y2[rest], y3[rest]) and not torch.isfinite(y2[1]).any()
+    xk = lb.q8_pack(x)
+    bad = torch.where(y > 0, dy, torch.full_like(dy, math.nan))
+    for a, r in zip(lb.linear_q8_backward(bad, w, xk, kept, 0.0),
+                    lb.linear_q8_backward(torch.where(y > 0, dy, torch.zeros_like(dy)), w, xk, kept, 0.0)):
+        assert torch.equal(a, r)
+
+
 @gpu
 def test_linear_q8_large_rows_split_sums(dev):
     """A training step's row count: the weight gradient's split sums against 64 bits."""
@@ -654,6 +695,25 @@ def _functional_step(lb, x, w, b, dy, packed):
 
 
 @gpu
+def test_mx4_layer_is_frozen(dev):
+    """A layer built from a module holds what the module held then: neither an in-place change of the
+    module's parameters nor new storage for them reaches it."""
+    from apn_amd import lowbit as lb
+    from apn_amd.linear import layer_pairs
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(torch.nn.Linear(33, 64), torch.nn.ReLU(), torch.nn.Linear(64, 20)).to(dev)
+    x = torch.randn(50, 33, device=dev)
+    layers = lb.mx4_layers(layer_pairs(net))
+    y = lb.mx4_sequential(layers, x)
+    with torch.no_grad():
+        for p in net.parameters():
+            p.fill_(math.nan)
+            p.data = torch.full_like(p, 7.0)
+    fill = [torch.full((64,), math.nan, device=dev) for _ in range(64)]   # takes freed storage, if any
+    assert torch.equal(lb.mx4_sequential(layers, x), y) and len(fill) == 64
+
+
+@gpu
 def test_captured_and_replayed_beside_eager_work(dev):
     """Two captures of the functional forms share nothing: replayed in turn with eager calls and new
     inputs between them, every replay equals the eager result."""
@@ -719,6 +779,20 @@ def test_autograd_stack_refuses_capture(dev):
         except RuntimeError as e:
             said = str(e)
     assert said is not None and "captured" in said
+
+
+@gpu
+@autograd
+def test_autograd_stack_refuses_captured_backward(dev, monkeypatch):
+    """The backward pass of an eager forward (the capture is pretended: a real one would end in it)."""
+    from apn_amd import linear as LIN
+    net = _stack(dev, [32, 32], [0.01], 1)
+    y = LIN.sequential(net, torch.randn(64, 32, device=dev), checkpoint="q8").sum()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="captured"):
+        y.backward()
+    monkeypatch.undo()
+    assert all(p.grad is None for p in net.parameters())
 
 
 @gpu
