@@ -110,10 +110,20 @@ __device__ __forceinline__ void tile_of(const Args& p, int64_t& m0, int& n0) {
   m0 = (group * 8 + in_group % gm) * RM;
   n0 = (int)(in_group / gm) * RN;
 }
-// without a branch per value: p.below is 1 without an activation, the slope with one
+// p.below is 1 without an activation, the slope with one. ACT: which it is, known where there are many
+// values (NONE, RELU, LEAKY), ANY without a branch per value elsewhere.
+enum { NONE, RELU, LEAKY, ANY };
+template <int ACT>
 __device__ __forceinline__ float activate(const Args& p, float v) {
-  const float b = p.relu ? (v != v ? v : 0.f) : v * p.below;
+  if (ACT == NONE) return v;
+  const float b = ACT == RELU || (ACT == ANY && p.relu) ? (v != v ? v : 0.f) : v * p.below;
   return v > 0.f ? v : b;
+}
+template <typename F>
+__device__ __forceinline__ void with_act(const Args& p, F f) {
+  if (p.relu) f(std::integral_constant<int, RELU>());
+  else if (p.below == 1.f) f(std::integral_constant<int, NONE>());
+  else f(std::integral_constant<int, LEAKY>());
 }
 __device__ __forceinline__ f32x4 bias4(const Args& p, int n) {
   f32x4 b = {0.f, 0.f, 0.f, 0.f};
@@ -123,15 +133,16 @@ __device__ __forceinline__ f32x4 bias4(const Args& p, int n) {
   }
   return b;
 }
+template <int ACT>
 __device__ __forceinline__ void finish4(const Args& p, const f32x4& v, const f32x4& bias, float (&y)[4]) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) y[r] = activate(p, v[r] + bias[r]);
+  for (int r = 0; r < 4; ++r) y[r] = activate<ACT>(p, v[r] + bias[r]);
 }
 // The results of TN column tiles of one row tile, four tiles at a time: 16-bit types are transposed
 // over the four lanes of a row, so that lane q stores the 32 B of tile q and a row's 128 B go out
 // together; floats go out as they are (64 B of a row together). All biases come before any store:
 // a load waited for behind a store waits for the store too.
-template <int T, int TN>
+template <int T, int TN, int ACT>
 __device__ __forceinline__ void store_row(const Args& p, int64_t m, int n0, int q, const f32x4 (&acc)[TN],
                                           const f32x4 (&bias)[TN]) {
   typedef typename Elem<T>::type E;
@@ -149,7 +160,7 @@ __device__ __forceinline__ void store_row(const Args& p, int64_t m, int n0, int 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float y[4];
-          finish4(p, acc[(g + j) % TN], bias[(g + j) % TN], y);
+          finish4<ACT>(p, acc[(g + j) % TN], bias[(g + j) % TN], y);
           a[j] = __builtin_bit_cast(uint32_t, e2{(E)y[0], (E)y[1]});
           b[j] = __builtin_bit_cast(uint32_t, e2{(E)y[2], (E)y[3]});
         }
@@ -166,11 +177,31 @@ __device__ __forceinline__ void store_row(const Args& p, int64_t m, int n0, int 
 #pragma unroll
       for (int j = g; j < g + 4 && j < TN; ++j) {
         float y[4];
-        finish4(p, acc[j], bias[j], y);
+        finish4<ACT>(p, acc[j], bias[j], y);
         if (m < p.M) store4<T>(o + 16 * j + 4 * q, left - 16 * j - 4 * q, y);
       }
     }
   }
+}
+
+// A row's scale bytes of steps s .. s + 3 (word i: step s + i, byte c: block c): zero behind the last
+// block, whatever the padding holds ...
+__device__ __forceinline__ u32x4 trim_scales(const Args& p, int s, u32x4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = p.nb - 4 * (s + i);
+    v[i] = n >= 4 ? v[i] : n <= 0 ? 0u : v[i] & ((1u << (8 * n)) - 1u);
+  }
+  return v;
+}
+// ... and transposed: word c, byte i
+__device__ __forceinline__ u32x4 by_block(u32x4 v) {
+  const uint32_t a = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u);
+  const uint32_t b = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u);
+  const uint32_t d = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u);
+  const uint32_t e = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
+  return u32x4{__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(b, a, 0x07060302u),
+               __builtin_amdgcn_perm(e, d, 0x05040100u), __builtin_amdgcn_perm(e, d, 0x07060302u)};
 }
 
 // Tile kernel: WM x WN waves of TM x TN 16 x 16 tiles. Both operands go through LDS in fragment
@@ -250,21 +281,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(Args p) {
 #pragma unroll
     for (int r = 0; r < SR; ++r) {   // bytes (step i, block c) to (block c, step i)
       u32x4 v = sv[r];
-      if (4 * s + 16 > p.nb) {   // zeros behind the last block, whatever the padding holds
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int n = p.nb - 4 * (s + i);
-          v[i] = n >= 4 ? v[i] : n <= 0 ? 0u : v[i] & ((1u << (8 * n)) - 1u);
-        }
-      }
-      const uint32_t a = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u);
-      const uint32_t b = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u);
-      const uint32_t d = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u);
-      const uint32_t e = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
-      if (ROWS >= THREADS || tid < ROWS)
-        sc[buf + tid + THREADS * r] =
-            u32x4{__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(b, a, 0x07060302u),
-                  __builtin_amdgcn_perm(e, d, 0x05040100u), __builtin_amdgcn_perm(e, d, 0x07060302u)};
+      if (4 * s + 16 > p.nb) v = trim_scales(p, s, v);
+      if (ROWS >= THREADS || tid < ROWS) sc[buf + tid + THREADS * r] = by_block(v);
     }
   };
   f32x4 acc[TM][TN];
@@ -333,9 +351,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(Args p) {
   f32x4 bias[TN];
 #pragma unroll
   for (int j = 0; j < TN; ++j) bias[j] = bias4(p, n0 + (wn * TN + j) * 16 + 4 * q);
+  with_act(p, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
-    store_row<T, TN>(p, m0 + (wm * TM + i) * 16 + l, n0 + wn * TN * 16, q, acc[i], bias);
+    for (int i = 0; i < TM; ++i)
+      store_row<T, TN, decltype(act)::value>(p, m0 + (wm * TM + i) * 16 + l, n0 + wn * TN * 16, q, acc[i], bias);
+  });
 }
 
 // 256 x 256 tile for large products: 4 waves, one per SIMD, each 128 x 128 (256 accumulators), both
@@ -368,10 +388,11 @@ __device__ __forceinline__ void arrive() {
 
 constexpr int TILE256_LDS = 4 * 2 * 256 * 64 + 2 * 2 * 256 * 16;
 
-template <int T>
+// WIDE: rows of scales are whole 16-B pieces (K a multiple of 512) and lie on 16-B boundaries
+template <int T, bool WIDE>
 __global__ __launch_bounds__(256, 1) void k_tile256(Args p) {
   constexpr int R = 256, STAGE = 2 * R * 64, SCALES = 2 * R * 16;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // 4 STAGE of codes, 2 SCALES
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // 4 STAGE of codes, SCALES as read, SCALES turned
   const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave & 1, wn = wave >> 1;
   int64_t m0;
@@ -392,16 +413,15 @@ __global__ __launch_bounds__(256, 1) void k_tile256(Args p) {
     to_lds<16>(base + (int64_t)at * 64 + (int64_t)i * 16 * row_bytes, src - (at == last ? back : 0u),
                lds0 + (s & 3) * STAGE + (wave * 8 + i) * 1024);
   };
-  // scales of steps s .. s + 3: 16 B of a row, 64 rows an instruction, where rows of scales are whole
-  // 16-B pieces (K a multiple of 512), else the four words one by one (word j of all rows together)
+  // Scales of steps s .. s + 3 as they lie in memory: 16 B of a row, 64 rows an instruction, or the
+  // four words one by one (word j of all rows together)
   const uint8_t* const sbase = (xs_side ? p.as : p.bs) + row0 * p.ss;
-  const bool wide = p.ss % 16 == 0 && ((uintptr_t)p.as | (uintptr_t)p.bs) % 16 == 0;
   auto load_scales = [&](int s) __attribute__((always_inline)) {
-    const uint32_t to = lds0 + 4 * STAGE + ((s >> 2) & 1) * SCALES;
+    const uint32_t to = lds0 + 4 * STAGE;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint8_t* const b = sbase + (int64_t)i * 64 * p.ss;
-      if (wide) {
+      if (WIDE) {
         to_lds<16>(b + min(4 * s, p.ss - 16), (uint32_t)lane * (uint32_t)p.ss, to + (wave * 2 + i) * 1024);
       } else {
 #pragma unroll
@@ -410,6 +430,26 @@ __global__ __launch_bounds__(256, 1) void k_tile256(Args p) {
                     to + j * 2048 + (wave * 2 + i) * 256);
       }
     }
+  };
+  // ... and as they are used: a row's words by block, byte i that of step s + i; a thread turns two rows.
+  // (Every lane picking its bytes from the rows as they lie, 16 B read for 4 B used: 91 us against 85,
+  // 8192 x 4096 x 4096.)
+  u32x4* const turned = (u32x4*)(lds + 4 * STAGE + SCALES);
+  auto raw_scales = [&](int r) __attribute__((always_inline)) {
+    const uint8_t* const b = lds + 4 * STAGE;
+    const int row = tid + 256 * r;
+    u32x4 v;
+    if (WIDE) {
+      v = *(const u32x4*)(b + 16 * row);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = *(const uint32_t*)(b + j * 2048 + 4 * row);
+    }
+    return v;
+  };
+  auto turn_scales = [&](int s, int r, u32x4 v) __attribute__((always_inline)) {
+    v = trim_scales(p, s, v);   // (a branch here, and the step's products move behind it)
+    turned[tid + 256 * r] = by_block(v);
   };
   f32x4 acc[8][8];
 #pragma unroll
@@ -424,30 +464,18 @@ __global__ __launch_bounds__(256, 1) void k_tile256(Args p) {
     x[i] = *(const u32x4*)(b + (wm * 8 + i) * 1024);
     w[i] = *(const u32x4*)(b + (16 + wn * 8 + i) * 1024);
   };
-  // a row's scales of four steps: byte q of the four words
-  const uint32_t pick = 0x0c0c0400u + 0x0101u * q;
-  auto raw_scale = [&](int s, int row) __attribute__((always_inline)) {
-    const uint8_t* b = lds + 4 * STAGE + ((s >> 2) & 1) * SCALES;
-    u32x4 v;
-    if (wide) {
-      v = *(const u32x4*)(b + 16 * row);
-    } else {
+  auto scale_of = [&](int row) __attribute__((always_inline)) { return ((const int*)(turned + row + l))[q]; };
+  // blocks of step s behind the last one: X's codes as zeros (in LDS: in registers, the compiler
+  // copies the fragments around the branch in every step)
+  auto clear = [&](int s) __attribute__((always_inline)) {
+    const int have = p.nb - 4 * s;
+    if (have < 4) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = *(const uint32_t*)(b + j * 2048 + 4 * row);
-    }
-    return v;
-  };
-  auto scale_of = [&](const u32x4& v) __attribute__((always_inline)) {
-    return (int)(__builtin_amdgcn_perm(v[1], v[0], pick) | __builtin_amdgcn_perm(v[3], v[2], pick) << 16);
-  };
-  // zero behind the last block, whatever the padding holds
-  auto trim_scales = [&](int s) __attribute__((always_inline)) {
-    if (4 * s + 16 > p.nb) {
-      const int n = (p.nb - 4 * s - q + 3) / 4;   // steps whose block q exists
-      const uint32_t keep = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
-      asm volatile("");
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sm[i] &= keep, sn[i] &= keep;
+      for (int j = 0; j < 4; ++j) {
+        const int at = tid + 256 * j, c = (at & 3) ^ ((at >> 4) & 3);   // slot 4 r + (c ^ r / 4) of a row tile
+        if (c >= have) *(u32x4*)(lds + (s & 3) * STAGE + 16 * at) = u32x4{0u, 0u, 0u, 0u};
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
   };
   load_scales(0);
@@ -456,13 +484,16 @@ __global__ __launch_bounds__(256, 1) void k_tile256(Args p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) load(s, i);
   arrive<16>();
+  turn_scales(0, 0, raw_scales(0));
+  turn_scales(0, 1, raw_scales(1));
+  clear(0);
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     fetch(0, i, xf[0], wf[0]);
-    sm[i] = scale_of(raw_scale(0, (wm * 8 + i) * 16 + l));
-    sn[i] = scale_of(raw_scale(0, 256 + (wn * 8 + i) * 16 + l));
+    sm[i] = scale_of((wm * 8 + i) * 16);
+    sn[i] = scale_of(256 + (wn * 8 + i) * 16);
   }
-  trim_scales(0);
   for (int s = 0; s < steps; s += 4) {
     auto turn = [&](auto I) __attribute__((always_inline)) {
       constexpr int i = decltype(I)::value;
@@ -470,34 +501,27 @@ __global__ __launch_bounds__(256, 1) void k_tile256(Args p) {
       // Step s + i + 1 has arrived when no more are out than the last step sent: 8, and the scales
       // with step 0's. Every wave then has its fragments of the buffer that is written next.
       if (i != 1) arrive<8>();
-      else if (wide) arrive<10>();
-      else arrive<16>();
+      else arrive<WIDE ? 10 : 16>();
       if (i == 0) load_scales(s + 4);
-      if (s + i == last && blocks < 4) {   // blocks behind the last one: X's codes as zeros
-        asm volatile("");                  // (a branch: as selects they would run in every step)
-#pragma unroll
-        for (int m = 0; m < 8; ++m)
-          if (q >= blocks) xf[i & 1][m] = u32x4{0u, 0u, 0u, 0u};
-      }
-      u32x4 a, b;
+      clear(s + i + 1);
       int next[8];
+      u32x4 raw;   // (there since this turn's wait; turned, they are read behind the next one)
 #pragma unroll
       for (int m = 0; m < 8; ++m) {
         fetch(s + i + 1, m, xf[(i & 1) ^ 1], wf[(i & 1) ^ 1]);
-        if (i == 3) {   // the next group's scales
-          a = raw_scale(s + 4, (wm * 8 + m) * 16 + l);
-          b = raw_scale(s + 4, 256 + (wn * 8 + m) * 16 + l);
-        }
+        if (i == 2 && m % 4 == 1) raw = raw_scales(m / 4);
+        if (i == 2 && m % 4 == 3) turn_scales(s + 4, m / 4, raw);
+        int x_scale;
+        if (i == 3) x_scale = scale_of((wm * 8 + m) * 16), next[m] = scale_of(256 + (wn * 8 + m) * 16);
 #pragma unroll
         for (int n = 0; n < 8; ++n) acc[m][n] = mma<i>(wf[i & 1][n], sn[n], xf[i & 1][m], sm[m], acc[m][n]);
         load(s + i + 3, m);
-        if (i == 3) sm[m] = scale_of(a), next[m] = scale_of(b);
+        if (i == 3) sm[m] = x_scale;
         __builtin_amdgcn_sched_barrier(0);
       }
       if (i == 3) {
 #pragma unroll
         for (int m = 0; m < 8; ++m) sn[m] = next[m];
-        trim_scales(s + 4);
       }
     };
     turn(std::integral_constant<int, 0>());
@@ -509,8 +533,11 @@ __global__ __launch_bounds__(256, 1) void k_tile256(Args p) {
   f32x4 bias[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) bias[j] = bias4(p, n0 + (wn * 8 + j) * 16 + 4 * q);
+  with_act(p, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) store_row<T, 8>(p, m0 + (wm * 8 + i) * 16 + l, n0 + wn * 128, q, acc[i], bias);
+    for (int i = 0; i < 8; ++i)
+      store_row<T, 8, decltype(act)::value>(p, m0 + (wm * 8 + i) * 16 + l, n0 + wn * 128, q, acc[i], bias);
+  });
 }
 
 // Up to 16 rows: 16 columns a workgroup, K over its 8 waves -- two steps (128 B of a row of B, a
@@ -594,7 +621,7 @@ __global__ __launch_bounds__(512) void k_few(FewArgs f) {
     for (int j = 1; j < 8; ++j) t += red[64 * j + lane];
     float y[4];
     const int c = n0 + 4 * q;
-    finish4(p, t, bias4(p, c), y);
+    finish4<ANY>(p, t, bias4(p, c), y);
     typedef typename Elem<T>::type E;
     store4<T>((E*)p.out + l * p.ld_out + c, p.N - c, y);
   }
@@ -755,7 +782,7 @@ __global__ __launch_bounds__(64 * SW, SW / 4) void k_network(NetArgs f) {
         for (int t = 0; t < NT; ++t) none[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         Args p{};
         p.out = f.out, p.M = f.M, p.ld_out = f.ld_out, p.N = y.N, p.relu = y.relu, p.below = y.below;
-        store_row<T, NT>(p, tile * 16 + l, 0, q, acc, none);
+        store_row<T, NT, ANY>(p, tile * 16 + l, 0, q, acc, none);
         break;
       }
       os = 0;
@@ -826,6 +853,12 @@ void launch_tile(const Args& a, hipStream_t s) {
   hipLaunchKernelGGL((k_tile<WM, WN, TM, TN, T>), dim3((unsigned)tiles_of<WM, WN, TM, TN, T>(a)), dim3(64 * WM * WN), 0,
                      s, a);
 }
+template <int T>
+void launch_tile256(const Args& a, hipStream_t s) {
+  const bool wide = a.ss % 16 == 0 && ((uintptr_t)a.as | (uintptr_t)a.bs) % 16 == 0;
+  const auto kernel = wide ? k_tile256<T, true> : k_tile256<T, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles_of<2, 2, 8, 8, T>(a)), dim3(256), TILE256_LDS, s, a);
+}
 // The largest tile that still gives most CUs one
 template <int T>
 void launch_linear(const Args& a, hipStream_t s) {
@@ -834,7 +867,7 @@ void launch_linear(const Args& a, hipStream_t s) {
     return;
   }
   if (a.N >= 256 && a.M >= 256 && tiles_of<2, 2, 8, 8, T>(a) >= 192)
-    hipLaunchKernelGGL((k_tile256<T>), dim3((unsigned)tiles_of<2, 2, 8, 8, T>(a)), dim3(256), TILE256_LDS, s, a);
+    launch_tile256<T>(a, s);
   else if (tiles_of<2, 2, 4, 4, T>(a) >= 128) launch_tile<2, 2, 4, 4, T>(a, s);
   else launch_tile<2, 2, 2, 2, T>(a, s);
 }
