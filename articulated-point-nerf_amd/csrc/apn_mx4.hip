@@ -87,8 +87,8 @@ struct Args {
   const float* bias;
   void* out;
   int64_t M, ld_out;
-  int N, nb, ss, relu;   // nb: blocks of K; ss: bytes per scale row
-  float below;           // factor of results that are not positive
+  int N, nb, ss, act;   // nb: blocks of K; ss: bytes per scale row
+  float slope;
 };
 
 template <int I>   // the scales are byte I of sa and sb
@@ -110,20 +110,25 @@ __device__ __forceinline__ void tile_of(const Args& p, int64_t& m0, int& n0) {
   m0 = (group * 8 + in_group % gm) * RM;
   n0 = (int)(in_group / gm) * RN;
 }
-// p.below is 1 without an activation, the slope with one. ACT: which it is, known where there are many
-// values (NONE, RELU, LEAKY), ANY without a branch per value elsewhere.
-enum { NONE, RELU, LEAKY, ANY };
+// The activation, by kind: none, ReLU, LeakyReLU with a slope below 1 and with any other. (A maximum
+// that keeps NaN is one instruction where comparing and selecting are up to six.)
+enum { NONE, RELU, LEAKY, SLOPE };
+inline int act_kind(int act, float slope) {
+  return !act || slope == 1.f ? NONE : slope == 0.f ? RELU : slope < 1.f ? LEAKY : SLOPE;
+}
 template <int ACT>
-__device__ __forceinline__ float activate(const Args& p, float v) {
-  if (ACT == NONE) return v;
-  const float b = ACT == RELU || (ACT == ANY && p.relu) ? (v != v ? v : 0.f) : v * p.below;
-  return v > 0.f ? v : b;
+__device__ __forceinline__ float activate(float v, float slope) {
+  if (ACT == RELU) return __builtin_elementwise_maximum(v, 0.f);
+  if (ACT == LEAKY) return __builtin_elementwise_maximum(v, v * slope);
+  if (ACT == SLOPE) return v > 0.f ? v : v * slope;
+  return v;
 }
 template <typename F>
-__device__ __forceinline__ void with_act(const Args& p, F f) {
-  if (p.relu) f(std::integral_constant<int, RELU>());
-  else if (p.below == 1.f) f(std::integral_constant<int, NONE>());
-  else f(std::integral_constant<int, LEAKY>());
+__device__ __forceinline__ void with_act(int act, F f) {   // act: uniform
+  if (act == LEAKY) f(std::integral_constant<int, LEAKY>());
+  else if (act == RELU) f(std::integral_constant<int, RELU>());
+  else if (act == NONE) f(std::integral_constant<int, NONE>());
+  else f(std::integral_constant<int, SLOPE>());
 }
 __device__ __forceinline__ f32x4 bias4(const Args& p, int n) {
   f32x4 b = {0.f, 0.f, 0.f, 0.f};
@@ -136,18 +141,16 @@ __device__ __forceinline__ f32x4 bias4(const Args& p, int n) {
 template <int ACT>
 __device__ __forceinline__ void finish4(const Args& p, const f32x4& v, const f32x4& bias, float (&y)[4]) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) y[r] = activate<ACT>(p, v[r] + bias[r]);
+  for (int r = 0; r < 4; ++r) y[r] = activate<ACT>(v[r] + bias[r], p.slope);
 }
 // The results of TN column tiles of one row tile, four tiles at a time: 16-bit types are transposed
 // over the four lanes of a row, so that lane q stores the 32 B of tile q and a row's 128 B go out
 // together; floats go out as they are (64 B of a row together). All biases come before any store:
-// a load waited for behind a store waits for the store too.
-template <int T, int TN, int ACT>
-__device__ __forceinline__ void store_row(const Args& p, int64_t m, int n0, int q, const f32x4 (&acc)[TN],
-                                          const f32x4 (&bias)[TN]) {
+// a load waited for behind a store waits for the store too. values(t, y): the four of tile t.
+template <int T, int TN, typename F>
+__device__ __forceinline__ void store_row(void* out, int64_t ld_out, int64_t m, bool live, int left, int q, F values) {
   typedef typename Elem<T>::type E;
-  E* o = (E*)p.out + m * p.ld_out + n0;
-  const int left = p.N - n0;
+  E* o = (E*)out + m * ld_out;
 #pragma unroll
   for (int g = 0; g < TN; g += 4) {
     bool whole = false;
@@ -160,13 +163,13 @@ __device__ __forceinline__ void store_row(const Args& p, int64_t m, int n0, int 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float y[4];
-          finish4<ACT>(p, acc[(g + j) % TN], bias[(g + j) % TN], y);
+          values((g + j) % TN, y);
           a[j] = __builtin_bit_cast(uint32_t, e2{(E)y[0], (E)y[1]});
           b[j] = __builtin_bit_cast(uint32_t, e2{(E)y[2], (E)y[3]});
         }
         transpose4(a);
         transpose4(b);
-        if (m < p.M) {
+        if (live) {
           E* d = o + 16 * (g + q);
           *(u32x4u*)d = u32x4{a[0], b[0], a[1], b[1]};
           *(u32x4u*)(d + 8) = u32x4{a[2], b[2], a[3], b[3]};
@@ -177,8 +180,8 @@ __device__ __forceinline__ void store_row(const Args& p, int64_t m, int n0, int 
 #pragma unroll
       for (int j = g; j < g + 4 && j < TN; ++j) {
         float y[4];
-        finish4<ACT>(p, acc[j], bias[j], y);
-        if (m < p.M) store4<T>(o + 16 * j + 4 * q, left - 16 * j - 4 * q, y);
+        values(j, y);
+        if (live) store4<T>(o + 16 * j + 4 * q, left - 16 * j - 4 * q, y);
       }
     }
   }
@@ -351,10 +354,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(Args p) {
   f32x4 bias[TN];
 #pragma unroll
   for (int j = 0; j < TN; ++j) bias[j] = bias4(p, n0 + (wn * TN + j) * 16 + 4 * q);
-  with_act(p, [&](auto act) __attribute__((always_inline)) {
+  const int c0 = n0 + wn * TN * 16;
+  with_act(p.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
-      store_row<T, TN, decltype(act)::value>(p, m0 + (wm * TM + i) * 16 + l, n0 + wn * TN * 16, q, acc[i], bias);
+    for (int i = 0; i < TM; ++i) {
+      const int64_t m = m0 + (wm * TM + i) * 16 + l;
+      store_row<T, TN>((typename Elem<T>::type*)p.out + c0, p.ld_out, m, m < p.M, p.N - c0, q,
+                       [&](int t, float (&y)[4]) __attribute__((always_inline)) {
+                         finish4<decltype(act)::value>(p, acc[i][t], bias[t], y);
+                       });
+    }
   });
 }
 
@@ -533,10 +542,14 @@ __global__ __launch_bounds__(256, 1) void k_tile256(Args p) {
   f32x4 bias[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) bias[j] = bias4(p, n0 + (wn * 8 + j) * 16 + 4 * q);
-  with_act(p, [&](auto act) __attribute__((always_inline)) {
+  const int c0 = n0 + wn * 128;
+  with_act(p.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      store_row<T, 8, decltype(act)::value>(p, m0 + (wm * 8 + i) * 16 + l, n0 + wn * 128, q, acc[i], bias);
+      store_row<T, 8>((typename Elem<T>::type*)p.out + c0, p.ld_out, m0 + (wm * 8 + i) * 16 + l, true, p.N - c0, q,
+                      [&](int t, float (&y)[4]) __attribute__((always_inline)) {
+                        finish4<decltype(act)::value>(p, acc[i][t], bias[t], y);
+                      });
   });
 }
 
@@ -621,7 +634,8 @@ __global__ __launch_bounds__(512) void k_few(FewArgs f) {
     for (int j = 1; j < 8; ++j) t += red[64 * j + lane];
     float y[4];
     const int c = n0 + 4 * q;
-    finish4<ANY>(p, t, bias4(p, c), y);
+    const f32x4 bias = bias4(p, c);
+    with_act(p.act, [&](auto act) __attribute__((always_inline)) { finish4<decltype(act)::value>(p, t, bias, y); });
     typedef typename Elem<T>::type E;
     store4<T>((E*)p.out + l * p.ld_out + c, p.N - c, y);
   }
@@ -638,8 +652,8 @@ struct NetLayer {
   const uint8_t* codes;
   const uint8_t* scales;
   const float* bias;
-  int N, nb, ss, relu;
-  float below;
+  int N, nb, ss;
+  float slope, floor;   // activation: risen()
   int at;   // byte offset of its LDS part: codes [column tile][step][lane] 16 B, scales [tile][lane], biases
 };
 constexpr int NET_DEPTH = 8, NET_COLS = 256;
@@ -656,12 +670,17 @@ inline int net_bytes(int N, int nb) {
   return tiles * (((nb + 3) / 4) * 1024 + 256 + 64);
 }
 
+// Any activation of slope at most 1 without a branch: ReLU has slope 0 and floor 0 (which also takes
+// the place of 0 x infinity), LeakyReLU and none (slope 1) floor -infinity.
+__device__ __forceinline__ float risen(float v, const NetLayer& y) {
+  return __builtin_elementwise_maximum(v, fmaxf(v * y.slope, y.floor));
+}
 // one block's 8 values of a lane (columns 4 q .. and 16 + 4 q ..): 4 + 4 nibbles, and the scale byte
 __device__ __forceinline__ uint32_t quant_block(const float (&v)[8], int& byte) {
-  uint32_t a = 0;
+  float a = fabsf(v[0]);   // (the maximum keeps NaN)
 #pragma unroll
-  for (int j = 0; j < 8; ++j) a = max(a, abs_bits(v[j]));
-  byte = mx4_byte(row_max(a));
+  for (int j = 1; j < 8; ++j) a = __builtin_elementwise_maximum(a, fabsf(v[j]));
+  byte = mx4_byte(row_max(abs_bits(a)));
   return quant8(v, byte);
 }
 // four blocks' nibbles as the operand of a step: lane q's block, its columns in order
@@ -777,12 +796,11 @@ __global__ __launch_bounds__(64 * SW, SW / 4) void k_network(NetArgs f) {
           acc[t] = a;
         }
       if (d + 1 == f.depth) {
-        f32x4 none[NT];   // (the biases are in the sums)
+        const int64_t m = tile * 16 + l;
+        store_row<T, NT>(f.out, f.ld_out, m, m < f.M, y.N, q, [&](int t, float (&v)[4]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) none[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        Args p{};
-        p.out = f.out, p.M = f.M, p.ld_out = f.ld_out, p.N = y.N, p.relu = y.relu, p.below = y.below;
-        store_row<T, NT, ANY>(p, tile * 16 + l, 0, q, acc, none);
+          for (int j = 0; j < 4; ++j) v[j] = risen(acc[t][j], y);
+        });
         break;
       }
       os = 0;
@@ -795,10 +813,7 @@ __global__ __launch_bounds__(64 * SW, SW / 4) void k_network(NetArgs f) {
           if (t < nt) {
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float z = acc[t + (j >> 2)][j & 3], b = y.relu ? (z != z ? z : 0.f) : z * y.below;
-              v[j] = z > 0.f ? z : b;
-            }
+            for (int j = 0; j < 8; ++j) v[j] = risen(acc[t + (j >> 2)][j & 3], y);
             int byte;
             r[k] = quant_block(v, byte);   // (columns behind N are zeros: zero weights and bias)
             sb |= (uint32_t)byte << (8 * k);
@@ -943,7 +958,7 @@ extern "C" int apn_mx4_linear(const uint8_t* a_codes, const uint8_t* a_scales, c
   for (int64_t m = 0; m < M; m += piece) {
     char* o = (char*)out + m * ld_out * (type == APN_F32 ? 4 : 2);
     mx4::Args a{a_codes + m * row, a_scales + m * ss, b_codes, b_scales, bias, o, std::min(piece, M - m), ld_out,
-                (int)N, (int)blocks_of(K), (int)ss, act && slope == 0.f, act ? slope : 1.f};
+                (int)N, (int)blocks_of(K), (int)ss, mx4::act_kind(act, slope), slope};
     if (type == APN_F32) mx4::launch_linear<APN_F32>(a, s);
     else if (type == APN_BF16) mx4::launch_linear<APN_BF16>(a, s);
     else mx4::launch_linear<APN_F16>(a, s);
@@ -960,7 +975,7 @@ extern "C" int apn_mx4_linear_few(const void* x, int32_t x_type, int64_t ldx, co
   if (M == 0) return APN_OK;
   if (!x || !b_codes || !b_scales || !out || (uintptr_t)b_codes % 16 || (uintptr_t)b_scales % 4) return APN_ERR_ARG;
   const mx4::FewArgs a{{nullptr, nullptr, b_codes, b_scales, bias, out, M, ld_out, (int)N, (int)blocks_of(K),
-                        (int)scale_stride(K), act && slope == 0.f, act ? slope : 1.f}, x, ldx, (int)K};
+                        (int)scale_stride(K), mx4::act_kind(act, slope), slope}, x, ldx, (int)K};
   hipStream_t s = (hipStream_t)stream;
   if (x_type == APN_F32) mx4::launch_few<APN_F32>(a, type, s);
   else if (x_type == APN_BF16) mx4::launch_few<APN_BF16>(a, type, s);
@@ -973,7 +988,9 @@ extern "C" size_t apn_mx4_network_lds_bytes(int32_t depth, const apn_mx4_layer* 
   size_t bytes = 0;
   for (int d = 0; d < depth; ++d) {
     const apn_mx4_layer& y = layers[d];
-    if (y.N < 1 || y.K < 1 || y.N > mx4::NET_COLS || y.K > mx4::NET_COLS || (d && y.K != layers[d - 1].N)) return 0;
+    if (y.N < 1 || y.K < 1 || y.N > mx4::NET_COLS || y.K > mx4::NET_COLS || (d && y.K != layers[d - 1].N) ||
+        (y.act && !(y.slope <= 1.f)))
+      return 0;
     bytes += (size_t)mx4::net_bytes((int)y.N, (int)blocks_of(y.K));
   }
   return bytes <= 160 * 1024 ? bytes : 0;
@@ -993,7 +1010,7 @@ extern "C" int apn_mx4_network(const void* x, int32_t x_type, int64_t ldx, int64
     const apn_mx4_layer& y = layers[d];
     if (!y.codes || !y.scales || (uintptr_t)y.codes % 16) return APN_ERR_ARG;
     a.layer[d] = {y.codes, y.scales, y.bias, (int)y.N, (int)blocks_of(y.K), (int)scale_stride(y.K),
-                  y.act && y.slope == 0.f, y.act ? y.slope : 1.f, a.bytes};
+                  y.act ? y.slope : 1.f, y.act && y.slope == 0.f ? 0.f : -INFINITY, a.bytes};
     a.bytes += mx4::net_bytes((int)y.N, (int)blocks_of(y.K));
   }
   hipStream_t s = (hipStream_t)stream;

@@ -535,7 +535,7 @@ int apn_mx4_linear_few(const void* x, int32_t x_type, int64_t ldx, const uint8_t
 /* A stack of such layers on float rows x [M, K0] in one launch, the rows between them in mx4:
  * h = x; h = act(mx4(h) b^T + bias) for each layer; out [M, N of the last]. Layers in a host array;
  * K of each but the first = N of the one before; apn_mx4_network_lds_bytes says whether the stack
- * fits (depth <= 8, K and N <= 256, the weights' bytes): 0 = no. ldx, ld_out < 2^24. */
+ * fits (depth <= 8, K and N <= 256, slopes <= 1, the weights' bytes): 0 = no. ldx, ld_out < 2^24. */
 typedef struct {
   const uint8_t* codes;
   const uint8_t* scales;
