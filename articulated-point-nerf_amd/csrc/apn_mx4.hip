@@ -647,7 +647,9 @@ __global__ __launch_bounds__(512) void k_few(FewArgs f) {
 // is 8 values of each of a row's four lanes, its codes 32 bits a lane, and four blocks transposed over
 // the four lanes are the next product's operand: lane q the 16 B of block 4 s + q. The input's floats
 // come in the same arrangement (four lanes on 64 B of a row), the next tile's while this one is
-// computed. Bound by the input and output rows.
+// computed. 262144 rows through 191-128-128-128-128 take 76 us, the input and output rows' 52 us at a
+// copy's rate; bound by vector instructions (about 1100 a tile: with compares and selects for the
+// activations 1580 and 95 us) and by the registers that the rows on their way leave.
 struct NetLayer {
   const uint8_t* codes;
   const uint8_t* scales;
@@ -675,13 +677,37 @@ inline int net_bytes(int N, int nb) {
 __device__ __forceinline__ float risen(float v, const NetLayer& y) {
   return __builtin_elementwise_maximum(v, fmaxf(v * y.slope, y.floor));
 }
-// one block's 8 values of a lane (columns 4 q .. and 16 + 4 q ..): 4 + 4 nibbles, and the scale byte
-__device__ __forceinline__ uint32_t quant_block(const float (&v)[8], int& byte) {
-  float a = fabsf(v[0]);   // (the maximum keeps NaN)
+// A lane has 8 values of each of four blocks (columns 4 q .. and 16 + 4 q ..): the largest magnitude of
+// one block's (NaN if there is one) ...
+__device__ __forceinline__ uint32_t max8(const float (&v)[8]) {
+  float a = fabsf(v[0]);
 #pragma unroll
   for (int j = 1; j < 8; ++j) a = __builtin_elementwise_maximum(a, fabsf(v[j]));
-  byte = mx4_byte(row_max(abs_bits(a)));
-  return quant8(v, byte);
+  return abs_bits(a);
+}
+// ... of block q over the row's four lanes, of all four at once ...
+__device__ __forceinline__ uint32_t group_max(const uint32_t (&a)[4]) {
+  const auto s = __builtin_amdgcn_permlane32_swap(a[0], a[2], false, false);
+  const auto t = __builtin_amdgcn_permlane32_swap(a[1], a[3], false, false);
+  const auto u = __builtin_amdgcn_permlane16_swap(max(s[0], s[1]), max(t[0], t[1]), false, false);
+  return max(u[0], u[1]);
+}
+// ... the four scale bytes, block q's in lane q, in every lane ...
+__device__ __forceinline__ uint32_t all_bytes(int byte, int q) {
+  const uint32_t w = (uint32_t)byte << (8 * q);
+  const auto s = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  const uint32_t v = s[0] | s[1];
+  const auto t = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return t[0] | t[1];
+}
+// ... and block k's codes (of a block that is not finite any: its scale says so)
+__device__ __forceinline__ uint32_t quant8_of(const float (&v)[8], uint32_t bytes, int k) {
+  const float sc = __uint_as_float(max((bytes >> (8 * k) & 0xffu) << 23, 0x00400000u));
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], sc, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], sc, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], sc, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], sc, 3);
 }
 // four blocks' nibbles as the operand of a step: lane q's block, its columns in order
 __device__ __forceinline__ u32x4 to_operand(uint32_t (&r)[4]) {
@@ -757,27 +783,35 @@ __global__ __launch_bounds__(64 * SW, SW / 4) void k_network(NetArgs f) {
     for (int s = 0; s < STEPS; ++s) op[s] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
     for (int s = 0; s < (KB + 3) / 4; ++s) {   // the input
-      uint32_t r[4] = {0u, 0u, 0u, 0u}, sb = 0;
+      uint32_t r[4] = {0u, 0u, 0u, 0u}, top[4] = {0u, 0u, 0u, 0u};
+      auto values = [&](int b, float (&v)[8]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int k = 0; k < 4 && 4 * s + k < KB; ++k) {
-        const int b = 4 * s + k;
-        if (b <= last) {
+        for (int j = 0; j < 8; ++j) v[j] = (float)x[b][j >> 2][j & 3];
+        if (b == last && !whole) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = 32 * b + 16 * (j >> 2) + 4 * q + (j & 3) < f.K ? v[j] : 0.f;
+        }
+      };
+#pragma unroll
+      for (int k = 0; k < 4 && 4 * s + k < KB; ++k)
+        if (4 * s + k <= last) {
           float v[8];
+          values(4 * s + k, v);
+          top[k] = max8(v);
+        }
+      const int byte = mx4_byte(group_max(top));
+      const uint32_t bytes = all_bytes(byte, q);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = (float)x[b][j >> 2][j & 3];
-          if (b == last && !whole) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = 32 * b + 16 * (j >> 2) + 4 * q + (j & 3) < f.K ? v[j] : 0.f;
-          }
-          int byte;
-          r[k] = quant_block(v, byte);
-          sb |= (uint32_t)byte << (8 * k);
-          if (more) load(tile + stride, b);
+      for (int k = 0; k < 4 && 4 * s + k < KB; ++k)
+        if (4 * s + k <= last) {
+          float v[8];
+          values(4 * s + k, v);
+          r[k] = quant8_of(v, bytes, k);
+          if (more) load(tile + stride, 4 * s + k);
           __builtin_amdgcn_sched_barrier(0);
         }
-      }
       op[s] = to_operand(r);
-      os |= ((sb >> (8 * q)) & 0xffu) << (8 * s);
+      os |= (uint32_t)byte << (8 * s);
     }
     for (int d = 0; d < f.depth; ++d) {
       const NetLayer& y = f.layer[d];
@@ -814,8 +848,8 @@ __global__ __launch_bounds__(64 * SW, SW / 4) void k_network(NetArgs f) {
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = risen(acc[t + (j >> 2)][j & 3], y);
-            int byte;
-            r[k] = quant_block(v, byte);   // (columns behind N are zeros: zero weights and bias)
+            const int byte = mx4_byte(row_max(max8(v)));   // (columns behind N are zeros: zero weights and bias)
+            r[k] = quant8_of(v, (uint32_t)byte, 0);
             sb |= (uint32_t)byte << (8 * k);
             __builtin_amdgcn_sched_barrier(0);
           }

@@ -979,3 +979,38 @@ def test_refusals_gpu(dev):
         lb.mx4_sequential([w], x)
     with pytest.raises(TypeError, match="float"):
         lb.mx4_sequential([layer], x.double())
+
+
+@gpu
+@pytest.mark.parametrize("slopes", [[2.0, None, 2.0], [0.01, 1.0, 1.5], [-2.0, 1.0, 0.0]])
+def test_mx4_sequential_other_slopes(dev, slopes):
+    """Slopes of 1, above and below: the stack equals its layers one after the other (the one-launch
+    form takes slopes up to 1, others go layer by layer)."""
+    from apn_amd import lowbit as lb
+    g = torch.Generator(device=dev).manual_seed(7)
+    layers, k = [], 100
+    for n, slope in zip((64, 96, 33), slopes):
+        w = torch.randint(-3, 4, (n, k), device=dev, generator=g).float()   # exact sums in any order
+        layers.append(lb.MX4Layer(lb.mx4_quantize(w), torch.randint(-2, 3, (n,), device=dev, generator=g).float(), slope))
+        k = n
+    h = torch.randint(-6, 7, (130, 100), device=dev, generator=g).float()
+    y = lb.mx4_sequential(layers, h)
+    for layer in layers:
+        h = lb.mx4_linear(h, layer.weight, layer.bias, layer.slope)
+    assert torch.equal(y, h)
+
+
+@gpu
+def test_mx4_sequential_overflow(dev):
+    """Sums that leave float32's range: ReLU takes -inf to 0 and +inf to NaN (its block's scale), the
+    other rows are untouched."""
+    from apn_amd import lowbit as lb
+    big = torch.full((32, 32), 3e38, device=dev)
+    x = torch.zeros(20, 32, device=dev)
+    x[3], x[5] = -4.0, 4.0
+    first = lb.MX4Layer(lb.mx4_quantize(big), None, 0.0)
+    second = lb.MX4Layer(lb.mx4_quantize(torch.ones(16, 32, device=dev)), torch.ones(16, device=dev), None)
+    y = lb.mx4_sequential([first, second], x)
+    want = torch.ones(20, 16, device=dev)
+    want[5] = math.nan
+    assert torch.equal(torch.nan_to_num(y, nan=7.0), torch.nan_to_num(want, nan=7.0))
