@@ -369,8 +369,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(Args p) {
 
 // 256 x 256 tile for large products: 4 waves, one per SIMD, each 128 x 128 (256 accumulators), both
 // operands straight from memory into LDS (no registers on the way), four buffers of one step (32 KB)
-// so that three steps are on their way: a step is 0.43 us of matrix work and L2 answers in about 1 us
-// (with one step on its way in registers the 8192 x 4096 x 4096 product took 150 us, with two 119).
+// so that three steps are on their way: a step is 0.5 us of matrix work and L2 answers in about 1 us
+// (with one step on its way in registers the 8192 x 4096 x 4096 product took 150 us, with two 119; here
+// 84, of which the products alone are 50, the results' stores 13 and their arithmetic 3). Bound by the
+// matrix units' rate under load, the loads beside them, and an epilogue that nothing hides.
 // The LDS side of such a load is lane by lane, so the lanes choose what they read: row lane / 4, and
 // of its four blocks the one that lands conflict-free -- slot 4 r + (c ^ r / 4) of a 16-row tile. The
 // next step's fragments come from LDS while this step's are multiplied.
@@ -908,15 +910,15 @@ void launch_tile256(const Args& a, hipStream_t s) {
   const auto kernel = wide ? k_tile256<T, true> : k_tile256<T, false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)tiles_of<2, 2, 8, 8, T>(a)), dim3(256), TILE256_LDS, s, a);
 }
-// The largest tile that still gives most CUs one
+// Few rows of codes and a long K: k_few (1 x 4096 x 4096 7.1 us, in tiles 10.1; 16 rows 10.0 and 10.4;
+// but 4 x 2048 x 2048 7.6 and 6.7). Else the largest tile that still gives half of the CUs one: 169 tiles
+// of 256 x 256 (M = N = 3328, K = 4096) 38 us, as 128 x 128 50, and 121 tiles (2816) 36 and 35; 144 tiles
+// of 128 x 128 (1500 x 1000 x 1500) 9.6 us, as 64 x 64 9.4, and 64 tiles (1000 x 1000 x 1000) 8.6 and 6.4.
 template <int T>
 void launch_linear(const Args& a, hipStream_t s) {
-  if (a.M <= 16) {
+  if (a.M <= 16 && a.nb > 64)
     hipLaunchKernelGGL((k_few<-1, T>), dim3((unsigned)ceil_div(a.N, 16)), dim3(512), 0, s, FewArgs{a, nullptr, 0, 0});
-    return;
-  }
-  if (a.N >= 256 && a.M >= 256 && tiles_of<2, 2, 8, 8, T>(a) >= 192)
-    launch_tile256<T>(a, s);
+  else if (a.N >= 256 && a.M >= 256 && tiles_of<2, 2, 8, 8, T>(a) >= 128) launch_tile256<T>(a, s);
   else if (tiles_of<2, 2, 4, 4, T>(a) >= 128) launch_tile<2, 2, 4, 4, T>(a, s);
   else launch_tile<2, 2, 2, 2, T>(a, s);
 }
@@ -938,6 +940,7 @@ template <int TX, int T>
 void launch_net(const NetArgs& a, hipStream_t s) {
   int cols = 0;
   for (int d = 0; d < a.depth; ++d) cols = std::max(cols, a.layer[d].N);
+  // (feat_net's 262144 rows: 76 us, in the wide form 115)
   if (a.K <= 192 && cols <= 128) launch_net_as<TX, T, 6, 8, 16>(a, s);
   else launch_net_as<TX, T, 8, 16, 8>(a, s);
 }

@@ -887,35 +887,35 @@ __global__ __launch_bounds__(256) void k_idw_bwd(int64_t S, int C, const float* 
                                                  float* __restrict__ d_out, float* __restrict__ d_w) {
   const int lane = threadIdx.x & 63, k = lane >> 3, q = lane & 7;
   for (int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); s < S; s += (int64_t)gridDim.x * 4) {
-  const int64_t row = 8 * s + k;
-  const float wk = w[row];
-  float dot = 0.f;
-  for (int c = 4 * q; c < C; c += 32) {
-    float g[4];
-    if (c + 4 <= C) {
-      const f32x4 a = *(const Octet<float>::half*)(dh + s * C + c);
+    const int64_t row = 8 * s + k;
+    const float wk = w[row];
+    float dot = 0.f;
+    for (int c = 4 * q; c < C; c += 32) {
+      float g[4];
+      if (c + 4 <= C) {
+        const f32x4 a = *(const Octet<float>::half*)(dh + s * C + c);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) g[j] = a[j];
-    } else {
+        for (int j = 0; j < 4; ++j) g[j] = a[j];
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) g[j] = c + j < C ? dh[s * C + c + j] : 0.f;
-    }
-    if (d_w) {
-      const uint32_t x = *(const uint32_t*)(codes + row * ldc + c);
-      const float sc = pow2_of(scales[row * ss + (c >> 5)]);
+        for (int j = 0; j < 4; ++j) g[j] = c + j < C ? dh[s * C + c + j] : 0.f;
+      }
+      if (d_w) {
+        const uint32_t x = *(const uint32_t*)(codes + row * ldc + c);
+        const float sc = pow2_of(scales[row * ss + (c >> 5)]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (c + j < C) dot = fmaf(q8_value((x >> (8 * j)) & 0xffu, sc), g[j], dot);
+        for (int j = 0; j < 4; ++j)
+          if (c + j < C) dot = fmaf(q8_value((x >> (8 * j)) & 0xffu, sc), g[j], dot);
+      }
+      if (d_out) {
+        const float o[4] = {wk * g[0], wk * g[1], wk * g[2], wk * g[3]};
+        store4<APN_F32>(d_out + row * C + c, C - c, o);
+      }
     }
-    if (d_out) {
-      const float o[4] = {wk * g[0], wk * g[1], wk * g[2], wk * g[3]};
-      store4<APN_F32>(d_out + row * C + c, C - c, o);
-    }
-  }
-  dot += __shfl_xor(dot, 1);
-  dot += __shfl_xor(dot, 2);
-  dot += __shfl_xor(dot, 4);
-  if (d_w && q == 0) d_w[row] = dot;
+    dot += __shfl_xor(dot, 1);
+    dot += __shfl_xor(dot, 2);
+    dot += __shfl_xor(dot, 4);
+    if (d_w && q == 0) d_w[row] = dot;
   }
 }
 
@@ -953,7 +953,7 @@ constexpr int64_t MAX_COLS = (int64_t)1 << 20;   // row widths: 32-bit column ar
 constexpr int64_t MAX_LD = (int64_t)1 << 24;     // row strides: 64 rows within 32 bits of bytes
 
 // The weight gradient's tiles are 192 columns wide where one such tile takes the place of two of 128
-// (dY is read once instead of twice).
+// (dY is read once instead of twice: 203008 x 191 x 128 53 us, with 128 72).
 inline int dw_width(int64_t K) { return K > 128 && K <= 192 ? 192 : 128; }
 inline int64_t dw_tiles(int64_t N, int64_t K) {
   const int64_t kw = dw_width(K);
@@ -991,9 +991,10 @@ void launch_stream(const RowArgs& a, hipStream_t s) {
                      3 * KS * CT * 64 * 16 + 16 * CT * 4, s, a);
 }
 
-// Few tiles: at most one for each wave of a full launch, so the columns are split finer. Few rows:
-// one row of 256 x 256 forward 4.6 us and dX 6.9 us, against 15 us in k_rows; 16 rows of 128 x 128
-// 5.3 and 4.9 us, 17 rows in the streaming kernel 8.2 and 5.3 us.
+// Few tiles: at most one for each wave of a full launch; the columns are then split finer (64 instead
+// of 128 a workgroup: 8192 x 128 x 128 8.8 us against 11.2, but 203008 rows 69 against 65 and 191 columns
+// of dX 104 against 84). Few rows: 16 x 256 x 256 forward 4.9 us and dX 7.3, 15 in k_rows; 16 x 128 x 128
+// 4.2 and 4.8, 6.2 and 5.5 in k_rows_stream.
 constexpr int64_t FEW_TILES = SW * 256, FEW_ROWS = 16;
 
 template <bool WT, bool MASK, bool Q8>
@@ -1010,7 +1011,7 @@ int launch_rows(const RowArgs& a, hipStream_t s) {
   if (stream && few && a.R <= 128) launch_stream<WT, MASK, Q8, 4, 4>(a, s);
   else if (stream && few) launch_stream<WT, MASK, Q8, 6, 4>(a, s);
   else if (stream && a.R <= 128 && a.C > 128 && a.C <= 192)
-    launch_stream<WT, MASK, Q8, 4, 12>(a, s);   // rows read once, not twice
+    launch_stream<WT, MASK, Q8, 4, 12>(a, s);   // rows read once, not twice (dX of 191 columns: 84 us, not 88)
   else if (stream && a.R <= 128) launch_stream<WT, MASK, Q8, 4, 8>(a, s);
   else if (stream) launch_stream<WT, MASK, Q8, 6, 8>(a, s);
   else {
@@ -1109,8 +1110,8 @@ extern "C" int apn_q8_linear_bwd_dw(const float* dy, int64_t ld_dy, const uint8_
   if (!dw) {
     hipLaunchKernelGGL(q8::k_db, dim3((unsigned)ceil_div(N, 64), 1, (unsigned)sp), dim3(512), 0, s, a);
     if (sp > 1)
-      hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)ceil_div(n, 64)), dim3(1024), 0, s, part, sp, n, (int64_t)0, dw,
-                         db);
+      hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)ceil_div(n, 64)), dim3(1024), 0, s, part, sp, n,
+                         (int64_t)0, dw, db);
     return launch_status();
   }
   const int width = q8::dw_width(K);
@@ -1118,7 +1119,8 @@ extern "C" int apn_q8_linear_bwd_dw(const float* dy, int64_t ld_dy, const uint8_
   if (width == 192) q8::launch_dw<3>(a, grid, s);
   else q8::launch_dw<2>(a, grid, s);
   if (sp > 1)
-    hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)ceil_div(n, 64)), dim3(1024), 0, s, part, sp, n, N * K, dw, db);
+    hipLaunchKernelGGL(q8::k_add_splits, dim3((unsigned)ceil_div(n, 64)), dim3(1024), 0, s, part, sp, n, N * K, dw,
+                       db);
   return launch_status();
 }
 

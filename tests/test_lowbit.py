@@ -982,6 +982,12 @@ def test_refusals_gpu(dev):
 
 
 @gpu
+@pytest.mark.parametrize("M,K,N", [(5, 2304, 40), (16, 4100, 70), (8, 130, 33), (9, 2080, 16), (1, 2049, 1)])
+def test_mx4_linear_few_rows_vs_float64(dev, M, K, N):
+    test_mx4_linear_vs_float64(dev, M, K, N, torch.float32)
+
+
+@gpu
 @pytest.mark.parametrize("slopes", [[2.0, None, 2.0], [0.01, 1.0, 1.5], [-2.0, 1.0, 0.0]])
 def test_mx4_sequential_other_slopes(dev, slopes):
     """Slopes of 1, above and below: the stack equals its layers one after the other (the one-launch
