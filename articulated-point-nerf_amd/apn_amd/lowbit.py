@@ -295,6 +295,13 @@ def linear_q8_backward(dy: torch.Tensor, weight: torch.Tensor, x_kept: Q8Rows | 
     xc, xs = x_kept._at if want_w else (None, None)
     empty = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dy.device)  # noqa: E731
     dx = dw = db = None
+    # (dx last: dy is then in the 256 MB cache for it, and dx for the layer below: 99 -> 96 us, 203008 x 128 x 128)
+    if want_w or want_b:
+        dw = empty(N, K) if want_w else None
+        db = empty(N) if want_b else None
+        ws = empty(max(int(L.load().apn_q8_linear_bwd_dw_workspace_bytes(M, N, K)) // 4, 1))
+        _launch(dev, "apn_q8_linear_bwd_dw", dy.data_ptr(), ld_dy, mask, sl, xc, xs, M, N, K,
+                _addr(dw), _addr(db), ws.data_ptr())
     if want_x:
         Kp = -(-K // 4) * 4   # rows of whole 16-byte pieces, as linear's: odd rows written 1.5 x as slowly
         dx = empty(M, Kp)
@@ -302,12 +309,6 @@ def linear_q8_backward(dy: torch.Tensor, weight: torch.Tensor, x_kept: Q8Rows | 
                 dx.data_ptr(), Kp)
         if Kp != K:
             dx = dx[:, :K]
-    if want_w or want_b:
-        dw = empty(N, K) if want_w else None
-        db = empty(N) if want_b else None
-        ws = empty(max(int(L.load().apn_q8_linear_bwd_dw_workspace_bytes(M, N, K)) // 4, 1))
-        _launch(dev, "apn_q8_linear_bwd_dw", dy.data_ptr(), ld_dy, mask, sl, xc, xs, M, N, K,
-                _addr(dw), _addr(db), ws.data_ptr())
     return dx, dw, db
 
 
