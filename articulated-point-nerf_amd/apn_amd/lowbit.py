@@ -129,6 +129,15 @@ def _act(slope, what):
     return 1, slope
 
 
+def _act_backward(slope, what):
+    """The slope of an activation whose derivative is taken from the sign of its output. Below 0 an
+    output is never negative: its sign does not tell the two sides apart."""
+    act, sl = _act(slope, what)
+    if act and sl < 0.0:
+        raise ValueError(f"{what}: no backward pass through a negative slope ({sl}): the kept sign is the output's")
+    return sl
+
+
 class _BlockRows:
     """Codes and scales of [rows, cols] values; ``codes`` uint8 [rows, _BYTES ceil(cols / 32)],
     ``scales`` uint8 [rows, 4 ceil(ceil(cols / 32) / 4)], both contiguous; codes behind column cols
@@ -244,7 +253,8 @@ def q8_pack(x: torch.Tensor) -> Q8Rows:
 def linear_q8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, slope: float | None = None):
     """(y, kept): y [M, N] = act(x weight^T + bias) in float32 and its 8-bit checkpoint, in one pass.
     x [..., K] and weight [N, K] float32; ``slope``: None (no activation), 0 (ReLU) or the LeakyReLU
-    negative slope. The products are f32-accurate."""
+    negative slope (a slope below 0 has no backward pass: ``linear_q8_backward``). The products are
+    f32-accurate."""
     what = "linear_q8"
     if x.dtype != torch.float32 or weight.dtype != torch.float32:
         raise TypeError(f"{what}: float32 only, got {x.dtype} and {weight.dtype}")
@@ -266,7 +276,8 @@ def linear_q8_backward(dy: torch.Tensor, weight: torch.Tensor, x_kept: Q8Rows | 
     output: g = dy * (y > 0 ? 1 : slope), dx = g weight, dw = g^T x', db = sum g, with x' the
     values of ``x_kept``. ``need``: which of the three are computed (None for the others; x_kept
     may be None without dw). A gradient masked by slope 0 is 0 whatever dy holds there. Sums over
-    the rows are taken in a fixed order."""
+    the rows are taken in a fixed order. ``slope`` is at least 0 (else ValueError): the derivative comes
+    from the sign bit of y's codes, which is that of the activation's input only then."""
     what = "linear_q8_backward"
     want_x, want_w, want_b = need
     for kept, name in ((x_kept, "x_kept"), (y_kept, "y_kept")):
@@ -284,7 +295,7 @@ def linear_q8_backward(dy: torch.Tensor, weight: torch.Tensor, x_kept: Q8Rows | 
         raise ValueError(f"{what}: x_kept is {x_kept.shape}, expected {(M, K)}")
     if y_kept is not None and y_kept.shape != (M, N):
         raise ValueError(f"{what}: y_kept is {y_kept.shape}, expected {(M, N)}")
-    _, sl = _act(slope, what)
+    sl = _act_backward(slope, what)
     if slope is not None and y_kept is None:
         raise ValueError(f"{what}: an activation needs y_kept")
     dev = _device(what, dy, w)
@@ -378,7 +389,7 @@ def sequential_q8(layers, x: torch.Tensor, col_pos=None, keep_output=False):
     """A stack of (torch.nn.Linear, slope) pairs under autograd with 8-bit activation checkpoints:
     between forward and backward no float row of the stack is kept, only the 8-bit checkpoint of x
     and of each layer's output. ``col_pos``: linear.linear's. With ``keep_output`` returns
-    (y, Q8Rows of y).
+    (y, Q8Rows of y). Slopes are at least 0 (linear_q8_backward).
 
     Not under graph capture: a captured backward reaches the parameters' gradient accumulators, and
     one that an eager step created earlier on another stream ends the capture and with it the
@@ -387,6 +398,8 @@ def sequential_q8(layers, x: torch.Tensor, col_pos=None, keep_output=False):
     layers = list(layers)
     if not layers:
         raise ValueError(f"{what}: no layers")
+    for _, slope in layers:
+        _act_backward(slope, what)
     L.require_cuda(x, what=what)
     _not_captured(what)
     params = [p for layer, _ in layers for p in (layer.weight, layer.bias)]

@@ -112,7 +112,8 @@ struct RowArgs {
   float slope;
 };
 
-// the gradient through the activation; slope 0 gives 0 whatever g holds
+// The gradient through the activation; slope 0 gives 0 whatever g holds. The output's sign is the
+// input's only for slopes of 0 and above (the entry points refuse others).
 __device__ __forceinline__ float masked(float g, uint32_t code, float slope) {
   return code & 0x80u ? (slope == 0.f ? 0.f : g * slope) : g;
 }
@@ -1076,7 +1077,7 @@ extern "C" int apn_q8_linear_bwd_dx(const float* dy, int64_t ld_dy, const uint8_
   if (M < 0 || N < 1 || K < 1 || N > q8::MAX_COLS || K > q8::MAX_COLS || ld_dy < N || ldw < K || ld_dx < K)
     return APN_ERR_ARG;
   if (M == 0) return APN_OK;
-  if (!dy || !w || !dx || (uintptr_t)y_codes % 16) return APN_ERR_ARG;
+  if (!dy || !w || !dx || (uintptr_t)y_codes % 16 || (y_codes && !(slope >= 0.f))) return APN_ERR_ARG;
   q8::RowArgs a{dy, y_codes, w, nullptr, dx, nullptr, nullptr, M, ld_dy, blocks_of(N) * BLK, ldw, ld_dx, 0, (int)N,
                 (int)K, 0, 0, slope};
   hipStream_t s = (hipStream_t)stream;
@@ -1094,7 +1095,8 @@ extern "C" int apn_q8_linear_bwd_dw(const float* dy, int64_t ld_dy, const uint8_
   if (M < 0 || N < 1 || K < 1 || N > q8::MAX_COLS || K > q8::MAX_COLS || ld_dy < N) return APN_ERR_ARG;
   if (!dw && !db) return APN_OK;
   if (M > 0 && (!dy || !workspace || (dw && (!x_codes || !x_scales)))) return APN_ERR_ARG;
-  if ((uintptr_t)y_codes % 16 || (uintptr_t)x_codes % 16 || ld_dy >= q8::MAX_LD) return APN_ERR_ARG;
+  if ((uintptr_t)y_codes % 16 || (uintptr_t)x_codes % 16 || ld_dy >= q8::MAX_LD || (y_codes && !(slope >= 0.f)))
+    return APN_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   if (M == 0) {   // no rows: zero gradients
     if (dw) APN_TRY(fill_i32((int*)dw, 0, N * K, s));

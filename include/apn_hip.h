@@ -505,9 +505,10 @@ int apn_q8_linear_fwd(const float* x, int64_t ldx, const float* w, int64_t ldw, 
                       int64_t N, int64_t K, int32_t act, float slope, float* y, int64_t ldy, uint8_t* codes,
                       uint8_t* scales, void* stream);
 /* Its backward from the checkpoints. G = dy * (code of y positive ? 1 : slope), G = dy when
- * y_codes is NULL: dx [M, K] = G w;  dw [N, K] = G^T x', db [N] = sum_m G (either may be NULL), with x' the
- * values of x's checkpoint. workspace: apn_q8_linear_bwd_dw_workspace_bytes(M, N, K); partial sums
- * are added in a fixed order. ld_dy < 2^24 for dw and db. */
+ * y_codes is NULL; with y_codes slope >= 0 (below 0 no output is negative, and its sign does not say
+ * on which side its input was): dx [M, K] = G w;  dw [N, K] = G^T x', db [N] = sum_m G (either may be
+ * NULL), with x' the values of x's checkpoint. workspace: apn_q8_linear_bwd_dw_workspace_bytes(M, N,
+ * K); partial sums are added in a fixed order. ld_dy < 2^24 for dw and db. */
 int apn_q8_linear_bwd_dx(const float* dy, int64_t ld_dy, const uint8_t* y_codes, float slope, const float* w,
                          int64_t ldw, int64_t M, int64_t N, int64_t K, float* dx, int64_t ld_dx, void* stream);
 size_t apn_q8_linear_bwd_dw_workspace_bytes(int64_t M, int64_t N, int64_t K);

@@ -1020,3 +1020,60 @@ def test_mx4_sequential_overflow(dev):
     want = torch.ones(20, 16, device=dev)
     want[5] = math.nan
     assert torch.equal(torch.nan_to_num(y, nan=7.0), torch.nan_to_num(want, nan=7.0))
+
+
+# --- the activation's side, from the output's sign ------------------------------------------------------
+
+def test_negative_slopes_have_no_backward_cpu():
+    """With a slope below 0 every output of the activation is positive, so the checkpoint's sign does
+    not say on which side of the kink its input was: such a backward is refused, before anything runs."""
+    from apn_amd import _lib, linear as LIN, lowbit as lb
+    x, w = torch.zeros(4, 33), torch.zeros(5, 33)
+    with pytest.raises(ValueError, match="slope"):
+        lb.linear_q8_backward(torch.zeros(4, 5), w, None, None, -0.5, (True, False, False))
+    with pytest.raises(ValueError, match="slope"):
+        lb.sequential_q8([(torch.nn.Linear(33, 5), 0.01), (torch.nn.Linear(5, 5), -0.5)], x)
+    # the CPU form of a stack runs torch's own modules, whatever its slopes
+    net = torch.nn.Sequential(torch.nn.Linear(33, 5), torch.nn.LeakyReLU(-0.5))
+    assert torch.equal(LIN.sequential(net, x + 1, checkpoint="q8"), net(x + 1))
+    lib, p = _lib.load(), 4096    # a pointer that is never followed
+    for slope in (-0.5, math.nan):
+        assert lib.apn_q8_linear_bwd_dx(p, 8, p, slope, p, 32, 4, 8, 32, p, 32, None) == 1
+        assert lib.apn_q8_linear_bwd_dw(p, 8, p, slope, p, p, 4, 8, 32, p, p, p, None) == 1
+
+
+@gpu
+@autograd
+def test_negative_slopes_are_refused_under_autograd(dev):
+    from apn_amd import linear as LIN, lowbit as lb
+    x, w, b, dy = _rand(40, 24, 33, 12, dev)
+    y, kept = lb.linear_q8(x, w, b, -0.5)
+    with pytest.raises(ValueError, match="slope"):
+        lb.linear_q8_backward(dy, w, lb.q8_pack(x), kept, -0.5)
+    net = _stack(dev, [33, 24, 8], [-0.5, 0.01], 13)
+    with pytest.raises(ValueError, match="slope"):
+        LIN.sequential(net, x, checkpoint="q8")
+    assert lb.linear_q8_backward(dy, w, lb.q8_pack(x), kept, -0.0)[0].shape == x.shape   # -0 is ReLU's
+
+
+@gpu
+@pytest.mark.parametrize("slope", [0.0, 1e-30, 0.01, 1.0, 2.0])
+@pytest.mark.parametrize("M,K,N", [(3, 40, 33), (70, 70, 34), (500, 250, 66)])
+def test_linear_q8_backward_gates_on_the_input_of_the_activation(dev, M, K, N, slope):
+    """The derivative belongs to the activation's input v, not to its output: the gradients from
+    ``linear_q8``'s own checkpoint against the formula in 64 bits with v from the same product without
+    its activation (the same sums, so the same sign), an exact 0 among them."""
+    from apn_amd import lowbit as lb
+    x, w, b, dy = _rand(M, N, K, M + N, dev)
+    x[1], b[::5] = 0.0, 0.0          # v = 0 in every fifth column of row 1
+    v, _ = lb.linear_q8(x, w, b, None)
+    _, kept = lb.linear_q8(x, w, b, slope)
+    xk = lb.q8_pack(x)
+    dx, dw, db = lb.linear_q8_backward(dy, w, xk, kept, slope)
+    g = torch.where(v > 0, dy.double(), dy.double() * slope)
+    xv = ref_q8(x)[2].to(dev)
+    # (below 2^-110 a factor of a product is cut at bf16's smallest step: each is off by at most 2^-133)
+    tiny = 2.0 ** -133
+    _within(dx, g @ w.double(), _bound(N, g.abs() @ w.double().abs()) + tiny * N * float(w.abs().max()) + tiny)
+    _within(dw, (xv.t() @ g).t(), _bound(M, (xv.abs().t() @ g.abs()).t()) + tiny * M * float(xv.abs().max()) + tiny)
+    _within(db, g.sum(0), _bound(M, g.abs().sum(0)) + tiny * M)
