@@ -36,6 +36,8 @@ class _GemmLinear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, slope, col_pos=None):
         if x.dtype != torch.float32 or weight.dtype != torch.float32:
             raise TypeError("apn linear: float32 only")
+        if slope is not None and slope < 0:
+            raise ValueError(f"apn linear: the output's sign gives no derivative for a negative slope ({slope})")
         dev = x.device
         x2 = x.reshape(-1, x.shape[-1])
         if x2.stride(-1) != 1 or x2.stride(0) < x2.shape[1]:
@@ -123,6 +125,8 @@ def linear(x: torch.Tensor, layer: torch.nn.Linear, slope=None, col_pos=None) ->
         if slope is None:
             return y
         return torch.relu(y) if slope == 0 else torch.nn.functional.leaky_relu(y, slope)
+    if slope is not None and slope < 0:   # no output is negative then: the activation keeps its own input
+        return torch.nn.functional.leaky_relu(_GemmLinear.apply(x, layer.weight, layer.bias, None, col_pos), slope)
     return _GemmLinear.apply(x, layer.weight, layer.bias, slope, col_pos)
 
 

@@ -220,3 +220,47 @@ def test_gemm_linear_padded_rows_equal_contiguous():
         res.append([y.detach()] + [p.grad for p in ps])
     for u, v in zip(*res):
         assert torch.equal(u, v)
+
+
+def test_gemm_linear_fused_activation_refuses_negative_slopes():
+    """The fused layer takes the activation's derivative from the sign of its output, which with a
+    negative slope is never negative."""
+    from apn_amd.linear import _GemmLinear
+    with pytest.raises(ValueError, match="slope"):
+        _GemmLinear.apply(torch.zeros(4, 3), torch.zeros(5, 3), torch.zeros(5), -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.autograd
+@pytest.mark.parametrize("M,K,N", [(1, 33, 20), (300, 70, 130), (2000, 128, 5)])
+def test_linear_negative_slope_vs_float64(M, K, N):
+    """A Linear layer with LeakyReLU(-0.5), by itself and within a Sequential: output and all gradients
+    against the formula in 64 bits, the derivative taken at the activation's input (from the same
+    product without activation: the same sums, so the same sign). A float32 sum of n products in any
+    order is off by at most (n + 16) 2^-23 of the sum of their magnitudes."""
+    from apn_amd.linear import linear, sequential
+    dev = torch.device("cuda")
+    torch.manual_seed(M + N)
+    layer = torch.nn.Linear(K, N).to(dev)
+    x = torch.randn(M, K, device=dev, requires_grad=True)
+    dy = torch.randn(M, N, device=dev)
+    x64, w64, b64 = x.detach().double(), layer.weight.detach().double(), layer.bias.detach().double()
+    with torch.no_grad():
+        v = linear(x, layer)
+    pre = x64 @ w64.t() + b64
+    g = torch.where(v > 0, dy.double(), dy.double() * -0.5)
+    S = x64.abs() @ w64.abs().t() + b64.abs()
+    u = 2.0 ** -23
+    want = {"y": (torch.where(v > 0, pre, pre * -0.5), (K + 16) * u * S),
+            "dx": (g @ w64, (N + 16) * u * (g.abs() @ w64.abs())),
+            "dw": (g.t() @ x64, (M + 16) * u * (g.abs().t() @ x64.abs())),
+            "db": (g.sum(0), (M + 16) * u * g.abs().sum(0))}
+    for run in (lambda: linear(x, layer, -0.5),
+                lambda: sequential(torch.nn.Sequential(layer, torch.nn.LeakyReLU(-0.5)), x)):
+        x.grad = None
+        layer.zero_grad(set_to_none=True)
+        y = run()
+        y.backward(dy)
+        got = {"y": y.detach(), "dx": x.grad, "dw": layer.weight.grad, "db": layer.bias.grad}
+        for k, (ref, bound) in want.items():
+            assert float(((got[k].double() - ref).abs() - bound).max()) <= 0, k
