@@ -371,7 +371,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(Args p) {
 // operands straight from memory into LDS (no registers on the way), four buffers of one step (32 KB)
 // so that three steps are on their way: a step is 0.5 us of matrix work and L2 answers in about 1 us
 // (with one step on its way in registers the 8192 x 4096 x 4096 product took 150 us, with two 119; here
-// 84, of which the products alone are 50, the results' stores 13 and their arithmetic 3). Bound by the
+// 85, of which the products alone are 50, the results' stores 13 and their arithmetic 3). Bound by the
 // matrix units' rate under load, the loads beside them, and an epilogue that nothing hides.
 // The LDS side of such a load is lane by lane, so the lanes choose what they read: row lane / 4, and
 // of its four blocks the one that lands conflict-free -- slot 4 r + (c ^ r / 4) of a 16-row tile. The
@@ -380,15 +380,21 @@ __device__ __forceinline__ uint32_t lds_at(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
 }
 // 64 lanes x W bytes from base + lane bytes to LDS byte address `to` + W lane; arrives under vmcnt
-// (no register is written, so nothing waits for it but the kernel's own s_waitcnt; m0 is set for the
-// load alone, the compiler keeps nothing in it; one wait state between m0 and its use)
+// (no register is written by the load, so nothing waits for it but the kernel's own s_waitcnt). m0
+// is the compiler's, and a clobber of it is not honoured: it is put back behind the load, which reads
+// it when it is issued. One wait state between m0 and its use.
 template <int W>
 __device__ __forceinline__ void to_lds(const uint8_t* base, uint32_t lane_bytes, uint32_t to) {
+  uint32_t kept;
   if (W == 16)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(lane_bytes), "s"(base)
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(kept)
+                 : "s"(to), "v"(lane_bytes), "s"(base)
                  : "memory");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(lane_bytes), "s"(base)
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %2, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(kept)
+                 : "s"(to), "v"(lane_bytes), "s"(base)
                  : "memory");
 }
 // at most N loads out, LDS reads done, all waves here

@@ -59,3 +59,23 @@ def test_no_packed_fp32_valu_in_device_code(lib):
     assert "v_mfma_f32_16x16x32_f16" in allcode                # really the MLP kernels' ISA
     bad = [ln.strip() for ln in allcode.splitlines() if PACKED_F32.search(ln)]
     assert not bad, f"{len(bad)} packed-FP32 VALU instructions, e.g. {bad[:3]}"
+
+
+@pytest.mark.parametrize("lib", LIBS, ids=["product", "debug"])
+def test_lds_loads_put_m0_back(lib):
+    """The loads straight into LDS (inline assembly) take their LDS address from m0, a register that
+    belongs to the compiler and whose clobber it does not honour: each of them saves m0 and puts it back."""
+    if not os.path.exists(lib):
+        pytest.skip(f"{os.path.basename(lib)} not built")
+    loads = 0
+    for text in _disassemble_device_code(lib):
+        lines = [ln.split("//")[0].split() for ln in text.splitlines() if ln.startswith("\t")]
+        for i, ln in enumerate(lines):
+            if not ln or not ln[0].startswith("global_load_lds_"):
+                continue
+            loads += 1
+            save, move, wait, back = lines[i - 3], lines[i - 2], lines[i - 1], lines[i + 1]
+            assert save[0] == "s_mov_b32" and save[2] == "m0", save
+            assert move[:2] == ["s_mov_b32", "m0,"] and wait[0] == "s_nop", (move, wait)
+            assert back == ["s_mov_b32", "m0,", save[1].rstrip(",")], (save, back)
+    assert loads > 0
