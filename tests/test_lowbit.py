@@ -1077,3 +1077,37 @@ def test_linear_q8_backward_gates_on_the_input_of_the_activation(dev, M, K, N, s
     _within(dx, g @ w.double(), _bound(N, g.abs() @ w.double().abs()) + tiny * N * float(w.abs().max()) + tiny)
     _within(dw, (xv.t() @ g).t(), _bound(M, (xv.abs().t() @ g.abs()).t()) + tiny * M * float(xv.abs().max()) + tiny)
     _within(db, g.sum(0), _bound(M, g.abs().sum(0)) + tiny * M)
+
+
+# --- forms that no case above reaches, or does not show to be reached -----------------------------------
+
+def _entries(monkeypatch, lb):
+    """The list that the entry points launched from now on are put into."""
+    seen = []
+    launch = lb._launch
+    monkeypatch.setattr(lb, "_launch", lambda dev, entry, *args: (seen.append(entry), launch(dev, entry, *args))[1])
+    return seen
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,sizes,slope", [(1, [1, 1, 1], 0.0), (17, [31, 33, 5], 0.01), (5000, [192, 128, 128], 0.0),
+                                           (333, [256, 256, 256, 256, 256], 0.01), (100, [129, 130, 1, 7], -0.5),
+                                           (40, [8] * 9, None), (65, [191, 64, 255, 30], None), (1000, [256, 128, 128, 128, 128], 0.01)])
+def test_mx4_stack_takes_one_launch(dev, monkeypatch, M, sizes, slope, dtype):
+    """Stacks up to the one-launch form's limits run in it, and their results are those of the layers one
+    by one, bit for bit: small whole numbers, so that every sum is exact in any order."""
+    from apn_amd import lowbit as lb
+    g = torch.Generator(device=dev).manual_seed(sum(sizes) + M)
+    ints = lambda top, *shape: torch.randint(-top, top + 1, shape, device=dev, generator=g).float()  # noqa: E731
+    packed = [lb.MX4Layer(lb.mx4_quantize(ints(3, n, k)), ints(2, n) if i != 1 else None, slope)
+              for i, (k, n) in enumerate(zip(sizes[:-1], sizes[1:]))]
+    x = ints(6, M, sizes[0] + 3).to(dtype)[:, 1:sizes[0] + 1]
+    h = x
+    for p in packed:
+        h = lb.mx4_linear(h, p.weight, p.bias, p.slope)
+    seen = _entries(monkeypatch, lb)
+    for out_dtype in (torch.float32, torch.bfloat16, torch.float16):
+        y = lb.mx4_sequential(packed, x, out_dtype)
+        assert torch.equal(y, h.to(out_dtype))
+    assert seen == ["apn_mx4_network"] * 3
