@@ -1111,3 +1111,35 @@ def test_mx4_stack_takes_one_launch(dev, monkeypatch, M, sizes, slope, dtype):
         y = lb.mx4_sequential(packed, x, out_dtype)
         assert torch.equal(y, h.to(out_dtype))
     assert seen == ["apn_mx4_network"] * 3
+
+
+@gpu
+@pytest.mark.parametrize("x_dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,K,N", [(1, 8193, 17), (8, 16500, 33), (9, 33, 20), (12, 8200, 16), (16, 130, 40), (16, 20000, 31)])
+def test_mx4_few_float_rows_entry_vs_float64(dev, M, K, N, x_dtype):
+    """``apn_mx4_linear_few`` itself over all its row counts (the Python call takes it up to 8 rows), and
+    over reductions of more than one panel of 8192 columns; more rows are refused."""
+    from apn_amd import _lib, lowbit as lb
+    x, w, b, _ = _rand(M, N, K, M + K + N, dev)
+    x = x.to(x_dtype)
+    wq = lb.mx4_quantize(w)
+    out = torch.full((M + 1, N + 2), 7.0, device=dev)
+    lb._launch(dev.index or 0, "apn_mx4_linear_few", x.data_ptr(), lb._TYPES[x_dtype], K, *wq._at, b.data_ptr(), M, N, K,
+               1, 0.01, out.data_ptr(), 0, N + 2)
+    xv, wv = ref_mx4(x.float())[2].to(dev), ref_mx4(w)[2].to(dev)
+    S = xv.abs() @ wv.abs().t() + b.double().abs()
+    _within(out[:M, :N], _act64(xv @ wv.t() + b.double(), 0.01), (K + 16) * U * S)
+    assert (out[M] == 7.0).all() and (out[:, N:] == 7.0).all()      # nothing behind the rows and columns
+    with pytest.raises(_lib.APNError):
+        lb._launch(dev.index or 0, "apn_mx4_linear_few", x.data_ptr(), 0, K, *wq._at, None, 17, N, K, 0, 0.0,
+                   out.data_ptr(), 0, N + 2)
+
+
+@gpu
+@pytest.mark.parametrize("M,K,N", [(1, 8193, 40), (16, 16500, 33)])
+def test_mx4_few_coded_rows_of_several_panels(dev, M, K, N):
+    from apn_amd import lowbit as lb
+    x, w, b, _ = _rand(M, N, K, M + K + N, dev)
+    xq, wq = lb.mx4_quantize(x), lb.mx4_quantize(w)
+    xv, wv = ref_mx4(x)[2].to(dev), ref_mx4(w)[2].to(dev)
+    _within(lb.mx4_linear(xq, wq, b), xv @ wv.t() + b.double(), (K + 16) * U * (xv.abs() @ wv.abs().t() + b.double().abs()))
