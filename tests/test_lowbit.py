@@ -1143,3 +1143,19 @@ def test_mx4_few_coded_rows_of_several_panels(dev, M, K, N):
     xq, wq = lb.mx4_quantize(x), lb.mx4_quantize(w)
     xv, wv = ref_mx4(x)[2].to(dev), ref_mx4(w)[2].to(dev)
     _within(lb.mx4_linear(xq, wq, b), xv @ wv.t() + b.double(), (K + 16) * U * (xv.abs() @ wv.abs().t() + b.double().abs()))
+
+
+@gpu
+@pytest.mark.parametrize("slope", [None, 0.0, 0.01])
+@pytest.mark.parametrize("M,K,N", [(49200, 100, 150), (49200, 150, 100), (49155, 191, 192), (49200, 256, 128)])
+def test_linear_q8_many_rows_every_form(dev, M, K, N, slope):
+    """Row counts past the fine column split, so that each wide form of the rows kernels runs (reductions
+    up to 128 and 192 columns and above, outputs up to 128 and 192), forward and dX with and without
+    signs. A factor whose parts were cut or kept wrong is off by 2^-8 of itself."""
+    test_linear_q8_vs_float64(dev, M, K, N, slope)
+    from apn_amd import lowbit as lb
+    _, w, _, dy = _rand(M, N, K, 3, dev)
+    y = torch.randn(M, N, device=dev, generator=torch.Generator(device=dev).manual_seed(4))
+    dx = lb.linear_q8_backward(dy, w, None, lb.q8_pack(y), slope, (True, False, False))[0]
+    g = dy.double() if slope is None else torch.where(y > 0, dy.double(), dy.double() * slope)
+    _within(dx, g @ w.double(), _bound(N, g.abs() @ w.double().abs()))
