@@ -1159,3 +1159,48 @@ def test_linear_q8_many_rows_every_form(dev, M, K, N, slope):
     dx = lb.linear_q8_backward(dy, w, None, lb.q8_pack(y), slope, (True, False, False))[0]
     g = dy.double() if slope is None else torch.where(y > 0, dy.double(), dy.double() * slope)
     _within(dx, g @ w.double(), _bound(N, g.abs() @ w.double().abs()))
+
+
+@gpu
+@autograd
+def test_pose_embedding_scene_with_checkpoints_then_preview(dev, monkeypatch):
+    """A model with a pose embedding, whose first feat_net layer is 256 columns wide (the general rows
+    kernel, the wide form of the one-launch stack): a training step with 8-bit checkpoints against the
+    plain step, then a frame with feat_net in 4 bits, each through the operators. A kept value is within
+    2^-7 of its block's largest magnitude, about 3 of the block's root mean square: 0.03 of a gradient
+    whose terms do not cancel (feat_net's own), several times that of those reached through the blend
+    weights alone, where they partly do."""
+    from apn_amd import harness, lowbit as lb, synthetic as S
+    scene = S.make_scene("G2")
+    model = harness.build_model(scene, dev)
+    rk = scene.render_kwargs(dev)
+    t = torch.tensor([scene.cfg.t], device=dev)
+    with torch.no_grad():
+        target = model(t + 0.1, render_kwargs=rk)["rgb_marched"].clone()
+    seen = _entries(monkeypatch, lb)
+    runs = []
+    for ck in (None, "q8"):
+        model.activation_checkpoint = ck
+        model.zero_grad(set_to_none=True)
+        out = model(t, render_kwargs=rk)
+        torch.nn.functional.mse_loss(out["rgb_marched"], target).backward()
+        runs.append((out["rgb_marched"].detach(), {k: p.grad.clone() for k, p in model.named_parameters()
+                                                   if p.grad is not None}))
+        assert bool(seen) == (ck == "q8")
+    assert {"apn_q8_pack", "apn_q8_linear_fwd", "apn_q8_linear_bwd_dw", "apn_q8_linear_bwd_dx"} == set(seen)
+    assert model.feat_net[0].weight.shape[1] + 1 == 256     # and one column of padding behind the 63 of the position
+    (a, ga), (b, gb) = runs
+    assert float((a - b).abs().max()) < 1e-5
+    assert set(ga) == set(gb) and any(k.startswith("pose_embedding_net") for k in ga)
+    for k in ga:
+        bound = 0.03 if k.startswith("feat_net") else 0.1
+        assert float((ga[k] - gb[k]).norm()) <= bound * float(ga[k].norm()) + 1e-12, k
+    model.activation_checkpoint = None
+    del seen[:]
+    with torch.no_grad():
+        full = model(t, render_kwargs=rk)["rgb_marched"].clone()
+        model.feat_format = "mx4"
+        low = model(t, render_kwargs=rk)["rgb_marched"].clone()
+    assert set(seen) == {"apn_mx4_quantize", "apn_mx4_network"}
+    assert torch.isfinite(low).all() and not torch.equal(low, full)
+    assert float((low - full).square().mean()) < 0.05 ** 2
