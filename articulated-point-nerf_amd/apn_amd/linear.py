@@ -170,8 +170,8 @@ def sequential(net: torch.nn.Module, x: torch.Tensor, col_pos=None, checkpoint=N
     """A Sequential of Linear / LeakyReLU / ReLU (nested Sequentials flattened): each Linear runs
     with the activation that follows it fused into its epilogue (``col_pos``: the first layer's,
     see linear). ``checkpoint="q8"`` (device tensors under autograd): between forward and backward
-    the rows of consecutive Linear layers are kept in 8 bits (lowbit.sequential_q8) instead of
-    float32; elsewhere it changes nothing."""
+    the rows of consecutive Linear layers are kept in 8 bits (lowbit.sequential_q8: slopes of 0 and
+    above) instead of float32; elsewhere it changes nothing."""
     if checkpoint not in (None, "q8"):
         raise ValueError(f"apn linear: checkpoint must be None or 'q8', got {checkpoint!r}")
     q8 = checkpoint == "q8" and x.is_cuda and torch.is_grad_enabled()

@@ -5,10 +5,10 @@
 //
 //   q8   code = (x > 0 ? 0 : 0x80) | q, q = min(rint(|x| / 2^s), 127): the sign bit answers
 //        "was the activation's output positive" exactly, also where q rounds to 0, so the backward
-//        pass takes the LeakyReLU derivative from it. s is the smallest exponent that holds the
-//        block's largest magnitude in 7 bits after rounding. Half a step of rounding: at most
-//        2^-7 of the block's largest magnitude (the power of two costs up to one bit against a
-//        free scale; it makes scaling exact and q 2^s exact in bf16, the matrix operand).
+//        pass takes the LeakyReLU derivative from it (slopes of 0 and above). s is the smallest
+//        exponent that holds the block's largest magnitude in 7 bits after rounding. Half a step of
+//        rounding: at most 2^-7 of the block's largest magnitude (the power of two costs up to one
+//        bit against a free scale; it makes scaling exact and q 2^s exact in bf16, the matrix operand).
 //   mx4  nibble = sign << 3 | index into {0, .5, 1, 1.5, 2, 3, 4, 6}; s = floor(log2 max|x|) - 2
 //        (the OCP microscaling conversion: the largest magnitude lands in [4, 8) and saturates
 //        at 6), nearest, ties to even.

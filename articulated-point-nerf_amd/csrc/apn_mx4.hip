@@ -655,9 +655,10 @@ __global__ __launch_bounds__(512) void k_few(FewArgs f) {
 // is 8 values of each of a row's four lanes, its codes 32 bits a lane, and four blocks transposed over
 // the four lanes are the next product's operand: lane q the 16 B of block 4 s + q. The input's floats
 // come in the same arrangement (four lanes on 64 B of a row), the next tile's while this one is
-// computed. 262144 rows through 191-128-128-128-128 take 76 us, the input and output rows' 52 us at a
-// copy's rate; bound by vector instructions (about 1100 a tile: with compares and selects for the
-// activations 1580 and 95 us) and by the registers that the rows on their way leave.
+// computed. 262144 rows through 191-128-128-128-128 take 77 us (84 with f32 output), the input and output
+// rows' 52 us (66) at a copy's rate; half of the cycles are vector instructions (1280 a tile; with
+// compares and selects for the activations 95 us), the rest mostly waits for rows, of which the registers
+// leave few on their way.
 struct NetLayer {
   const uint8_t* codes;
   const uint8_t* scales;

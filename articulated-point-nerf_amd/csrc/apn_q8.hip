@@ -8,12 +8,13 @@
 //
 // f32 products on the bf16 matrix units: every f32 factor is cut (not rounded) into three bf16
 // numbers hi + mid + lo whose 3 x 8 mantissa bits are its 24 exactly, and
-//   x w = hi hi + (hi mid + mid hi) + (hi lo + mid mid + lo hi) + (<= 2^-22 |x w|, left out)
-// with f32 accumulation: six bf16 products, 2.5 PFLOP/s / 6 = 416 TFLOP/s against 157 of the
-// f32-input MFMA. A checkpoint factor q 2^s is one exact bf16 number, so dW takes three. Values
-// below 2^-110 lose mantissa bits to bf16's smallest subnormal (2^-133, absolute). An infinity
-// makes its row's outputs NaN (inf - inf in the cut, inf * 0 in the products): non-finite stays
-// non-finite.
+//   x w = hi hi + (hi mid + mid hi) + (hi lo + mid mid + lo hi) + (<= 2^-21 |x w|, left out)
+// (mid < 2^-7 and lo < 2^-15 of the factor; what is left out has the product's own sign, so a sum of
+// products of one sign loses it in one direction) with f32 accumulation: six bf16 products, 2.5 PFLOP/s
+// / 6 = 416 TFLOP/s against 157 of the f32-input MFMA. A checkpoint factor q 2^s is one exact bf16
+// number, so dW takes three. Values below 2^-110 lose mantissa bits to bf16's smallest subnormal
+// (2^-133, absolute). An infinity makes its row's outputs NaN (inf - inf in the cut, inf * 0 in the
+// products): non-finite stays non-finite.
 #include "apn_lowbit.h"
 
 #include <algorithm>
@@ -477,8 +478,8 @@ __global__ __launch_bounds__(512, 4) void k_rows(RowArgs p) {
     }
   };
   auto stage = [&](u32x4* sh) __attribute__((always_inline)) {
-    // (registers of their own: left in the loads' tuple, the compiler lets the cut parts overwrite an
-    // octet's elements before their use)
+    // (registers of their own: in an earlier form of this loop the compiled code let the cut parts overwrite
+    // an octet's elements before their use)
 #pragma unroll
     for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(xv[j]), "+v"(wv[j]));
     if (MASK) {
