@@ -1091,16 +1091,24 @@ def _entries(monkeypatch, lb):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("M,sizes,slope", [(1, [1, 1, 1], 0.0), (17, [31, 33, 5], 0.01), (5000, [192, 128, 128], 0.0),
-                                           (333, [256, 256, 256, 256, 256], 0.01), (100, [129, 130, 1, 7], -0.5),
-                                           (40, [8] * 9, None), (65, [191, 64, 255, 30], None), (1000, [256, 128, 128, 128, 128], 0.01)])
+@pytest.mark.parametrize("M,sizes,slope", [(1, [1, 1, 1], 0.0), (17, [31, 33, 5], 0.5), (5000, [192, 128, 128], 0.0),
+                                           (333, [256, 256, 256, 256, 256], 0.5), (100, [129, 130, 1, 7], -0.5),
+                                           (40, [8] * 9, None), (65, [191, 64, 255, 30], None), (1000, [256, 128, 128, 128, 128], 0.5)])
 def test_mx4_stack_takes_one_launch(dev, monkeypatch, M, sizes, slope, dtype):
     """Stacks up to the one-launch form's limits run in it, and their results are those of the layers one
-    by one, bit for bit: small whole numbers, so that every sum is exact in any order."""
+    by one, bit for bit, because every sum is exact in any order: inputs are whole numbers up to 6, a
+    weight row has at most four entries of 1 or -1, biases are up to 2, and quantising (to at most 5/4 of
+    the block's largest) keeps multiples of a power of two. A layer's sums are thus at most 5 times its
+    inputs and 2: below 2^22 after 8 layers (slope None), below 2^13 and multiples of 2^-4 after 4 (slopes
+    of 1/2)."""
     from apn_amd import lowbit as lb
     g = torch.Generator(device=dev).manual_seed(sum(sizes) + M)
     ints = lambda top, *shape: torch.randint(-top, top + 1, shape, device=dev, generator=g).float()  # noqa: E731
-    packed = [lb.MX4Layer(lb.mx4_quantize(ints(3, n, k)), ints(2, n) if i != 1 else None, slope)
+
+    def weight(n, k):
+        w = torch.zeros(n, k, device=dev)
+        return w.scatter_(1, torch.randint(0, k, (n, min(k, 4)), device=dev, generator=g), ints(1, n, min(k, 4)))
+    packed = [lb.MX4Layer(lb.mx4_quantize(weight(n, k)), ints(2, n) if i != 1 else None, slope)
               for i, (k, n) in enumerate(zip(sizes[:-1], sizes[1:]))]
     x = ints(6, M, sizes[0] + 3).to(dtype)[:, 1:sizes[0] + 1]
     h = x
